@@ -10,6 +10,7 @@
 #include <string>
 #include <vector>
 
+#include "capi_guard.h"
 #include "common.cuh"
 #include "gptoss.h"
 #include "engine.h"
@@ -22,16 +23,14 @@ thread_local std::string g_error;
 
 template <class F>
 int guard(F&& f) {
-    try {
-        f();
-        return 0;
-    } catch (const std::exception& e) {
-        g_error = e.what();
-    } catch (...) {
-        g_error = "unknown error";
-    }
-    return -1;
+    return gpt::abi_guard(f);
 }
+
+}  // namespace
+
+std::string& gpt::last_error_slot() { return g_error; }
+
+namespace {
 
 void sync_check(const char* what) {
     const cudaError_t e = cudaDeviceSynchronize();

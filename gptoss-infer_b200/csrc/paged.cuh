@@ -1,0 +1,113 @@
+// Device helpers of the paged cache kernels.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "paged.h"
+
+namespace gpt {
+namespace paged {
+
+__device__ __forceinline__ void report(int* err, int code) { atomicCAS(err, 0, code); }
+
+// The sequence that row t of the batch belongs to: the last b with cu[b] <= t, by a 32-way search of one warp (two
+// dependent reads for up to 1024 sequences). Reads cu[0 .. seqs - 1] only, whatever the values.
+__device__ __forceinline__ int find_sequence(const int* __restrict__ cu, int seqs, int t, int lane) {
+    int lo = 0, hi = seqs;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned below = __ballot_sync(kFull, at < hi && cu[at] <= t);
+        const int n = below ? 32 - __clz(below) : 1;
+        lo += (n - 1) * step;
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
+// Sequence b's rows and cache length, forced into range (with an error word) whatever the arrays hold.
+struct Seq {
+    int row0, n, len;        // first row, new tokens, cache length with them
+};
+__device__ __forceinline__ Seq load_seq(const KvBatch& b, const FastDiv& page, int i, int* err) {
+    int r0 = b.cu[i], r1 = b.cu[i + 1], len = b.lens[i];
+    if (r0 < 0 || r1 < r0 || r1 > b.tokens) {
+        report(err, kKvBadBatch);
+        r0 = min(max(r0, 0), b.tokens);
+        r1 = min(max(r1, r0), b.tokens);
+    }
+    const long long cap = (long long)b.table_stride * page.d;
+    if (len < 0 || len > cap) {
+        report(err, kKvBadLength);
+        len = len < 0 ? 0 : int(cap);
+    }
+    return {r0, r1 - r0, len};
+}
+
+__device__ __forceinline__ int safe_page(int id, const KvView& c) {
+    if (unsigned(id) < unsigned(c.num_pages)) return id;
+    report(c.err, kKvBadPage);
+    return 0;
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// Stores one value rounded to nearest in the given type.
+__device__ __forceinline__ void store_as(void* base, long long i, float x, int type) {
+    if (type == kF32) static_cast<float*>(base)[i] = x;
+    else if (type == kF16) static_cast<__half*>(base)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, bool half) {
+    if (half) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Eight consecutive values, 16-byte aligned (32-byte for fp32 pairs of loads).
+template <class T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __half>::value) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                x[2 * i] = f.x; x[2 * i + 1] = f.y;
+            } else {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store8(char* p, const float (&x)[8], int type) {
+    if (type == kF32) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        const bool h = type == kF16;
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2(x[0], x[1], h), pack2(x[2], x[3], h), pack2(x[4], x[5], h),
+                                                  pack2(x[6], x[7], h));
+    }
+}
+
+}  // namespace paged
+}  // namespace gpt

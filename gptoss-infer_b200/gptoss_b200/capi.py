@@ -70,7 +70,23 @@ SIGNATURES = {
     "gptoss_bench_steps": ([P, I32, I32], I32),
     "gptoss_generate_greedy": ([P, I32, I32, P], I32),
     "gptoss_kv_fill_random": ([P, I32, ctypes.c_ulonglong], I32),
+    "gptoss_kv_pool_create": ([P, P, I32, I32, I32, I32, I32, I32, P], P),
+    "gptoss_kv_pool_destroy": ([P], None),
+    "gptoss_kv_pool_status": ([P, P], I32),
+    "gptoss_kv_append": ([P, I32, P, P, P, P, I32, I64, I64, I32, P, P, I32, I32, I32, P, I32, P], I32),
+    "gptoss_paged_attention": ([P, I32, P, P, I32, I64, I32, P, F32, I32, P, I64, P], I32),
+    "gptoss_kv_fork": ([P, P, P, P, I32, P, P, I32, I32, P, P, P, P], I32),
+    "gptoss_kv_compact": ([P, P, P, P, I32, I32, P, P, P, P, P], I32),
+    "gptoss_beam_select": ([P, I32, I64, P, P, I32, I32, I32, I32, I32, P, P, P, P], I32),
 }
+
+
+
+class KvBatch(ctypes.Structure):
+    """gptoss_kv_batch: a batch of sequences with their new tokens (device pointers)."""
+    _fields_ = [("seqs", ctypes.c_int32), ("tokens", ctypes.c_int32), ("max_new", ctypes.c_int32),
+                ("table_stride", ctypes.c_int32), ("cu_tokens", P), ("kv_lens", P), ("tables", P)]
+
 
 _lib = None
 

@@ -264,6 +264,94 @@ int gptoss_set_prefill_terms(int terms);
  * the float64 bound. Returns the previous mode, or -2 (mode outside -1 .. 1). */
 int gptoss_set_prefill_packing(int mode);
 
+/* ---- [extension] Paged key/value cache: many sequences, prompt chunks and beams ---------------------------- */
+
+/* [extension] A pool of cache pages of `layers` layers in the caller's device memory (it must stay valid for the
+ * handle's lifetime): element (layer l, page p, slot s, head h, dim d) of k and of v sits at l * strides[0] +
+ * p * strides[1] + s * strides[2] + h * strides[3] + d (strides in elements, host array of 4, multiples of 8), so both
+ * slot-major and head-major pages are described without a copy. type: 1 = fp16, 2 = bf16. head_dim 64 or 128; any
+ * page_size >= 1. A sequence's table is an int32 row of page ids: position p lives in page table[p / page_size], slot
+ * p % page_size; entries past its last position are never read. The handle owns its workspaces (a few MB) and an error
+ * word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
+ * current at its creation. Returns NULL on failure (gptoss_last_error). Synchronizes. */
+typedef struct gptoss_kv_pool gptoss_kv_pool;
+gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, int num_pages, int page_size,
+                                      int kv_heads, int head_dim, const long long* strides);
+void gptoss_kv_pool_destroy(gptoss_kv_pool* pool);
+/* [extension] Synchronizes, stores the pool's error word in *code and clears it. 0: every call since read valid tables
+ * and lengths. Device-side data is checked on the device: 300 a page id outside the pool, 301 a length outside its
+ * table, 302 cu_tokens out of order, 303 a position outside the cos/sin table (or negative), 304 no free page left,
+ * 305 a parent outside the sequences, 310 .. 319 a bounded wait gave up. What a flagged call wrote is not meaningful
+ * for the sequences concerned; nothing outside the given arrays is touched. */
+int gptoss_kv_pool_status(gptoss_kv_pool* pool, int* code);
+
+/* [extension] A batch of sequences with their new tokens. Sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1) of
+ * the batch (none, one or many); kv_lens[b] counts its cached positions with these new ones, so its row i stands at
+ * position kv_lens[b] - new + i. tables: int32 [seqs][table_stride]. Device pointers. max_new: an upper bound on the
+ * new tokens of one sequence, as the host knows it: it only steers the choice of kernel. */
+typedef struct {
+    int32_t seqs, tokens, max_new, table_stride;
+    const int32_t* cu_tokens;                /* [seqs + 1], cu_tokens[0] = 0, cu_tokens[seqs] = tokens */
+    const int32_t* kv_lens;                  /* [seqs] */
+    const int32_t* tables;
+} gptoss_kv_batch;
+
+/* [extension] Rotary positions and the append of a batch's new tokens to one layer of the pool, asynchronous on
+ * `stream`: q [tokens][q_heads][head_dim] is rotated into q_out (same shape, contiguous), k and v
+ * [tokens][kv_heads][head_dim] go into the cache, k rotated. q_stride, kv_stride: elements between tokens, so the three
+ * may lie in one fused projection. type, q_out_type: 0 = fp32, 1 = fp16, 2 = bf16. cos_t, sin_t: fp32
+ * [positions][rot_dim / 2], with any scaling of the frequencies for long contexts in them. The first rot_dim (even)
+ * dims of a head turn, in pairs (j, j + rot_dim / 2), or (2j, 2j + 1) with interleaved = 1; the others pass. fp32
+ * arithmetic, one rounding to the stored type. q_out may alias q when their types and strides agree. */
+int gptoss_kv_append(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* batch, const void* q, const void* k,
+                     const void* v, int type, long long q_stride, long long kv_stride, int q_heads,
+                     const float* cos_t, const float* sin_t, int positions, int rot_dim, int interleaved, void* q_out,
+                     int q_out_type, void* stream);
+
+/* [extension] Causal attention of a batch's new tokens over the cache (their own keys and values appended before),
+ * asynchronous on `stream`: out[t][h] = sum_j w_j v_j / (sum_j w_j + exp(sinks[h])), w_j = exp(scale q.k_j), over the
+ * positions j <= p of the token at p, and j > p - window with window > 0. Query head h reads key/value head
+ * h / (q_heads / kv_heads). sinks: fp32 [q_heads] or NULL (no sink term). q and out: [tokens] rows of q_heads *
+ * head_dim, q_stride and out_stride elements apart, 16-byte aligned, of the cache's type, or fp32 beside an fp16 cache
+ * (products then keep about 22 bits). Statistics and sums are fp32. A row that sees no key is 0. Results do not depend
+ * on timing. */
+int gptoss_paged_attention(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* batch, const void* q, int type,
+                           long long q_stride, int q_heads, const float* sinks, float scale, int window, void* out,
+                           long long out_stride, void* stream);
+
+/* [extension] Forks, reorders, grows and frees sequences, asynchronous on `stream`. Child m continues sequence
+ * parents[m] (-1: an empty child) of the given `seqs` and gets room for extra[m] more positions (extra NULL: none):
+ * tables_out [children][table_stride] (unused entries -1), lens_out[m] = lens[parent] + extra[m]. refs and refs_out
+ * (int32 [num_pages], may alias) count each page's references: those of the given sequences are dropped (a sequence
+ * without a child is thereby freed), the children's added. Full pages are shared. A part-filled last page stays with
+ * the parent's first child if its count was 1, and is copied to a fresh page for every other child, in all layers of
+ * the pool. Fresh pages are the lowest-numbered ones left with count 0, in the order of the children; if they run out,
+ * the children concerned get the length that their pages hold and the pool's status is 304. */
+int gptoss_kv_fork(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* tables, const int32_t* lens, int seqs,
+                   const int32_t* parents, const int32_t* extra, int children, int table_stride, int32_t* refs_out,
+                   int32_t* tables_out, int32_t* lens_out, void* stream);
+
+/* [extension] Moves the live pages (count > 0) to the lowest page numbers, in all layers, asynchronous on `stream`:
+ * the live pages past the number of live pages go to the free ones below it, both in ascending order. remap[num_pages]:
+ * each live page's new number, -1 for a free page; *live: how many there are. refs_out and tables_out (the tables of
+ * `seqs` sequences with lengths lens, remapped, unused entries -1) may alias refs and tables. */
+int gptoss_kv_compact(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* tables, const int32_t* lens, int seqs,
+                      int table_stride, int32_t* refs_out, int32_t* tables_out, int32_t* remap, int32_t* live,
+                      void* stream);
+
+/* [extension] Beam selection, asynchronous on `stream`: for each of `batch` requests the best `picks` (1 .. 64) of its
+ * beams (1 .. 64) x vocab candidates, score = scores[row] + log softmax(logits[row])[token], best first, equal scores
+ * to the lower row, then the lower token. logits: [batch * beams] rows of vocab, row_stride elements apart, type 0 =
+ * fp32, 1 = fp16, 2 = bf16; scores fp32 [batch * beams]. done (NULL, or uint8 [batch * beams]): a finished row's only
+ * candidate is done_token, at scores[row]. A NaN logit counts as -inf; candidates of score -inf are not picked, and
+ * places without a candidate get score -inf, row -1, token -1. Outputs [batch][picks]: out_scores fp32, rows (of
+ * logits, so they serve as gptoss_kv_fork's parents), tokens. Sums and ranking use fp32 statistics and fp64 scores.
+ * Uses the calling thread's workspace: calls from one thread must not overlap on the GPU, and the first call at a
+ * larger size allocates (before a stream capture). */
+int gptoss_beam_select(const void* logits, int type, long long row_stride, const float* scores, const uint8_t* done,
+                       int done_token, int batch, int beams, int vocab, int picks, float* out_scores, int32_t* rows,
+                       int32_t* tokens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
