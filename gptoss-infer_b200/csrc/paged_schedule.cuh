@@ -1,0 +1,209 @@
+// Work items of the paged attention kernels and their split over the grid.
+//
+// An item is (sequence, key/value head, tile of R query rows), row = token * group + head of the group; its work is the
+// key range [lo, hi) that its rows see together, in groups of UNIT keys (at least one). All items laid end to end are
+// cut into one contiguous span of groups per CTA, so every CTA gets the same number of groups whatever the lengths: a
+// span may begin or end inside an item. An item cut into pieces is put together by the CTA that finishes last, from the
+// pieces in their order, so the result does not depend on timing. Each CTA leaves at most two pieces (the item it
+// starts in and the item it ends in), which bounds the workspace by the grid alone. Every CTA finds its span itself
+// from the lengths in device memory: the host needs none of them.
+#pragma once
+#include "paged.cuh"
+
+namespace gpt {
+namespace paged {
+
+struct Item {
+    int b, h, t, nt;         // sequence, key/value head, row tile, the sequence's row tiles
+    Seq s;
+    int rows;                // valid rows of this tile
+    int p0, p1;              // positions of its first and last row
+    int lo, hi;              // keys any of its rows sees (lo <= hi)
+    int n;                   // groups
+};
+
+template <int R, int UNIT>
+struct Schedule {
+    const KvView& c;
+    const KvBatch& b;
+    int window;
+    FastDiv group;
+
+    __device__ __forceinline__ int row_tiles(int n) const { return (n * int(group.d) + R - 1) / R; }
+
+    __device__ __forceinline__ void fill(Item& it) const {
+        const int r0 = it.t * R;
+        it.rows = min(R, it.s.n * int(group.d) - r0);
+        it.p0 = it.s.len - it.s.n + int(group.div(r0));
+        it.p1 = it.s.len - it.s.n + int(group.div(r0 + it.rows - 1));
+        it.lo = window ? max(0, it.p0 - window + 1) : 0;
+        it.hi = max(it.lo, it.p1 + 1);
+        it.n = max(1, (it.hi - it.lo + UNIT - 1) / UNIT);
+    }
+
+    // Groups of one key/value head of a sequence.
+    __device__ __forceinline__ int head_groups(const Seq& s) const {
+        Item it;
+        it.s = s;
+        it.nt = row_tiles(s.n);
+        int sum = 0;
+        for (it.t = 0; it.t < it.nt; ++it.t) {
+            fill(it);
+            sum += it.n;
+        }
+        return sum;
+    }
+
+    // First item at or after (b, 0, 0); false past the last sequence.
+    __device__ __forceinline__ bool open(Item& it, int i) const {
+        for (; i < b.seqs; ++i) {
+            it.s = load_seq(b, c.page, i, c.err);
+            it.nt = row_tiles(it.s.n);
+            if (it.nt > 0) {
+                it.b = i;
+                it.h = it.t = 0;
+                fill(it);
+                return true;
+            }
+        }
+        it.b = b.seqs;
+        it.n = 0x7fffffff;
+        return false;
+    }
+    __device__ __forceinline__ void next(Item& it) const {
+        if (++it.t < it.nt) {
+            fill(it);
+        } else if (++it.h < c.kv_heads) {
+            it.t = 0;
+            fill(it);
+        } else {
+            open(it, it.b + 1);
+        }
+    }
+    // Steps k groups on from group g of the item.
+    __device__ __forceinline__ void step(Item& it, int& g, int k) const {
+        g += k;
+        while (g >= it.n && it.b < b.seqs) {
+            g -= it.n;
+            next(it);
+        }
+    }
+};
+
+// What a CTA works on: groups [start, start + len) of all, `per` groups per CTA; the item and group it starts in.
+struct Span {
+    long long start;
+    int len, per, g;
+    Item it;
+};
+
+// Sum over the block in thread order and each thread's exclusive prefix; NT threads, two barriers.
+template <int NT>
+__device__ __forceinline__ long long block_prefix(long long v, long long* warp_sums, long long* total) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    long long x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) {
+        if (w < warp) before += warp_sums[w];
+        all += warp_sums[w];
+    }
+    *total = all;
+    return before + x - v;
+}
+
+// Finds this CTA's span; all NT threads call it. scratch: NT / 32 + 2 words of shared memory.
+template <int NT, int R, int UNIT>
+__device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, long long* scratch) {
+    const int seqs = sch.b.seqs, kvh = sch.c.kv_heads;
+    long long total = 0, mine = 0, before = 0;
+    for (int i0 = 0; i0 < seqs; i0 += NT) {
+        const int i = i0 + threadIdx.x;
+        mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err)) * kvh : 0;
+        long long sum;
+        before = total + block_prefix<NT>(mine, scratch, &sum);
+        total += sum;
+    }
+    Span sp;
+    sp.per = int((total + gridDim.x - 1) / gridDim.x);
+    sp.start = (long long)blockIdx.x * sp.per;
+    sp.len = int(max(0ll, min((long long)sp.per, total - sp.start)));
+    sp.g = 0;
+    if (sp.len == 0) return sp;
+    // the sequence that holds group `start`: its thread knows the prefix (with many sequences, a second pass)
+    long long* found = scratch + NT / 32;
+    if (seqs > NT) {
+        long long base = 0;
+        for (int i0 = 0; i0 < seqs; i0 += NT) {
+            const int i = i0 + threadIdx.x;
+            mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err)) * kvh : 0;
+            long long sum;
+            before = base + block_prefix<NT>(mine, scratch, &sum);
+            base += sum;
+            if (sp.start >= before && sp.start < before + mine) {
+                found[0] = i;
+                found[1] = before;
+            }
+        }
+    } else if (sp.start >= before && sp.start < before + mine) {
+        found[0] = threadIdx.x;
+        found[1] = before;
+    }
+    __syncthreads();
+    sch.open(sp.it, int(found[0]));
+    int off = 0;
+    const long long in_seq = sp.start - found[1];
+    const int per_head = sch.head_groups(sp.it.s);
+    sp.it.h = int(in_seq / per_head);
+    off = int(in_seq % per_head);
+    while (off >= sp.it.n) {
+        off -= sp.it.n;
+        ++sp.it.t;
+        sch.fill(sp.it);
+    }
+    sp.g = off;
+    return sp;
+}
+
+// One query row over keys [k0, k1) of a sequence, by one warp, in plain fp32 arithmetic and with masked keys never
+// multiplied: the path taken when a value that some row of a tile must not see is NaN or infinite (a matrix product
+// would carry it into every row as 0 * NaN). m (base-2 logarithm), l and o (dims lane * E ..) are left unnormalised.
+template <class T, class C, int D>
+__device__ __noinline__ void careful_row(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, int seq, int kh,
+                                         long long q_at, int lo, int hi, float* m_out, float* l_out, float* o_out) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x % 32;
+    float q[E], o[E] = {};
+    for (int e = 0; e < E; ++e) q[e] = to_f32(static_cast<const T*>(a.q)[q_at + lane * E + e]);
+    const float sc = a.scale * 1.4426950408889634f;
+    float m = -INFINITY, z = 0.f;
+    for (int j = lo; j < hi; ++j) {
+        const int pg = c.page.div(j);
+        const int id = safe_page(b.tables[(long long)seq * b.table_stride + pg], c);
+        const long long off = id * c.page_stride + (j - pg * int(c.page.d)) * c.token_stride + kh * c.head_stride;
+        const C* k = reinterpret_cast<const C*>(c.k + off) + lane * E;
+        const C* v = reinterpret_cast<const C*>(c.v + off) + lane * E;
+        float x = 0.f;
+        for (int e = 0; e < E; ++e) x += q[e] * to_f32(k[e]);
+        x = warp_sum(x) * sc;
+        const float mm = fmaxf(m, x);
+        const float f = mm == -INFINITY ? 1.f : exp2f(m - mm), w = x == -INFINITY ? 0.f : exp2f(x - mm);
+        z = z * f + w;
+        for (int e = 0; e < E; ++e) o[e] = o[e] * f + w * to_f32(v[e]);
+        m = mm;
+    }
+    *m_out = m;
+    *l_out = z;
+    for (int e = 0; e < E; ++e) o_out[e] = o[e];
+}
+
+}  // namespace paged
+}  // namespace gpt
