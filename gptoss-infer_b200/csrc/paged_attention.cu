@@ -138,7 +138,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const Schedule<R, kGroup> sch{c, b, a.window, group};
-    const Span sp = find_span<kThreads>(sch, scratch);
+    const Span sp = find_span<kThreads>(sch, kWarps * (NS - 1), scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
 
@@ -178,20 +178,8 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
         cp_async_commit();
         slot_in = slot_in + 1 == NS ? 0 : slot_in + 1;
     };
-    look_up();
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) issue();
-
-    int slot_out = 0, at = 0;                         // at: span index of the current piece's first group
-    Item it = sp.it;
-    int g0 = sp.g;
-    if (threadIdx.x == 0) flags[0] = 0;
-    while (at < sp.len) {
-        const int g1 = min(it.n, g0 + sp.len - at);   // this piece: groups [g0, g1) of the item
+    const auto stage_q = [&](const Item& it) {        // an item's queries to shared memory
         const int r0 = it.t * R;
-        const int lo_last = a.window ? max(0, it.p1 - a.window + 1) : 0;
-        // --- queries
-        __syncthreads();
         if constexpr (S::kSplit) {
             for (int r = warp; r < R; r += kWarps) {
                 float x[D / 32], top = 0.f;
@@ -230,8 +218,25 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
                 *reinterpret_cast<uint4*>(q_tile + tile_off<D>(r, ch)) = x;
             }
         }
-        __syncthreads();
+    };
+    look_up();                                        // its latency passes while the first queries are fetched
+    stage_q(sp.it);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) issue();
 
+    int slot_out = 0, at = 0;                         // at: span index of the current piece's first group
+    Item it = sp.it;
+    int g0 = sp.g;
+    if (threadIdx.x == 0) flags[0] = 0;
+    while (at < sp.len) {
+        const int g1 = min(it.n, g0 + sp.len - at);   // this piece: groups [g0, g1) of the item
+        const int r0 = it.t * R;
+        const int lo_last = a.window ? max(0, it.p1 - a.window + 1) : 0;
+        if (at > 0) {
+            __syncthreads();
+            stage_q(it);
+        }
+        __syncthreads();
         float o[D / 16][NT][4], m[NT][2], l[NT][2], sc[NT][2];
         constexpr bool kHold = NT <= 2 && !(S::kSplit && D == 128);      // queries stay in registers
         uint32_t qf[kHold ? NT : 1][kHold ? D / 16 : 1][2], qg[kHold && S::kSplit ? NT : 1][kHold ? D / 16 : 1][2];
@@ -489,14 +494,13 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
         if (!whole) {
             // the item's first CTA and the number of its pieces follow from where its groups lie
             const long long first = sp.start + at - g0;
-            const int c0 = int(first / sp.per), c1 = int((first + it.n - 1) / sp.per);
+            const int c0 = blockIdx.x - (first < sp.start ? ceil_div(sp.start - first, sp.per) : 0);
+            const int c1 = blockIdx.x + int(unsigned(first + it.n - 1 - sp.start) / unsigned(sp.per));
             __syncthreads();
             if (threadIdx.x == 0) {
-                __threadfence();
-                const int done = atomicAdd(&counters[c0], 1);
+                const int done = arrive(&counters[c0]);
                 flags[1] = done == c1 - c0;
                 if (done == c1 - c0) counters[c0] = 0;
-                __threadfence();
             }
             __syncthreads();
             if (flags[1]) {

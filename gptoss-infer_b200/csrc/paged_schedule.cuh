@@ -41,15 +41,15 @@ struct Schedule {
         it.n = max(1, (it.hi - it.lo + UNIT - 1) / UNIT);
     }
 
-    // Groups of one key/value head of a sequence.
-    __device__ __forceinline__ int head_groups(const Seq& s) const {
+    // Groups of one key/value head of a sequence, each item's rounded up to a multiple of pad.
+    __device__ __forceinline__ int head_groups(const Seq& s, int pad) const {
         Item it;
         it.s = s;
         it.nt = row_tiles(s.n);
         int sum = 0;
         for (it.t = 0; it.t < it.nt; ++it.t) {
             fill(it);
-            sum += it.n;
+            sum += pad == 1 ? it.n : (it.n + pad - 1) / pad * pad;
         }
         return sum;
     }
@@ -97,6 +97,10 @@ struct Span {
     Item it;
 };
 
+__device__ __forceinline__ int ceil_div(long long a, int b) {
+    return a >> 31 ? int((a + b - 1) / b) : int((unsigned(a) + unsigned(b) - 1) / unsigned(b));
+}
+
 // Sum over the block in thread order and each thread's exclusive prefix; NT threads, two barriers.
 template <int NT>
 __device__ __forceinline__ long long block_prefix(long long v, long long* warp_sums, long long* total) {
@@ -121,22 +125,74 @@ __device__ __forceinline__ long long block_prefix(long long v, long long* warp_s
 }
 
 // Finds this CTA's span; all NT threads call it. scratch: NT / 32 + 2 words of shared memory.
+//
+// With few items (an eighth of the grid at most) a span never crosses from one item into the next: items are laid out
+// padded to whole spans of `per` groups, per = total / (grid - items), which costs at most a seventh of the grid and
+// saves the CTAs in between a second item's fixed cost (4K positions, 8 heads, one token: 17.9 us with spans cut
+// anywhere, 14.2 us without). least: the fewest groups worth a CTA of its own then.
 template <int NT, int R, int UNIT>
-__device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, long long* scratch) {
-    const int seqs = sch.b.seqs, kvh = sch.c.kv_heads;
+__device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int least, long long* scratch) {
+    const int seqs = sch.b.seqs, kvh = sch.c.kv_heads, grid = int(gridDim.x);
+    Span sp;
+    sp.g = 0;
+    if (seqs <= 32) {                                 // each warp for itself, a lane per sequence
+        const int lane = threadIdx.x % 32;
+        Seq s{0, 0, 0};
+        if (lane < seqs) s = load_seq(sch.b, sch.c.page, lane, sch.c.err);
+        int units = sch.head_groups(s, 1);
+        long long total = (long long)units * kvh;
+        int items = sch.row_tiles(s.n) * kvh;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            total += __shfl_xor_sync(kFull, total, o);
+            items += __shfl_xor_sync(kFull, items, o);
+        }
+        const bool whole = items * 8 <= grid;
+        sp.per = whole ? max(least, ceil_div(total, grid - items)) : ceil_div(total, grid);
+        sp.start = (long long)blockIdx.x * sp.per;
+        sp.len = 0;
+        if (sp.per == 0) return sp;
+        const int pad = whole ? sp.per : 1;
+        if (whole) units = sch.head_groups(s, pad);
+        const long long mine = (long long)units * kvh;
+        long long end = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(kFull, end, o);
+            if (lane >= o) end += y;
+        }
+        const unsigned holds = __ballot_sync(kFull, sp.start >= end - mine && sp.start < end);
+        if (holds == 0) return sp;
+        const int src = __ffs(holds) - 1;
+        total = __shfl_sync(kFull, end, 31);
+        const long long in_seq = sp.start - __shfl_sync(kFull, end - mine, src);
+        units = __shfl_sync(kFull, units, src);
+        Item& it = sp.it;
+        it.b = src;
+        it.s = {__shfl_sync(kFull, s.row0, src), __shfl_sync(kFull, s.n, src), __shfl_sync(kFull, s.len, src)};
+        it.nt = sch.row_tiles(it.s.n);
+        it.h = in_seq >> 31 ? int(in_seq / units) : int(unsigned(in_seq) / unsigned(units));
+        int off = int(in_seq - (long long)it.h * units);
+        it.t = 0;
+        for (sch.fill(it); off >= (it.n + pad - 1) / pad * pad; sch.fill(it)) {
+            off -= (it.n + pad - 1) / pad * pad;
+            ++it.t;
+        }
+        sp.g = off;
+        sp.len = whole ? min(sp.per, it.n - off) : int(min((long long)sp.per, total - sp.start));
+        return sp;
+    }
     long long total = 0, mine = 0, before = 0;
     for (int i0 = 0; i0 < seqs; i0 += NT) {
         const int i = i0 + threadIdx.x;
-        mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err)) * kvh : 0;
+        mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err), 1) * kvh : 0;
         long long sum;
         before = total + block_prefix<NT>(mine, scratch, &sum);
         total += sum;
     }
-    Span sp;
-    sp.per = int((total + gridDim.x - 1) / gridDim.x);
+    sp.per = ceil_div(total, grid);
     sp.start = (long long)blockIdx.x * sp.per;
     sp.len = int(max(0ll, min((long long)sp.per, total - sp.start)));
-    sp.g = 0;
     if (sp.len == 0) return sp;
     // the sequence that holds group `start`: its thread knows the prefix (with many sequences, a second pass)
     long long* found = scratch + NT / 32;
@@ -144,7 +200,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, long lon
         long long base = 0;
         for (int i0 = 0; i0 < seqs; i0 += NT) {
             const int i = i0 + threadIdx.x;
-            mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err)) * kvh : 0;
+            mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err), 1) * kvh : 0;
             long long sum;
             before = base + block_prefix<NT>(mine, scratch, &sum);
             base += sum;
@@ -159,11 +215,10 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, long lon
     }
     __syncthreads();
     sch.open(sp.it, int(found[0]));
-    int off = 0;
     const long long in_seq = sp.start - found[1];
-    const int per_head = sch.head_groups(sp.it.s);
-    sp.it.h = int(in_seq / per_head);
-    off = int(in_seq % per_head);
+    const int per_head = sch.head_groups(sp.it.s, 1);
+    sp.it.h = in_seq >> 31 ? int(in_seq / per_head) : int(unsigned(in_seq) / unsigned(per_head));
+    int off = int(in_seq - (long long)sp.it.h * per_head);
     while (off >= sp.it.n) {
         off -= sp.it.n;
         ++sp.it.t;
@@ -171,6 +226,14 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, long lon
     }
     sp.g = off;
     return sp;
+}
+
+// One more arrival at a counter, after everything this CTA wrote (the caller has passed a barrier since); what the
+// earlier arrivals wrote is visible to the CTA after its next barrier.
+__device__ __forceinline__ int arrive(int* counter) {
+    int old;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    return old;
 }
 
 // One query row over keys [k0, k1) of a sequence, by one warp, in plain fp32 arithmetic and with masked keys never

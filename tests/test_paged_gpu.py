@@ -206,6 +206,19 @@ def test_attention_window(lib, pair, shape, window):
     check_attention(out, *reference_attention(s, q, sinks, 0.125, window))
 
 
+@pytest.mark.parametrize("seqs", [31, 32, 33, 130, 300])
+@pytest.mark.parametrize("most,window", [(1, 0), (3, 40), (150, 0)])
+def test_attention_many_sequences(lib, seqs, most, window):
+    """Unequal lengths, some sequences without new tokens, some without positions."""
+    r = np.random.RandomState(seqs)
+    new = [int(x) for x in r.randint(0, most + 1, seqs)]
+    lens = [max(n, int(x)) if x > 20 else 0 for n, x in zip(new, r.randint(0, 500, seqs))]
+    s = Setup(lib, new, lens, page=16, kvh=2, dim=64, dtype=F16, seed=seqs)
+    q = new_q(s.T, 4, 64, F16)
+    out = run_attention(lib, s, q, None, window)
+    check_attention(out, *reference_attention(s, q, None, 0.125, window))
+
+
 def test_attention_window_never_reads_freed_pages(lib):
     """Pages wholly before the window may be freed: their table entries are not read, and no error is flagged."""
     s = Setup(lib, [1, 40], [500, 700], page=16, kvh=2, dim=64, dtype=F16, seed=7)
