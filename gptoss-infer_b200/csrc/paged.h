@@ -70,8 +70,12 @@ struct PagedAttnArgs {
     int type, kv_type, q_heads, window;
     float scale;
 };
-// Workspace of launch_paged_attention: partial results and counters; zeroed once, the kernels leave the counters at 0.
-size_t paged_attention_ws_bytes();
+// Workspace of launch_paged_attention: counters and partial results; zeroed once, the kernels leave the counters at 0.
+// The two kernels share it (their counters are the same words).
+constexpr size_t kCounterBytes = 2048;            // of both kernels, before the partial results
+size_t paged_attention_ws_bytes(int dim);
+size_t paged_tiles_ws_bytes(int dim);
+void launch_paged_tiles(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
 void launch_paged_attention(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
 
 struct BeamArgs {

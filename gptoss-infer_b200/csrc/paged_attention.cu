@@ -554,6 +554,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
 }
 
 constexpr int kMaxCtas = 2 * 160;                     // two CTAs per SM, SMs rounded up
+static_assert(kMaxCtas * sizeof(int) <= kCounterBytes, "one counter per CTA");
 constexpr int kSlotFloats = slot_floats<64, 64>() > slot_floats<32, 128>() ? slot_floats<64, 64>()
                                                                               : slot_floats<32, 128>();
 
@@ -566,7 +567,7 @@ void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
     const int grid = std::min(kMaxCtas, num_sms() * S::kPerSm);
     paged_rows_kernel<T, C, D, NT><<<grid, kThreads, S::kSmem, s>>>(
         c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
-        reinterpret_cast<float*>(static_cast<char*>(ws) + kMaxCtas * sizeof(int)));
+        reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes));
     check_launch("paged_attention");
 }
 
@@ -587,9 +588,12 @@ void by_shape(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* w
 
 }  // namespace
 
-size_t paged_attention_ws_bytes() { return kMaxCtas * (sizeof(int) + 2 * sizeof(float) * kSlotFloats); }
+size_t paged_attention_ws_bytes(int dim) {
+    return std::max(kCounterBytes + kMaxCtas * 2 * sizeof(float) * kSlotFloats, paged_tiles_ws_bytes(dim));
+}
 
 void launch_paged_attention(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    if ((long long)b.max_new * (a.q_heads / c.kv_heads) > 64) return launch_paged_tiles(c, b, a, ws, s);
     if (a.type == kF32) by_shape<float, __half>(c, b, a, ws, s);
     else if (a.type == kF16) by_shape<__half, __half>(c, b, a, ws, s);
     else by_shape<__nv_bfloat16, __nv_bfloat16>(c, b, a, ws, s);

@@ -1,0 +1,599 @@
+// Attention of new tokens over the paged cache: many rows per key/value head (prompt chunks), on tcgen05 tensor cores.
+//
+// The same sum as in paged_attention.cu. An item is 256 query rows (row = token * group + head of the group: all query
+// heads of a key/value head share its tiles) against tiles of 128 keys. Per tile and half of 128 rows:
+//   S = Q K^T            tcgen05.mma kind::f16, both operands in shared memory, K-major, accumulator in TMEM
+//   P = exp2(S - m)      one thread per row: 128 scores in registers, no exchange between threads
+//   O += P V             A operand P read from TMEM (written over S), V in shared memory as stored (rows = keys)
+// The two halves alternate: while one half's exponentials run, the other half's products do.
+//
+// Bound: with heads of 64 the exponentials (128 x 128 per 4.2 MFLOP, 16 a clock and SM), with heads of 128 the products.
+//
+// Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output), 8-11 copy keys and values (16-byte
+// asynchronous copies through a ring of tiles; any page size), 12 issues the products. The running maximum moves only when
+// it grows by more than 2^8, so the accumulator in TMEM is rescaled rarely (weights stay at most 256).
+//
+// fp32 queries: two fp16 parts of a row scaled by a power of two, and two of the weights, as in paged_attention.cu.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged_schedule.cuh"
+#include "kernels.h"
+#include "tc.cuh"
+
+namespace gpt {
+namespace {
+
+using namespace paged;
+
+constexpr int kThreads = 512, kRows = 256, kHalf = 128, kTile = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait_group() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Instruction descriptor of tcgen05.mma kind::f16: fp32 accumulator (bit 4), A and B both fp16 (0) or both bf16 (1) in
+// bits 7-9 and 10-12, B rows = K when `turned` (bit 16), N >> 3 in bits 17-22, M >> 4 in bits 24-28.
+__host__ __device__ constexpr uint32_t idesc_f16(bool bf16, bool turned, int M, int N) {
+    return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(turned) << 16) |
+           (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+// D (+)= A B^T, A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+// D (+)= A B, A in TMEM (one lane per row, two 16-bit values per column).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// A wait's outcome as the whole warp's.
+__device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(kFull, ok); }
+__device__ __forceinline__ void bar_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Shared-memory image of 128 rows of D 16-bit values: halves of 64 columns, each in the 128-byte swizzled layout. As a
+// K-major operand the rows are M or N; as V the rows are K (8-row groups 1024 bytes apart, 64-column halves 16 KB apart).
+template <int D>
+__device__ __forceinline__ uint32_t image_off(int r, int chunk) {
+    return uint32_t((chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+}
+
+template <class T, int D>
+struct Layout {
+    static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kTileBytes = 128 * D * 2;                       // a tile of keys or of values
+    static constexpr int kQ = 2 * kTileBytes * (kSplit ? 2 : 1);         // [half][part]
+    static constexpr int kSlots = D == 64 ? 8 : (kSplit ? 3 : 5);
+    static constexpr int kSmem = kQ + kSlots * kTileBytes + 2 * kRows * 4 + 512 + 160;
+};
+
+template <int D>
+__host__ __device__ constexpr int slot_floats() {
+    return kRows * D + 2 * kRows;                                        // sums [dim][row], maxima, sums of weights
+}
+
+enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kPFull = 18, kPvDone = 20, kQFull = 22, kQFree = 23, kDrain = 24, kBars = 25 };
+
+template <class T, class C, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* counters, float* slots) {
+    using L = Layout<T, D>;
+    constexpr int NS = L::kSlots, CH = D / 8;
+    constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
+    extern __shared__ __align__(1024) char smem[];
+    char* q_tile = smem;
+    char* ring = smem + L::kQ;
+    float* row_scale = reinterpret_cast<float*>(ring + NS * L::kTileBytes);   // [piece parity][row]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(row_scale + 2 * kRows);
+    int* flags = reinterpret_cast<int*>(bars + kBars);                   // [0..7] poisoned piece, [8] last, [9] TMEM
+    long long* scratch = reinterpret_cast<long long*>(reinterpret_cast<char*>(bars) + 512);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    int* err = c.err;
+    const Schedule<kRows, kTile> sch{c, b, a.window, group};
+    const Span sp = find_span<kThreads>(sch, 2, scratch);
+    if (sp.len == 0) return;
+    const int G = int(group.d);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) {
+            tc::mbar_init(&bars[kTileFull + i], 128);
+            tc::mbar_init(&bars[kFree + i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            tc::mbar_init(&bars[kSFull + t], 1);
+            tc::mbar_init(&bars[kPFull + t], 128);
+            tc::mbar_init(&bars[kPvDone + t], 1);
+        }
+        tc::mbar_init(&bars[kQFull], 128);
+        tc::mbar_init(&bars[kQFree], 1);
+        tc::mbar_init(&bars[kDrain], 1);
+        tc::fence_barrier_init();
+        for (int i = 0; i < 8; ++i) flags[i] = 0;
+    }
+    if (warp == 12) {
+        tc::tmem_alloc(reinterpret_cast<uint32_t*>(&flags[9]), 512);
+        tc::tmem_relinquish();
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = uint32_t(flags[9]);
+    // TMEM columns: S (and P over it) of half t at 128 t, O at 256 + 128 t
+    const auto s_col = [&](int t) { return tmem + 128 * t; };
+    const auto o_col = [&](int t) { return tmem + 256 + 128 * t; };
+
+    if (warp >= 8 && warp < 12) {
+        // ------------------------------------------------------------------------------------------- copies
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        const int tid = threadIdx.x - 256;
+        const uint32_t ring0 = tc::smem_u32(ring);
+        int issued = 0, done = 0, piece = 0, at = 0, g0 = sp.g;
+        Item it = sp.it;
+        bool good = true;
+        constexpr int kLag = NS >= 5 ? 3 : 2;
+        int info[kLag] = {};                          // per tile in flight: piece + 1 if it is values to be checked
+        const auto complete = [&] {                   // the oldest tile in flight is complete for all threads
+            tc::fence_proxy_async_smem();
+            const int slot = done % NS;
+            if (info[done % kLag]) {
+                bool bad = false;
+                for (int i = 0; i < kTile * CH / 128; ++i) {
+                    const int r = i * (128 / CH) + tid / CH, ch = tid % CH;
+                    const uint4 x = *reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, ch));
+                    constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
+                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || (w[k] >> 16 & e) == e;
+                }
+                if (bad) flags[(info[done % kLag] - 1) & 7] = info[done % kLag];
+            }
+            tc::mbar_arrive(&bars[kTileFull + slot]);
+            ++done;
+        };
+        const auto issue = [&](int k0, bool values, int check) {
+            if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1, err, kKvWait));
+            if (!good) return;
+            const char* base = (values ? c.v : c.k) + it.h * c.head_stride;
+            const int* table = b.tables + (long long)it.b * b.table_stride;
+            const uint32_t dst = ring0 + (issued % NS) * L::kTileBytes;
+            int ids[kTile * CH / 128];
+#pragma unroll
+            for (int i = 0; i < kTile * CH / 128; ++i) {
+                const int pos = k0 + i * (128 / CH) + tid / CH;
+                ids[i] = pos < it.hi ? __ldg(table + c.page.div(pos)) : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < kTile * CH / 128; ++i) {
+                const int r = i * (128 / CH) + tid / CH, ch = tid % CH, pos = k0 + r;
+                const bool ok = pos < it.hi;
+                const char* src = base + ch * 16;
+                if (ok) src += safe_page(ids[i], c) * c.page_stride + (pos - int(c.page.div(pos) * c.page.d)) * c.token_stride;
+                cp_async16_zfill(dst + image_off<D>(r, ch), src, ok);
+            }
+            cp_async_commit();
+            info[issued % kLag] = check;
+            ++issued;
+            if (issued - done == kLag) {
+                cp_async_wait_group<kLag - 1>();
+                complete();
+            }
+        };
+        while (at < sp.len && good) {
+            const int g1 = min(it.n, g0 + sp.len - at);
+            const int lo_last = a.window ? max(0, it.p1 - a.window + 1) : 0;
+            for (int g = g0; g < g1 && good; ++g) {
+                const int k0 = it.lo + g * kTile;
+                const bool edge = k0 + kTile > it.p0 + 1 || k0 < lo_last;
+                issue(k0, false, 0);
+                if (g == g0) {
+                    // queries of this piece, once the previous piece's products have read theirs
+                    if (piece > 0) good = all_ok(good && tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
+                    if (!good) break;
+                    const int r0 = it.t * kRows;
+                    if constexpr (L::kSplit) {
+                        for (int r = warp - 8; r < kRows; r += 4) {
+                            float x[D / 32], top = 0.f;
+                            const int tok = int(group.div(r0 + r));
+                            const float* src = static_cast<const float*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
+                                               (it.h * G + (r0 + r - tok * G)) * D + lane * (D / 32);
+#pragma unroll
+                            for (int e = 0; e < D / 32; ++e) {
+                                x[e] = r < it.rows ? src[e] : 0.f;
+                                top = fmaxf(top, fabsf(x[e]));
+                            }
+#pragma unroll
+                            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                            int ex = 0;
+                            if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+                            const float up = ldexpf(1.f, min(max(11 - ex, -126), 126));
+                            const float by = a.scale < 0.f ? -up : up;
+#pragma unroll
+                            for (int e = 0; e < D / 32; ++e) {
+                                const float y = x[e] * by;
+                                const __half hi = __float2half_rn(y);
+                                const int d = lane * (D / 32) + e;
+                                char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) + d % 8 * 2;
+                                *reinterpret_cast<__half*>(p) = hi;
+                                *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
+                            }
+                            if (lane == 0) row_scale[(piece & 1) * kRows + r] = fabsf(a.scale) * kLog2e / up;
+                        }
+                    } else {
+                        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 4
+                        for (int u = tid; u < kRows * CH; u += 128) {
+                            const int r = u / CH, ch = u % CH, tok = int(group.div(r0 + r));
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (r < it.rows)
+                                x = __ldg(reinterpret_cast<const uint4*>(
+                                    static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
+                                    (it.h * G + (r0 + r - tok * G)) * D + ch * 8));
+                            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                            *reinterpret_cast<uint4*>(q_tile + (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch)) = x;
+                        }
+                    }
+                    tc::fence_proxy_async_smem();
+                    tc::mbar_arrive(&bars[kQFull]);
+                }
+                issue(k0, true, edge ? piece + 1 : 0);
+            }
+            at += g1 - g0;
+            g0 = 0;
+            ++piece;
+            if (at < sp.len) sch.next(it);
+        }
+        cp_async_wait_group<0>();
+        while (good && done < issued) complete();
+    } else if (warp >= 12) {
+        // ------------------------------------------------------------------------------------------- products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == 12 && tc::elect_one()) {
+            constexpr uint32_t id_qk = idesc_f16(kBf16, false, 128, kTile), id_pv = idesc_f16(kBf16, true, 128, D);
+            const uint32_t q0 = tc::smem_u32(q_tile), ring0 = tc::smem_u32(ring);
+            int at = 0, g0 = sp.g, piece = 0, tile = 0;           // tile: ring position of the piece's first keys
+            int steps[2] = {0, 0};                                // products O += P V issued per half
+            Item it = sp.it;
+            bool good = true;
+            const auto wait = [&](int bar, int parity, int code) {
+                good = good && tc::mbar_wait(&bars[bar], parity & 1, err, code);
+                tc::tc_fence_after();
+            };
+            const auto qk = [&](int t, int slot) {
+                const uint32_t kt = ring0 + slot * L::kTileBytes;
+#pragma unroll
+                for (int part = 0; part < (L::kSplit ? 2 : 1); ++part) {
+                    const uint32_t q = q0 + (t * (L::kSplit ? 2 : 1) + part) * L::kTileBytes;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
+                        mma_ss(s_col(t), tc::desc_sw128(q + off), tc::desc_sw128(kt + off), id_qk, part + k > 0);
+                    }
+                }
+                tc::mma_commit(&bars[kSFull + t]);
+            };
+            const auto pv = [&](int t, int slot, bool first) {
+                const uint32_t vt = ring0 + slot * L::kTileBytes;
+#pragma unroll
+                for (int part = 0; part < (L::kSplit ? 2 : 1); ++part)
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        mma_ts(o_col(t), s_col(t) + part * 64 + k * 8,
+                               tc::smem_desc(vt + k * 2048, D == 64 ? 1024 : 128 * 128, 1024, 2), id_pv,
+                               !first || part + k > 0);
+                tc::mma_commit(&bars[kPvDone + t]);
+                ++steps[t];
+            };
+            while (at < sp.len && good) {
+                const int n = min(it.n, g0 + sp.len - at) - g0, halves = it.rows > kHalf ? 2 : 1;
+                // ring positions: keys of step j at tile + 2 j, values at tile + 2 j + 1
+                wait(kQFull, piece, kKvWait + 2);
+                wait(kTileFull + tile % NS, tile / NS, kKvWait + 3);
+                for (int t = 0; t < halves && good; ++t) {
+                    if (steps[t] > 0) wait(kPvDone + t, steps[t] - 1, kKvWait + 4);
+                    if (good) qk(t, tile % NS);
+                }
+                tc::mma_commit(&bars[kFree + tile % NS]);
+                if (n == 1) tc::mma_commit(&bars[kQFree]);
+                for (int j = 0; j < n && good; ++j) {
+                    const int v = tile + 2 * j + 1, k = v + 1;
+                    wait(kTileFull + v % NS, v / NS, kKvWait + 5);
+                    for (int t = 0; t < halves && good; ++t) {
+                        wait(kPFull + t, steps[t], kKvWait + 6);
+                        if (!good) break;
+                        pv(t, v % NS, j == 0);
+                        if (t == halves - 1) tc::mma_commit(&bars[kFree + v % NS]);
+                        if (j + 1 < n) {
+                            if (t == 0) wait(kTileFull + k % NS, k / NS, kKvWait + 7);
+                            wait(kPvDone + t, steps[t] - 1, kKvWait + 8);   // P lies where the next S goes
+                            if (good) qk(t, k % NS);
+                        }
+                    }
+                    if (j + 1 < n) {
+                        tc::mma_commit(&bars[kFree + k % NS]);
+                        if (j + 2 == n) tc::mma_commit(&bars[kQFree]);
+                    }
+                }
+                tile += 2 * n;
+                at += n;
+                g0 = 0;
+                ++piece;
+                if (at < sp.len) sch.next(it);
+            }
+            tc::mma_commit(&bars[kDrain]);
+            tc::mbar_wait(&bars[kDrain], 0, err, kKvWait + 9);
+        }
+    } else {
+        // ------------------------------------------------------------------------------------------- rows
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int t = warp / 4, row = t * kHalf + (warp % 4) * 32 + lane;
+        const uint32_t lanes = uint32_t((warp % 4) * 32) << 16;
+        int at = 0, g0 = sp.g, piece = 0, step = 0;
+        Item it = sp.it;
+        bool good = true;
+        while (at < sp.len) {
+            const int g1 = min(it.n, g0 + sp.len - at), halves = it.rows > kHalf ? 2 : 1;
+            const int r0 = it.t * kRows, rr = min(row, it.rows - 1), tok = int(group.div(r0 + rr));
+            const int head = it.h * G + (r0 + rr - tok * G);
+            const int p = it.s.len - it.s.n + tok, first = a.window ? p - a.window + 1 : 0;
+            const bool mine = t < halves && good, valid = row < it.rows && good;   // after a failed wait: barriers only
+            float m = -INFINITY, l = 0.f, sc = fabsf(a.scale) * kLog2e;
+            if (mine) {
+                // first and last position of this half's rows: between them some tiles are partly masked
+                const int pa = it.s.len - it.s.n + int(group.div(r0 + t * kHalf));
+                const int pz = it.s.len - it.s.n + int(group.div(r0 + min(it.rows, (t + 1) * kHalf) - 1));
+                const int lo_last = a.window ? max(0, pz - a.window + 1) : 0;
+                for (int g = g0; g < g1 && good; ++g, ++step) {
+                    const int k0 = it.lo + g * kTile;
+                    const bool edge = k0 + kTile > pa + 1 || k0 < lo_last;
+                    good = all_ok(tc::mbar_wait(&bars[kSFull + t], step & 1, err, kKvWait));
+                    if (!good) break;
+                    tc::tc_fence_after();
+                    uint32_t x[128];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        tc::tmem_ld_32x32b_x32(s_col(t) + lanes + i * 32, *reinterpret_cast<uint32_t(*)[32]>(x + i * 32));
+                    tc::tmem_ld_wait();
+                    if (L::kSplit && g == g0) sc = row_scale[(piece & 1) * kRows + row];
+                    if (edge) {
+                        const int from = first - k0, to = p - k0;
+#pragma unroll
+                        for (int i = 0; i < 128; ++i)
+                            if (i < from || i > to) x[i] = 0xff800000u;
+                    }
+                    float top4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) top4[i] = __uint_as_float(x[i]);
+#pragma unroll
+                    for (int i = 4; i < 128; ++i) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(x[i]));
+                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
+                    const bool past = top > m + 8.f;
+                    if (__any_sync(kFull, past)) {
+                        const float mm = past ? top : m, f = past ? ex2(m - mm) : 1.f;
+                        if (g > g0) {
+                            good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
+                            if (!good) break;
+                            tc::tc_fence_after();
+#pragma unroll
+                            for (int i = 0; i < D / 32; ++i) {
+                                uint32_t o[32];
+                                tc::tmem_ld_32x32b_x32(o_col(t) + lanes + i * 32, o);
+                                tc::tmem_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st_x32(o_col(t) + lanes + i * 32, o);
+                            }
+                        }
+                        m = mm;
+                        l *= f;
+                    }
+                    const float base = m == -INFINITY ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < 128; ++i) {
+                        const float w = ex2(fmaf(__uint_as_float(x[i]), sc, -base));
+                        sum[i & 3] += w;
+                        x[i] = __float_as_uint(w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t hi[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            hi[e] = pack2(__uint_as_float(x[i * 64 + 2 * e]), __uint_as_float(x[i * 64 + 2 * e + 1]), !kBf16);
+                        tmem_st_x32(s_col(t) + lanes + i * 32, hi);
+                        if constexpr (L::kSplit) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                                hi[e] = pack2(__uint_as_float(x[i * 64 + 2 * e]) - r.x,
+                                              __uint_as_float(x[i * 64 + 2 * e + 1]) - r.y, true);
+                            }
+                            tmem_st_x32(s_col(t) + lanes + 64 + i * 32, hi);
+                        }
+                    }
+                    tmem_st_wait();
+                    tc::tc_fence_before();
+                    tc::mbar_arrive(&bars[kPFull + t]);
+                }
+                if (good) good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
+                tc::tc_fence_after();
+            }
+            // ---- the piece's result
+            const bool whole = g0 == 0 && g1 == it.n;
+            const int at_slot = 2 * blockIdx.x + (g0 > 0 ? 0 : 1);
+            float* my = slots + (long long)at_slot * slot_floats<D>();
+            T* dst = static_cast<T*>(a.out) + (long long)(it.s.row0 + tok) * a.out_stride + head * D;
+            const auto put = [&](int d, const float (&y)[8], float inv) {     // eight finished values of this row
+                if constexpr (L::kSplit) {
+                    reinterpret_cast<float4*>(dst + d)[0] = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+                    reinterpret_cast<float4*>(dst + d)[1] = make_float4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv);
+                } else {
+                    *reinterpret_cast<uint4*>(dst + d) =
+                        make_uint4(pack2(y[0] * inv, y[1] * inv, !kBf16), pack2(y[2] * inv, y[3] * inv, !kBf16),
+                                   pack2(y[4] * inv, y[5] * inv, !kBf16), pack2(y[6] * inv, y[7] * inv, !kBf16));
+                }
+            };
+            const auto inverse = [&](float mm, float z) {
+                if (a.sinks && z > 0.f) z += ex2(a.sinks[head] * kLog2e - mm);
+                return z == 0.f ? 0.f : 1.f / z;
+            };
+            if (mine && good && flags[piece & 7] == piece + 1) {
+                // a value that some row must not see is NaN or infinite: the piece again, without products of masked values
+                const int klo = it.lo + g0 * kTile, khi = min(it.hi, it.lo + g1 * kTile);
+                for (int i = 0; i < 32; ++i) {
+                    const int r = t * kHalf + (warp % 4) * 32 + i;
+                    if (r >= it.rows) break;
+                    const int tk = int(group.div(r0 + r)), pp = it.s.len - it.s.n + tk, hd = it.h * G + (r0 + r - tk * G);
+                    float mm, ll, oo[D / 32];
+                    careful_row<T, C, D>(c, b, a, it.b, it.h, (long long)(it.s.row0 + tk) * a.q_stride + hd * D,
+                                         max(klo, a.window ? pp - a.window + 1 : 0), min(khi, pp + 1), &mm, &ll, oo);
+                    float z = ll;
+                    if (a.sinks && z > 0.f) z += ex2(a.sinks[hd] * kLog2e - mm);
+                    const float inv = z == 0.f ? 0.f : 1.f / z;
+                    for (int e = 0; e < D / 32; ++e) {
+                        const int d = lane * (D / 32) + e;
+                        if (whole) store_as(a.out, (long long)(it.s.row0 + tk) * a.out_stride + hd * D + d, oo[e] * inv, a.type);
+                        else my[d * kRows + r] = oo[e];
+                    }
+                    if (!whole && lane == 0) {
+                        my[kRows * D + r] = mm;
+                        my[kRows * D + kRows + r] = ll;
+                    }
+                }
+            } else if (mine && good) {
+                const float inv = inverse(m, l);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    uint32_t o[32];
+                    __syncwarp();
+                    tc::tmem_ld_32x32b_x32(o_col(t) + lanes + i * 32, o);
+                    tc::tmem_ld_wait();
+                    if (!valid) {
+                    } else if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            float y[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) y[k] = l == 0.f ? 0.f : __uint_as_float(o[e + k]);
+                            put(i * 32 + e, y, inv);
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) my[(i * 32 + e) * kRows + row] = __uint_as_float(o[e]);
+                    }
+                }
+                if (!whole && valid) {
+                    my[kRows * D + row] = m;
+                    my[kRows * D + kRows + row] = l;
+                }
+            }
+            tc::tc_fence_before();
+            if (!whole) {
+                const long long start = sp.start + at - g0;
+                const int c0 = blockIdx.x - (start < sp.start ? ceil_div(sp.start - start, sp.per) : 0);
+                const int c1 = blockIdx.x + int(unsigned(start + it.n - 1 - sp.start) / unsigned(sp.per));
+                bar_rows();
+                if (threadIdx.x == 0) {
+                    const int n = arrive(&counters[c0]);
+                    flags[8] = n == c1 - c0;
+                    if (n == c1 - c0) counters[c0] = 0;
+                }
+                bar_rows();
+                if (flags[8] && valid) {
+                    float mm = -INFINITY, z = 0.f;
+                    for (int i = c0; i <= c1; ++i)
+                        mm = fmaxf(mm, __ldcg(slots + (long long)(2 * i + (i == c0)) * slot_floats<D>() + kRows * D + row));
+                    const float base = mm == -INFINITY ? 0.f : mm;
+                    for (int i = c0; i <= c1; ++i) {
+                        const float* ps = slots + (long long)(2 * i + (i == c0)) * slot_floats<D>() + kRows * D;
+                        z += __ldcg(ps + kRows + row) * ex2(__ldcg(ps + row) - base);
+                    }
+                    const float inv = inverse(mm, z);
+                    for (int d = 0; d < D; d += 8) {
+                        float y[8] = {};
+                        for (int i = c0; i <= c1; ++i) {
+                            const float* ps = slots + (long long)(2 * i + (i == c0)) * slot_floats<D>();
+                            const float f = ex2(__ldcg(ps + kRows * D + row) - base);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] += __ldcg(ps + (d + e) * kRows + row) * f;
+                        }
+                        put(d, y, inv);
+                    }
+                }
+                bar_rows();                           // flags[8] is read before the next piece sets it
+            }
+            at += g1 - g0;
+            g0 = 0;
+            ++piece;
+            if (at < sp.len) sch.next(it);
+        }
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    if (warp == 12) tc::tmem_dealloc(tmem, 512);
+}
+
+constexpr int kMaxCtas = 160;
+
+template <class T, class C, int D>
+void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    using L = Layout<T, D>;
+    static const cudaError_t attr = cudaFuncSetAttribute(paged_tiles_kernel<T, C, D>,
+                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    GPT_CHECK(attr);
+    paged_tiles_kernel<T, C, D><<<std::min(kMaxCtas, num_sms()), kThreads, L::kSmem, s>>>(
+        c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
+        reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes));
+    check_launch("paged_attention");
+}
+
+}  // namespace
+
+size_t paged_tiles_ws_bytes(int dim) {
+    return kCounterBytes + kMaxCtas * 2 * sizeof(float) * (dim == 64 ? slot_floats<64>() : slot_floats<128>());
+}
+
+void launch_paged_tiles(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    if (c.dim == 64) {
+        if (a.type == kF32) launch<float, __half, 64>(c, b, a, ws, s);
+        else if (a.type == kF16) launch<__half, __half, 64>(c, b, a, ws, s);
+        else launch<__nv_bfloat16, __nv_bfloat16, 64>(c, b, a, ws, s);
+    } else {
+        if (a.type == kF32) launch<float, __half, 128>(c, b, a, ws, s);
+        else if (a.type == kF16) launch<__half, __half, 128>(c, b, a, ws, s);
+        else launch<__nv_bfloat16, __nv_bfloat16, 128>(c, b, a, ws, s);
+    }
+}
+
+}  // namespace gpt

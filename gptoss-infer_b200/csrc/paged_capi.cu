@@ -145,7 +145,7 @@ gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, in
         GPT_CHECK(cudaMalloc(&p->err, sizeof(int)));
         GPT_CHECK(cudaMemset(p->err, 0, sizeof(int)));
         p->pages.err = p->err;
-        const size_t n = gpt::paged_attention_ws_bytes();
+        const size_t n = gpt::paged_attention_ws_bytes(head_dim);
         GPT_CHECK(cudaMalloc(&p->attn_ws, n));
         GPT_CHECK(cudaMemset(p->attn_ws, 0, n));
         GPT_CHECK(cudaDeviceSynchronize());
