@@ -3,7 +3,7 @@
 // The same sum as in paged_attention.cu. An item is 256 query rows (row = token * group + head of the group: all query
 // heads of a key/value head share its tiles) against tiles of 128 keys. Per tile and half of 128 rows:
 //   S = Q K^T            tcgen05.mma kind::f16, both operands in shared memory, K-major, accumulator in TMEM
-//   P = exp2(S - m)      one thread per row: 128 scores in registers, no exchange between threads
+//   P = exp2(S - m)      one thread per row, no exchange between threads
 //   O += P V             A operand P read from TMEM (written over S), V in shared memory as stored (rows = keys)
 // The two halves alternate: while one half's exponentials run, the other half's products do.
 //
@@ -65,20 +65,114 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
         : "memory");
 }
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // A wait's outcome as the whole warp's.
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(kFull, ok); }
+__device__ __forceinline__ void bar_copies() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 __device__ __forceinline__ void bar_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Scores outside [from, to] of a run of 32 or 64 become -infinity.
+__device__ __forceinline__ void mask32(uint32_t (&x)[32], int from, int to) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (i < from || i > to) x[i] = 0xff800000u;
+}
+__device__ __forceinline__ void mask64(uint32_t (&x)[2][32], int from, int to) {
+    mask32(x[0], from, to);
+    mask32(x[1], from - 32, to - 32);
+}
+
+// Column, from S's first, of the weights of keys 32 i .. 32 i + 31 (16 columns; part 1: the low parts). They lie over
+// scores that have been read when they are written: the scores of keys 32 i .. are columns 32 i ...
+template <bool SPLIT>
+__host__ __device__ constexpr int p_col(int i, int part) {
+    return SPLIT ? 32 * i + 16 * part : 16 * i;
+}
+
+// Two fp32 values in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(uint32_t x, uint32_t y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(x), "r"(y));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+
+// The largest of this lane's 128 scores.
+template <bool EDGE>
+__device__ __forceinline__ float row_top(uint32_t s_at, int from, int to) {
+    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t x[2][32];
+        tc::tmem_ld_32x32b_x32(s_at + h * 64, x[0]);
+        tc::tmem_ld_32x32b_x32(s_at + h * 64 + 32, x[1]);
+        tc::tmem_ld_wait();
+        if constexpr (EDGE) mask64(x, from - h * 64, to - h * 64);
+#pragma unroll
+        for (int i = 0; i < 64; i += 2)
+            top[i / 2 & 3] = fmaxf(fmaxf(top[i / 2 & 3], __uint_as_float(x[i >> 5][i & 31])),
+                                   __uint_as_float(x[i >> 5][(i & 31) + 1]));
+    }
+    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+}
+
+// Weights exp2(score * sc + shift) of this lane's 128 scores, written over them; returns their sum.
+template <class C, bool SPLIT, bool EDGE>
+__device__ __forceinline__ float row_weights(uint32_t s_at, float sc, float shift, int from, int to) {
+    constexpr bool half = std::is_same<C, __half>::value;
+    const uint64_t sc2 = pair(__float_as_uint(sc), __float_as_uint(sc)),
+                   shift2 = pair(__float_as_uint(shift), __float_as_uint(shift));
+    uint64_t sum[2] = {0, 0};
+    uint32_t x[2][32];
+    tc::tmem_ld_32x32b_x32(s_at, x[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t(&y)[32] = x[i & 1];
+        tc::tmem_ld_wait();
+        if (i < 3) tc::tmem_ld_32x32b_x32(s_at + (i + 1) * 32, x[~i & 1]);
+        if constexpr (EDGE) mask32(y, from - i * 32, to - i * 32);
+        uint32_t hi[16], lo[SPLIT ? 16 : 1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float u, v;
+            unpair(fma2(pair(y[2 * e], y[2 * e + 1]), sc2, shift2), u, v);
+            u = ex2(u);
+            v = ex2(v);
+            sum[e & 1] = add2(sum[e & 1], pair(__float_as_uint(u), __float_as_uint(v)));
+            hi[e] = pack2(u, v, half);
+            if constexpr (SPLIT) {
+                const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                lo[e] = pack2(u - r.x, v - r.y, true);
+            }
+        }
+        tmem_st_x16(s_at + p_col<SPLIT>(i, 0), hi);
+        if constexpr (SPLIT) tmem_st_x16(s_at + p_col<true>(i, 1), lo);
+    }
+    float a, b, c, d;
+    unpair(sum[0], a, b);
+    unpair(sum[1], c, d);
+    return (a + b) + (c + d);
+}
 
 // Shared-memory image of 128 rows of D 16-bit values: halves of 64 columns, each in the 128-byte swizzled layout. As a
 // K-major operand the rows are M or N; as V the rows are K (8-row groups 1024 bytes apart, 64-column halves 16 KB apart).
@@ -93,7 +187,7 @@ struct Layout {
     static constexpr int kTileBytes = 128 * D * 2;                       // a tile of keys or of values
     static constexpr int kQ = 2 * kTileBytes * (kSplit ? 2 : 1);         // [half][part]
     static constexpr int kSlots = D == 64 ? 8 : (kSplit ? 3 : 5);
-    static constexpr int kSmem = kQ + kSlots * kTileBytes + 2 * kRows * 4 + 512 + 160;
+    static constexpr int kSmem = kQ + kSlots * kTileBytes + 2 * kRows + 2 * kTile * 8 + 416;
 };
 
 template <int D>
@@ -112,10 +206,11 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
     extern __shared__ __align__(1024) char smem[];
     char* q_tile = smem;
     char* ring = smem + L::kQ;
-    float* row_scale = reinterpret_cast<float*>(ring + NS * L::kTileBytes);   // [piece parity][row]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(row_scale + 2 * kRows);
+    int8_t* row_exp = reinterpret_cast<int8_t*>(ring + NS * L::kTileBytes);     // [piece parity][row]: scaled by 2^exp
+    long long* row_off = reinterpret_cast<long long*>(row_exp + 2 * kRows);     // [2][key of the tile]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(row_off + 2 * kTile);
     int* flags = reinterpret_cast<int*>(bars + kBars);                   // [0..7] poisoned piece, [8] last, [9] TMEM
-    long long* scratch = reinterpret_cast<long long*>(reinterpret_cast<char*>(bars) + 512);
+    long long* scratch = reinterpret_cast<long long*>(reinterpret_cast<char*>(bars) + 256);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     int* err = c.err;
@@ -154,18 +249,17 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
 
     if (warp >= 8 && warp < 12) {
         // ------------------------------------------------------------------------------------------- copies
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int tid = threadIdx.x - 256;
         const uint32_t ring0 = tc::smem_u32(ring);
         int issued = 0, done = 0, piece = 0, at = 0, g0 = sp.g;
         Item it = sp.it;
         bool good = true;
         constexpr int kLag = NS >= 5 ? 3 : 2;
-        int info[kLag] = {};                          // per tile in flight: piece + 1 if it is values to be checked
-        const auto complete = [&] {                   // the oldest tile in flight is complete for all threads
+        int check0 = 0, check1 = 0, check2 = 0;       // newest to oldest in flight: piece + 1 if its values are checked
+        const auto complete = [&](int check) {        // the oldest tile in flight is complete for all threads
             tc::fence_proxy_async_smem();
             const int slot = done % NS;
-            if (info[done % kLag]) {
+            if (check) {
                 bool bad = false;
                 for (int i = 0; i < kTile * CH / 128; ++i) {
                     const int r = i * (128 / CH) + tid / CH, ch = tid % CH;
@@ -175,50 +269,66 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
 #pragma unroll
                     for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || (w[k] >> 16 & e) == e;
                 }
-                if (bad) flags[(info[done % kLag] - 1) & 7] = info[done % kLag];
+                if (bad) flags[(check - 1) & 7] = check;
             }
             tc::mbar_arrive(&bars[kTileFull + slot]);
             ++done;
         };
-        const auto issue = [&](int k0, bool values, int check) {
+        // thread k finds key k of a tile: page ids are read a tile ahead, byte offsets shared through row_off (K and V
+        // lie at the same offsets); -1: no such key, filled with zeros
+        int id = 0, pos = 0;
+        const auto look_up = [&](int k0) {
+            pos = k0 + tid;
+            id = pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride + c.page.div(pos)) : -1;
+        };
+        const auto share = [&](int buf) {
+            long long off = -1;
+            if (pos < it.hi) {
+                if (unsigned(id) >= unsigned(c.num_pages)) {
+                    report(err, kKvBadPage);
+                    id = 0;
+                }
+                off = id * c.page_stride + (pos - int(c.page.div(pos) * c.page.d)) * c.token_stride + it.h * c.head_stride;
+            }
+            row_off[buf * kTile + tid] = off;
+            bar_copies();
+        };
+        const uint32_t my_dst = image_off<D>(tid / CH, tid % CH);
+        const auto issue = [&](int buf, bool values, int check) {
             if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1, err, kKvWait));
             if (!good) return;
-            const char* base = (values ? c.v : c.k) + it.h * c.head_stride;
-            const int* table = b.tables + (long long)it.b * b.table_stride;
-            const uint32_t dst = ring0 + (issued % NS) * L::kTileBytes;
-            int ids[kTile * CH / 128];
+            const char* base = (values ? c.v : c.k) + tid % CH * 16;
+            // rows 128 / CH apart: their chunks' places repeat every 8 rows
+            const uint32_t dst = ring0 + (issued % NS) * L::kTileBytes + my_dst;
+            const long long* offs = row_off + buf * kTile + tid / CH;
 #pragma unroll
             for (int i = 0; i < kTile * CH / 128; ++i) {
-                const int pos = k0 + i * (128 / CH) + tid / CH;
-                ids[i] = pos < it.hi ? __ldg(table + c.page.div(pos)) : 0;
-            }
-#pragma unroll
-            for (int i = 0; i < kTile * CH / 128; ++i) {
-                const int r = i * (128 / CH) + tid / CH, ch = tid % CH, pos = k0 + r;
-                const bool ok = pos < it.hi;
-                const char* src = base + ch * 16;
-                if (ok) src += safe_page(ids[i], c) * c.page_stride + (pos - int(c.page.div(pos) * c.page.d)) * c.token_stride;
-                cp_async16_zfill(dst + image_off<D>(r, ch), src, ok);
+                const long long off = offs[i * (128 / CH)];
+                cp_async16_zfill(dst + i * (128 / CH) * 128, base + (off < 0 ? 0 : off), off >= 0);
             }
             cp_async_commit();
-            info[issued % kLag] = check;
+            check2 = check1;
+            check1 = check0;
+            check0 = check;
             ++issued;
             if (issued - done == kLag) {
                 cp_async_wait_group<kLag - 1>();
-                complete();
+                complete(kLag == 3 ? check2 : check1);
             }
         };
-        while (at < sp.len && good) {
+        while (at < sp.len) {                         // after a failed wait: barriers only
             const int g1 = min(it.n, g0 + sp.len - at);
             const int lo_last = a.window ? max(0, it.p1 - a.window + 1) : 0;
-            for (int g = g0; g < g1 && good; ++g) {
+            for (int g = g0; g < g1; ++g) {
                 const int k0 = it.lo + g * kTile;
                 const bool edge = k0 + kTile > it.p0 + 1 || k0 < lo_last;
-                issue(k0, false, 0);
+                if (g == g0) look_up(k0);
+                share(g & 1);
+                if (g + 1 < g1) look_up(k0 + kTile);
+                issue(g & 1, false, 0);
                 if (g == g0) {
                     // queries of this piece, once the previous piece's products have read theirs
-                    if (piece > 0) good = all_ok(good && tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
-                    if (!good) break;
+                    if (piece > 0 && good) good = all_ok(tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
                     const int r0 = it.t * kRows;
                     if constexpr (L::kSplit) {
                         for (int r = warp - 8; r < kRows; r += 4) {
@@ -235,8 +345,8 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                             for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
                             int ex = 0;
                             if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-                            const float up = ldexpf(1.f, min(max(11 - ex, -126), 126));
-                            const float by = a.scale < 0.f ? -up : up;
+                            ex = min(max(11 - ex, -126), 126);
+                            const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, ex);
 #pragma unroll
                             for (int e = 0; e < D / 32; ++e) {
                                 const float y = x[e] * by;
@@ -246,7 +356,7 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                                 *reinterpret_cast<__half*>(p) = hi;
                                 *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
                             }
-                            if (lane == 0) row_scale[(piece & 1) * kRows + r] = fabsf(a.scale) * kLog2e / up;
+                            if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
                         }
                     } else {
                         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
@@ -265,18 +375,19 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                     tc::fence_proxy_async_smem();
                     tc::mbar_arrive(&bars[kQFull]);
                 }
-                issue(k0, true, edge ? piece + 1 : 0);
+                issue(g & 1, true, edge ? piece + 1 : 0);
             }
+            bar_copies();                             // row_off is read before the next piece writes it
             at += g1 - g0;
             g0 = 0;
             ++piece;
             if (at < sp.len) sch.next(it);
         }
         cp_async_wait_group<0>();
-        while (good && done < issued) complete();
+        if (good && issued - done == 2) complete(check1);
+        if (good && issued - done == 1) complete(check0);
     } else if (warp >= 12) {
         // ------------------------------------------------------------------------------------------- products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (warp == 12 && tc::elect_one()) {
             constexpr uint32_t id_qk = idesc_f16(kBf16, false, 128, kTile), id_pv = idesc_f16(kBf16, true, 128, D);
             const uint32_t q0 = tc::smem_u32(q_tile), ring0 = tc::smem_u32(ring);
@@ -307,7 +418,7 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                 for (int part = 0; part < (L::kSplit ? 2 : 1); ++part)
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
-                        mma_ts(o_col(t), s_col(t) + part * 64 + k * 8,
+                        mma_ts(o_col(t), s_col(t) + p_col<L::kSplit>(k / 2, part) + k % 2 * 8,
                                tc::smem_desc(vt + k * 2048, D == 64 ? 1024 : 128 * 128, 1024, 2), id_pv,
                                !first || part + k > 0);
                 tc::mma_commit(&bars[kPvDone + t]);
@@ -354,7 +465,6 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
         }
     } else {
         // ------------------------------------------------------------------------------------------- rows
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
         const int t = warp / 4, row = t * kHalf + (warp % 4) * 32 + lane;
         const uint32_t lanes = uint32_t((warp % 4) * 32) << 16;
         int at = 0, g0 = sp.g, piece = 0, step = 0;
@@ -378,24 +488,11 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                     good = all_ok(tc::mbar_wait(&bars[kSFull + t], step & 1, err, kKvWait));
                     if (!good) break;
                     tc::tc_fence_after();
-                    uint32_t x[128];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        tc::tmem_ld_32x32b_x32(s_col(t) + lanes + i * 32, *reinterpret_cast<uint32_t(*)[32]>(x + i * 32));
-                    tc::tmem_ld_wait();
-                    if (L::kSplit && g == g0) sc = row_scale[(piece & 1) * kRows + row];
-                    if (edge) {
-                        const int from = first - k0, to = p - k0;
-#pragma unroll
-                        for (int i = 0; i < 128; ++i)
-                            if (i < from || i > to) x[i] = 0xff800000u;
-                    }
-                    float top4[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) top4[i] = __uint_as_float(x[i]);
-#pragma unroll
-                    for (int i = 4; i < 128; ++i) top4[i & 3] = fmaxf(top4[i & 3], __uint_as_float(x[i]));
-                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
+                    if (L::kSplit && g == g0) sc *= __int_as_float((127 - row_exp[(piece & 1) * kRows + row]) << 23);
+                    // the row's largest score; then, 32 scores at a time, the weights, each over scores already read
+                    const int from = first - k0, to = p - k0;
+                    const uint32_t s_at = s_col(t) + lanes;
+                    const float top = (edge ? row_top<true>(s_at, from, to) : row_top<false>(s_at, 0, 0)) * sc;
                     const bool past = top > m + 8.f;
                     if (__any_sync(kFull, past)) {
                         const float mm = past ? top : m, f = past ? ex2(m - mm) : 1.f;
@@ -403,45 +500,22 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                             good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
                             if (!good) break;
                             tc::tc_fence_after();
-#pragma unroll
-                            for (int i = 0; i < D / 32; ++i) {
-                                uint32_t o[32];
-                                tc::tmem_ld_32x32b_x32(o_col(t) + lanes + i * 32, o);
+#pragma unroll 1
+                            for (int i = 0; i < D / 16; ++i) {
+                                uint32_t o[16];
+                                tc::tmem_ld_32x32b_x16(o_col(t) + lanes + i * 16, o);
                                 tc::tmem_ld_wait();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                                tmem_st_x32(o_col(t) + lanes + i * 32, o);
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st_x16(o_col(t) + lanes + i * 16, o);
                             }
                         }
                         m = mm;
                         l *= f;
                     }
                     const float base = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int i = 0; i < 128; ++i) {
-                        const float w = ex2(fmaf(__uint_as_float(x[i]), sc, -base));
-                        sum[i & 3] += w;
-                        x[i] = __float_as_uint(w);
-                    }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        uint32_t hi[32];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            hi[e] = pack2(__uint_as_float(x[i * 64 + 2 * e]), __uint_as_float(x[i * 64 + 2 * e + 1]), !kBf16);
-                        tmem_st_x32(s_col(t) + lanes + i * 32, hi);
-                        if constexpr (L::kSplit) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-                                hi[e] = pack2(__uint_as_float(x[i * 64 + 2 * e]) - r.x,
-                                              __uint_as_float(x[i * 64 + 2 * e + 1]) - r.y, true);
-                            }
-                            tmem_st_x32(s_col(t) + lanes + 64 + i * 32, hi);
-                        }
-                    }
+                    l += edge ? row_weights<C, L::kSplit, true>(s_at, sc, -base, from, to)
+                              : row_weights<C, L::kSplit, false>(s_at, sc, -base, 0, 0);
                     tmem_st_wait();
                     tc::tc_fence_before();
                     tc::mbar_arrive(&bars[kPFull + t]);
