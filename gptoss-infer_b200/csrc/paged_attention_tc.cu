@@ -4,8 +4,9 @@
 // heads of a key/value head share its tiles) against tiles of 128 keys. Per tile and half of 128 rows:
 //   S = Q K^T            tcgen05.mma kind::f16, both operands in shared memory, K-major, accumulator in TMEM
 //   P = exp2(S - m)      one thread per row, no exchange between threads
-//   O += P V             A operand P read from TMEM (written over S), V in shared memory as stored (rows = keys)
-// The two halves alternate: while one half's exponentials run, the other half's products do.
+//   O += P V             A operand P read from TMEM, V in shared memory as stored (rows = keys)
+// S is taken in tiles of 64 keys, read into registers and released at once, so the next scores are made while this
+// tile's exponentials run; the two halves run half a step apart.
 //
 // Bound: with heads of 64 the exponentials (128 x 128 per 4.2 MFLOP, 16 a clock and SM), with heads of 128 the products.
 //
@@ -79,22 +80,12 @@ __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(kFull, ok); 
 __device__ __forceinline__ void bar_copies() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
 __device__ __forceinline__ void bar_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Scores outside [from, to] of a run of 32 or 64 become -infinity.
-__device__ __forceinline__ void mask32(uint32_t (&x)[32], int from, int to) {
+// Scores outside [from, to] become -infinity.
+template <int N>
+__device__ __forceinline__ void mask(uint32_t (&x)[N], int from, int to) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < N; ++i)
         if (i < from || i > to) x[i] = 0xff800000u;
-}
-__device__ __forceinline__ void mask64(uint32_t (&x)[2][32], int from, int to) {
-    mask32(x[0], from, to);
-    mask32(x[1], from - 32, to - 32);
-}
-
-// Column, from S's first, of the weights of keys 32 i .. 32 i + 31 (16 columns; part 1: the low parts). They lie over
-// scores that have been read when they are written: the scores of keys 32 i .. are columns 32 i ...
-template <bool SPLIT>
-__host__ __device__ constexpr int p_col(int i, int part) {
-    return SPLIT ? 32 * i + 16 * part : 16 * i;
 }
 
 // Two fp32 values in a register pair: one instruction for both.
@@ -117,56 +108,31 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
-// The largest of this lane's 128 scores.
-template <bool EDGE>
-__device__ __forceinline__ float row_top(uint32_t s_at, int from, int to) {
-    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        uint32_t x[2][32];
-        tc::tmem_ld_32x32b_x32(s_at + h * 64, x[0]);
-        tc::tmem_ld_32x32b_x32(s_at + h * 64 + 32, x[1]);
-        tc::tmem_ld_wait();
-        if constexpr (EDGE) mask64(x, from - h * 64, to - h * 64);
-#pragma unroll
-        for (int i = 0; i < 64; i += 2)
-            top[i / 2 & 3] = fmaxf(fmaxf(top[i / 2 & 3], __uint_as_float(x[i >> 5][i & 31])),
-                                   __uint_as_float(x[i >> 5][(i & 31) + 1]));
-    }
-    return fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-}
-
-// Weights exp2(score * sc + shift) of this lane's 128 scores, written over them; returns their sum.
-template <class C, bool SPLIT, bool EDGE>
-__device__ __forceinline__ float row_weights(uint32_t s_at, float sc, float shift, int from, int to) {
+// Weights exp2(score * sc + shift) in place: words 0 .. N / 2 - 1 become the 16-bit weights, two a word, the next N / 2
+// (SPLIT) what rounding took from them. Returns the fp32 weights' sum.
+template <class C, bool SPLIT, int N>
+__device__ __forceinline__ float weights(uint32_t (&x)[N], float sc, float shift) {
     constexpr bool half = std::is_same<C, __half>::value;
     const uint64_t sc2 = pair(__float_as_uint(sc), __float_as_uint(sc)),
                    shift2 = pair(__float_as_uint(shift), __float_as_uint(shift));
     uint64_t sum[2] = {0, 0};
-    uint32_t x[2][32];
-    tc::tmem_ld_32x32b_x32(s_at, x[0]);
+    uint32_t low[SPLIT ? N / 2 : 1];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t(&y)[32] = x[i & 1];
-        tc::tmem_ld_wait();
-        if (i < 3) tc::tmem_ld_32x32b_x32(s_at + (i + 1) * 32, x[~i & 1]);
-        if constexpr (EDGE) mask32(y, from - i * 32, to - i * 32);
-        uint32_t hi[16], lo[SPLIT ? 16 : 1];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float u, v;
-            unpair(fma2(pair(y[2 * e], y[2 * e + 1]), sc2, shift2), u, v);
-            u = ex2(u);
-            v = ex2(v);
-            sum[e & 1] = add2(sum[e & 1], pair(__float_as_uint(u), __float_as_uint(v)));
-            hi[e] = pack2(u, v, half);
-            if constexpr (SPLIT) {
-                const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-                lo[e] = pack2(u - r.x, v - r.y, true);
-            }
+    for (int e = 0; e < N / 2; ++e) {
+        float u, v;
+        unpair(fma2(pair(x[2 * e], x[2 * e + 1]), sc2, shift2), u, v);
+        u = ex2(u);
+        v = ex2(v);
+        sum[e & 1] = add2(sum[e & 1], pair(__float_as_uint(u), __float_as_uint(v)));
+        x[e] = pack2(u, v, half);
+        if constexpr (SPLIT) {
+            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&x[e]));
+            low[e] = pack2(u - r.x, v - r.y, true);
         }
-        tmem_st_x16(s_at + p_col<SPLIT>(i, 0), hi);
-        if constexpr (SPLIT) tmem_st_x16(s_at + p_col<true>(i, 1), lo);
+    }
+    if constexpr (SPLIT) {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) x[N / 2 + e] = low[e];
     }
     float a, b, c, d;
     unpair(sum[0], a, b);
@@ -184,6 +150,7 @@ __device__ __forceinline__ uint32_t image_off(int r, int chunk) {
 template <class T, int D>
 struct Layout {
     static constexpr bool kSplit = sizeof(T) == 4;
+    static constexpr int kScores = 64;                                   // keys of a score tile in TMEM
     static constexpr int kTileBytes = 128 * D * 2;                       // a tile of keys or of values
     static constexpr int kQ = 2 * kTileBytes * (kSplit ? 2 : 1);         // [half][part]
     static constexpr int kSlots = D == 64 ? 8 : (kSplit ? 3 : 5);
@@ -195,13 +162,13 @@ __host__ __device__ constexpr int slot_floats() {
     return kRows * D + 2 * kRows;                                        // sums [dim][row], maxima, sums of weights
 }
 
-enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kPFull = 18, kPvDone = 20, kQFull = 22, kQFree = 23, kDrain = 24, kBars = 25 };
+enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kSFree = 18, kPFull = 20, kPvDone = 22, kQFull = 24, kQFree = 25, kDrain = 26, kBars = 27 };
 
 template <class T, class C, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* counters, float* slots) {
     using L = Layout<T, D>;
-    constexpr int NS = L::kSlots, CH = D / 8;
+    constexpr int NS = L::kSlots, CH = D / 8, SK = L::kScores, SUB = kTile / SK;
     constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
     extern __shared__ __align__(1024) char smem[];
     char* q_tile = smem;
@@ -226,6 +193,7 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
         }
         for (int t = 0; t < 2; ++t) {
             tc::mbar_init(&bars[kSFull + t], 1);
+            tc::mbar_init(&bars[kSFree + t], 128);
             tc::mbar_init(&bars[kPFull + t], 128);
             tc::mbar_init(&bars[kPvDone + t], 1);
         }
@@ -243,9 +211,10 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = uint32_t(flags[9]);
-    // TMEM columns: S (and P over it) of half t at 128 t, O at 256 + 128 t
-    const auto s_col = [&](int t) { return tmem + 128 * t; };
-    const auto o_col = [&](int t) { return tmem + 256 + 128 * t; };
+    // TMEM columns of half t, from 256 t: S [0, SK), P [SK, SK + SK / 2), its low parts the next SK / 2, O the last D
+    const auto s_col = [&](int t) { return tmem + 256 * t; };
+    const auto p_col = [&](int t, int part) { return tmem + 256 * t + SK + part * (SK / 2); };
+    const auto o_col = [&](int t) { return tmem + 256 * t + 256 - D; };
 
     if (warp >= 8 && warp < 12) {
         // ------------------------------------------------------------------------------------------- copies
@@ -389,71 +358,70 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
     } else if (warp >= 12) {
         // ------------------------------------------------------------------------------------------- products
         if (warp == 12 && tc::elect_one()) {
-            constexpr uint32_t id_qk = idesc_f16(kBf16, false, 128, kTile), id_pv = idesc_f16(kBf16, true, 128, D);
+            constexpr uint32_t id_qk = idesc_f16(kBf16, false, 128, SK), id_pv = idesc_f16(kBf16, true, 128, D);
             const uint32_t q0 = tc::smem_u32(q_tile), ring0 = tc::smem_u32(ring);
             int at = 0, g0 = sp.g, piece = 0, tile = 0;           // tile: ring position of the piece's first keys
-            int steps[2] = {0, 0};                                // products O += P V issued per half
+            int made[2] = {0, 0}, used[2] = {0, 0};               // score tiles and weight tiles issued per half
             Item it = sp.it;
             bool good = true;
             const auto wait = [&](int bar, int parity, int code) {
                 good = good && tc::mbar_wait(&bars[bar], parity & 1, err, code);
                 tc::tc_fence_after();
             };
-            const auto qk = [&](int t, int slot) {
-                const uint32_t kt = ring0 + slot * L::kTileBytes;
-#pragma unroll
-                for (int part = 0; part < (L::kSplit ? 2 : 1); ++part) {
-                    const uint32_t q = q0 + (t * (L::kSplit ? 2 : 1) + part) * L::kTileBytes;
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-                        mma_ss(s_col(t), tc::desc_sw128(q + off), tc::desc_sw128(kt + off), id_qk, part + k > 0);
-                    }
-                }
-                tc::mma_commit(&bars[kSFull + t]);
-            };
-            const auto pv = [&](int t, int slot, bool first) {
-                const uint32_t vt = ring0 + slot * L::kTileBytes;
-#pragma unroll
-                for (int part = 0; part < (L::kSplit ? 2 : 1); ++part)
-#pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        mma_ts(o_col(t), s_col(t) + p_col<L::kSplit>(k / 2, part) + k % 2 * 8,
-                               tc::smem_desc(vt + k * 2048, D == 64 ? 1024 : 128 * 128, 1024, 2), id_pv,
-                               !first || part + k > 0);
-                tc::mma_commit(&bars[kPvDone + t]);
-                ++steps[t];
-            };
             while (at < sp.len && good) {
-                const int n = min(it.n, g0 + sp.len - at) - g0, halves = it.rows > kHalf ? 2 : 1;
-                // ring positions: keys of step j at tile + 2 j, values at tile + 2 j + 1
-                wait(kQFull, piece, kKvWait + 2);
-                wait(kTileFull + tile % NS, tile / NS, kKvWait + 3);
-                for (int t = 0; t < halves && good; ++t) {
-                    if (steps[t] > 0) wait(kPvDone + t, steps[t] - 1, kKvWait + 4);
-                    if (good) qk(t, tile % NS);
-                }
-                tc::mma_commit(&bars[kFree + tile % NS]);
-                if (n == 1) tc::mma_commit(&bars[kQFree]);
-                for (int j = 0; j < n && good; ++j) {
-                    const int v = tile + 2 * j + 1, k = v + 1;
-                    wait(kTileFull + v % NS, v / NS, kKvWait + 5);
-                    for (int t = 0; t < halves && good; ++t) {
-                        wait(kPFull + t, steps[t], kKvWait + 6);
-                        if (!good) break;
-                        pv(t, v % NS, j == 0);
-                        if (t == halves - 1) tc::mma_commit(&bars[kFree + v % NS]);
-                        if (j + 1 < n) {
-                            if (t == 0) wait(kTileFull + k % NS, k / NS, kKvWait + 7);
-                            wait(kPvDone + t, steps[t] - 1, kKvWait + 8);   // P lies where the next S goes
-                            if (good) qk(t, k % NS);
+                const int n = min(it.n, g0 + sp.len - at) - g0, steps = n * SUB;
+                const bool two = it.rows > kHalf;
+                // ring positions: keys of tile j at tile + 2 j, values at tile + 2 j + 1
+                const auto qk = [&](int t, int u) {               // scores of keys SK u .. of the piece
+                    const int pos = tile + u / SUB * 2;
+                    if (t == 0 && u % SUB == 0) wait(kTileFull + pos % NS, pos / NS, kKvWait + 3);
+                    if (made[t] > 0) wait(kSFree + t, made[t] - 1, kKvWait + 4);
+                    if (!good) return;
+                    const uint32_t kt = ring0 + pos % NS * L::kTileBytes + u % SUB * (SK * 128);
+#pragma unroll
+                    for (int part = 0; part < (L::kSplit ? 2 : 1); ++part) {
+                        const uint32_t q = q0 + (t * (L::kSplit ? 2 : 1) + part) * L::kTileBytes;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
+                            mma_ss(s_col(t), tc::desc_sw128(q + off), tc::desc_sw128(kt + off), id_qk, part + k > 0);
                         }
                     }
-                    if (j + 1 < n) {
-                        tc::mma_commit(&bars[kFree + k % NS]);
-                        if (j + 2 == n) tc::mma_commit(&bars[kQFree]);
+                    tc::mma_commit(&bars[kSFull + t]);
+                    ++made[t];
+                    if (t == int(two)) {
+                        if (u % SUB == SUB - 1) tc::mma_commit(&bars[kFree + pos % NS]);
+                        if (u == steps - 1) tc::mma_commit(&bars[kQFree]);
                     }
+                };
+                const auto pv = [&](int t, int u) {
+                    const int pos = tile + u / SUB * 2 + 1;
+                    if (t == 0 && u % SUB == 0) wait(kTileFull + pos % NS, pos / NS, kKvWait + 5);
+                    wait(kPFull + t, used[t], kKvWait + 6);
+                    if (!good) return;
+                    const uint32_t vt = ring0 + pos % NS * L::kTileBytes + u % SUB * (SK * 128);
+#pragma unroll
+                    for (int part = 0; part < (L::kSplit ? 2 : 1); ++part)
+#pragma unroll
+                        for (int k = 0; k < SK / 16; ++k)
+                            mma_ts(o_col(t), p_col(t, part) + k * 8,
+                                   tc::smem_desc(vt + k * 2048, D == 64 ? 1024 : 128 * 128, 1024, 2), id_pv,
+                                   u > 0 || part + k > 0);
+                    tc::mma_commit(&bars[kPvDone + t]);
+                    ++used[t];
+                    if (t == int(two) && u % SUB == SUB - 1) tc::mma_commit(&bars[kFree + pos % NS]);
+                };
+                wait(kQFull, piece, kKvWait + 2);
+                qk(0, 0);
+                if (two) qk(1, 0);
+                // the halves half a step apart: one's products run while the other's weights are computed
+                for (int u = 0; u < steps && good; ++u) {
+                    if (u + 1 < steps) qk(0, u + 1);
+                    if (two && u > 0) pv(1, u - 1);
+                    if (two && u + 1 < steps) qk(1, u + 1);
+                    pv(0, u);
                 }
+                if (two && good) pv(1, steps - 1);
                 tile += 2 * n;
                 at += n;
                 g0 = 0;
@@ -482,21 +450,30 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                 const int pa = it.s.len - it.s.n + int(group.div(r0 + t * kHalf));
                 const int pz = it.s.len - it.s.n + int(group.div(r0 + min(it.rows, (t + 1) * kHalf) - 1));
                 const int lo_last = a.window ? max(0, pz - a.window + 1) : 0;
-                for (int g = g0; g < g1 && good; ++g, ++step) {
-                    const int k0 = it.lo + g * kTile;
-                    const bool edge = k0 + kTile > pa + 1 || k0 < lo_last;
+                for (int g = g0 * SUB; g < g1 * SUB && good; ++g, ++step) {
+                    const int k0 = it.lo + g * SK;
+                    const bool edge = k0 + SK > pa + 1 || k0 < lo_last;
                     good = all_ok(tc::mbar_wait(&bars[kSFull + t], step & 1, err, kKvWait));
                     if (!good) break;
                     tc::tc_fence_after();
-                    if (L::kSplit && g == g0) sc *= __int_as_float((127 - row_exp[(piece & 1) * kRows + row]) << 23);
-                    // the row's largest score; then, 32 scores at a time, the weights, each over scores already read
-                    const int from = first - k0, to = p - k0;
-                    const uint32_t s_at = s_col(t) + lanes;
-                    const float top = (edge ? row_top<true>(s_at, from, to) : row_top<false>(s_at, 0, 0)) * sc;
+                    uint32_t x[SK];
+#pragma unroll
+                    for (int i = 0; i < SK; i += 32)
+                        tc::tmem_ld_32x32b_x32(s_col(t) + lanes + i, *reinterpret_cast<uint32_t(*)[32]>(x + i));
+                    tc::tmem_ld_wait();
+                    tc::tc_fence_before();
+                    tc::mbar_arrive(&bars[kSFree + t]);   // the next scores may be written
+                    if (L::kSplit && g == g0 * SUB) sc *= __int_as_float((127 - row_exp[(piece & 1) * kRows + row]) << 23);
+                    if (edge) mask<SK>(x, first - k0, p - k0);
+                    float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < SK; i += 2)
+                        top4[i / 2 & 3] = fmaxf(fmaxf(top4[i / 2 & 3], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
                     const bool past = top > m + 8.f;
                     if (__any_sync(kFull, past)) {
                         const float mm = past ? top : m, f = past ? ex2(m - mm) : 1.f;
-                        if (g > g0) {
+                        if (g > g0 * SUB) {
                             good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
                             if (!good) break;
                             tc::tc_fence_after();
@@ -514,8 +491,15 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                         l *= f;
                     }
                     const float base = m == -INFINITY ? 0.f : m;
-                    l += edge ? row_weights<C, L::kSplit, true>(s_at, sc, -base, from, to)
-                              : row_weights<C, L::kSplit, false>(s_at, sc, -base, 0, 0);
+                    l += weights<C, L::kSplit, SK>(x, sc, -base);
+                    if (step > 0) good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
+                    if (!good) break;
+                    tc::tc_fence_after();             // the products have read the previous weights
+#pragma unroll
+                    for (int i = 0; i < SK / 2; i += 16) {
+                        tmem_st_x16(p_col(t, 0) + lanes + i, x + i);
+                        if constexpr (L::kSplit) tmem_st_x16(p_col(t, 1) + lanes + i, x + SK / 2 + i);
+                    }
                     tmem_st_wait();
                     tc::tc_fence_before();
                     tc::mbar_arrive(&bars[kPFull + t]);
