@@ -2,6 +2,7 @@
 // host launchers. Every launcher throws std::runtime_error on a launch failure; the C ABI (paged_capi.cu) checks the
 // arguments first and turns exceptions into -1.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstddef>
@@ -43,6 +44,12 @@ struct KvView {
     int num_pages, kv_heads, dim;
     FastDiv page;            // division by the page size
     int* err;
+    int layer, box_log;      // coordinates of KvMaps: the layer, 2^box_log slots per box (below 3: no maps)
+};
+
+// Tensor maps of a pool, [layer][page][slot][head][dim] in boxes of 2^box_log slots x 64 dims with the 128-byte swizzle.
+struct KvMaps {
+    CUtensorMap k, v;
 };
 
 // Sequence b's new tokens are rows cu[b] .. cu[b + 1) of the batch; its cache holds lens[b] positions with them.
@@ -75,8 +82,8 @@ struct PagedAttnArgs {
 constexpr size_t kCounterBytes = 2048;            // of both kernels, before the partial results
 size_t paged_attention_ws_bytes(int dim);
 size_t paged_tiles_ws_bytes(int dim);
-void launch_paged_tiles(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
-void launch_paged_attention(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
+void launch_paged_tiles(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
+void launch_paged_attention(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
 
 struct BeamArgs {
     const void* logits;

@@ -137,7 +137,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
     __shared__ long long scratch[kWarps + 2];
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Schedule<R, kGroup> sch{c, b, a.window, group};
+    const Schedule<R, kGroup> sch{c, b, a.window, group, 1};
     const Span sp = find_span<kThreads>(sch, kWarps * (NS - 1), scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
@@ -592,8 +592,8 @@ size_t paged_attention_ws_bytes(int dim) {
     return std::max(kCounterBytes + kMaxCtas * 2 * sizeof(float) * kSlotFloats, paged_tiles_ws_bytes(dim));
 }
 
-void launch_paged_attention(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
-    if ((long long)b.max_new * (a.q_heads / c.kv_heads) > 64) return launch_paged_tiles(c, b, a, ws, s);
+void launch_paged_attention(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    if ((long long)b.max_new * (a.q_heads / c.kv_heads) > 64) return launch_paged_tiles(maps, c, b, a, ws, s);
     if (a.type == kF32) by_shape<float, __half>(c, b, a, ws, s);
     else if (a.type == kF16) by_shape<__half, __half>(c, b, a, ws, s);
     else by_shape<__nv_bfloat16, __nv_bfloat16>(c, b, a, ws, s);

@@ -10,8 +10,9 @@
 //
 // Bound: with heads of 64 the exponentials (128 x 128 per 4.2 MFLOP, 16 a clock and SM), with heads of 128 the products.
 //
-// Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output), 8-11 copy keys and values (16-byte
-// asynchronous copies through a ring of tiles; any page size), 12 issues the products. The running maximum moves only when
+// Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output); the next two copy keys and values through a
+// ring of tiles with TMA (a box per run of slots in a page; page sizes that are multiples of 8), or the next four with
+// 16-byte asynchronous copies (any page size); one more issues the products. The running maximum moves only when
 // it grows by more than 2^8, so the accumulator in TMEM is rescaled rarely (weights stay at most 256).
 //
 // fp32 queries: two fp16 parts of a row scaled by a power of two, and two of the weights, as in paged_attention.cu.
@@ -27,7 +28,14 @@ namespace {
 
 using namespace paged;
 
-constexpr int kThreads = 512, kRows = 256, kHalf = 128, kTile = 128;
+constexpr int kRows = 256, kHalf = 128, kTile = 128;
+// Threads that bring in keys, values and queries: two warps with TMA, four without; one warp more issues the products.
+constexpr int copy_threads(bool tma) { return tma ? 64 : 128; }
+constexpr int block_threads(bool tma) { return tma ? 384 : 512; }
+#ifndef KMIX
+#define KMIX 3
+#endif
+constexpr int kMixed = KMIX;      // of 8 pairs of exponentials, those on the fp32 pipes
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -37,6 +45,15 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+// 5-D tiled TMA load: 64 dims (128 bytes, swizzled) x slots of one head, page and layer.
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int d, int h, int slot, int page,
+                                            int layer, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(d), "r"(h), "r"(slot), "r"(page), "r"(layer), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -49,6 +66,14 @@ __device__ __forceinline__ void cp_async_wait_group() {
 __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, bool turned, int M, int N) {
     return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(turned) << 16) |
            (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
+}
+// Shared-memory descriptors in the 128-byte swizzled layout: the high word (stride between 8-row groups 1024 bytes,
+// version 1, layout 2) is common to all, the low word is the address and the leading offset, both in 16-byte units.
+__device__ __forceinline__ uint64_t desc_of(uint32_t low) {
+    constexpr uint32_t high = (1024u >> 4) | (1u << 14) | (2u << 29);
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+    return d;
 }
 // D (+)= A B^T, A and B in shared memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -77,7 +102,8 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // A wait's outcome as the whole warp's.
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(kFull, ok); }
-__device__ __forceinline__ void bar_copies() { asm volatile("bar.sync 2, 128;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void bar_copies() { asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bar_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 // Scores outside [from, to] become -infinity.
@@ -108,31 +134,65 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
-// Weights exp2(score * sc + shift) in place: words 0 .. N / 2 - 1 become the 16-bit weights, two a word, the next N / 2
-// (SPLIT) what rounding took from them. Returns the fp32 weights' sum.
-template <class C, bool SPLIT, int N>
-__device__ __forceinline__ float weights(uint32_t (&x)[N], float sc, float shift) {
+// 2^x of two values on the fp32 pipes: x = n + f with n = round(x), |f| <= 1/2 (the sum with 1.5 * 2^23 leaves n in the
+// low mantissa bits), 2^f by the polynomial of least largest relative error on [-1/2, 1/2] (weighted least squares
+// iterated to equal ripple; degree 3: 7.5e-5, degree 4: 2.6e-6), n added to its exponent. x below -126 counts as -126.
+template <int DEGREE>
+__device__ __forceinline__ void exp2_pair(uint64_t x2, float& u, float& v) {
+    const auto both = [](float c) { return pair(__float_as_uint(c), __float_as_uint(c)); };
+    float a, b;
+    unpair(x2, a, b);
+    x2 = pair(__float_as_uint(fmaxf(a, -126.f)), __float_as_uint(fmaxf(b, -126.f)));
+    const uint64_t r = add2(x2, both(12582912.f)), f = fma2(add2(r, both(-12582912.f)), both(-1.f), x2);
+    uint64_t y;
+    if constexpr (DEGREE == 3) {
+        y = fma2(both(0.0551716685f), f, both(0.242611125f));
+        y = fma2(y, f, both(0.693260968f));
+        y = fma2(y, f, both(0.999928057f));
+    } else {
+        y = fma2(both(0.0095701022f), f, both(0.0559178591f));
+        y = fma2(y, f, both(0.240247443f));
+        y = fma2(y, f, both(0.693121791f));
+        y = fma2(y, f, both(0.999999285f));
+    }
+    float ya, yb, ra, rb;
+    unpair(y, ya, yb);
+    unpair(r, ra, rb);
+    u = __uint_as_float(__float_as_uint(ya) + (__float_as_uint(ra) << 23));
+    v = __uint_as_float(__float_as_uint(yb) + (__float_as_uint(rb) << 23));
+}
+
+// Weights exp2(score * sc + shift) as 16-bit values, two a TMEM column, to p_at; SPLIT: what rounding took from them to
+// p_low. Returns the fp32 weights' sum. MIX: kMixed of every 8 pairs on the fp32 pipes.
+template <class C, bool SPLIT, bool MIX, int N>
+__device__ __forceinline__ float weights(const uint32_t (&x)[N], float sc, float shift, uint32_t p_at, uint32_t p_low) {
     constexpr bool half = std::is_same<C, __half>::value;
     const uint64_t sc2 = pair(__float_as_uint(sc), __float_as_uint(sc)),
                    shift2 = pair(__float_as_uint(shift), __float_as_uint(shift));
     uint64_t sum[2] = {0, 0};
-    uint32_t low[SPLIT ? N / 2 : 1];
 #pragma unroll
-    for (int e = 0; e < N / 2; ++e) {
-        float u, v;
-        unpair(fma2(pair(x[2 * e], x[2 * e + 1]), sc2, shift2), u, v);
-        u = ex2(u);
-        v = ex2(v);
-        sum[e & 1] = add2(sum[e & 1], pair(__float_as_uint(u), __float_as_uint(v)));
-        x[e] = pack2(u, v, half);
-        if constexpr (SPLIT) {
-            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&x[e]));
-            low[e] = pack2(u - r.x, v - r.y, true);
+    for (int i = 0; i < N; i += 32) {
+        uint32_t hi[16], low[SPLIT ? 16 : 1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const uint64_t x2 = fma2(pair(x[i + 2 * e], x[i + 2 * e + 1]), sc2, shift2);
+            float u, v;
+            if (MIX && e * kMixed % 8 < kMixed) {
+                exp2_pair<half ? 4 : 3>(x2, u, v);
+            } else {
+                unpair(x2, u, v);
+                u = ex2(u);
+                v = ex2(v);
+            }
+            sum[e & 1] = add2(sum[e & 1], pair(__float_as_uint(u), __float_as_uint(v)));
+            hi[e] = pack2(u, v, half);
+            if constexpr (SPLIT) {
+                const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                low[e] = pack2(u - r.x, v - r.y, true);
+            }
         }
-    }
-    if constexpr (SPLIT) {
-#pragma unroll
-        for (int e = 0; e < N / 2; ++e) x[N / 2 + e] = low[e];
+        tmem_st_x16(p_at + i / 2, hi);
+        if constexpr (SPLIT) tmem_st_x16(p_low + i / 2, low);
     }
     float a, b, c, d;
     unpair(sum[0], a, b);
@@ -147,10 +207,10 @@ __device__ __forceinline__ uint32_t image_off(int r, int chunk) {
     return uint32_t((chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
 }
 
-template <class T, int D>
+template <class T, int D, bool TMA>
 struct Layout {
     static constexpr bool kSplit = sizeof(T) == 4;
-    static constexpr int kScores = 64;                                   // keys of a score tile in TMEM
+    static constexpr int kScores = TMA && D == 64 && !kSplit ? 128 : 64;        // keys of a score tile in TMEM
     static constexpr int kTileBytes = 128 * D * 2;                       // a tile of keys or of values
     static constexpr int kQ = 2 * kTileBytes * (kSplit ? 2 : 1);         // [half][part]
     static constexpr int kSlots = D == 64 ? 8 : (kSplit ? 3 : 5);
@@ -162,14 +222,17 @@ __host__ __device__ constexpr int slot_floats() {
     return kRows * D + 2 * kRows;                                        // sums [dim][row], maxima, sums of weights
 }
 
-enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kSFree = 18, kPFull = 20, kPvDone = 22, kQFull = 24, kQFree = 25, kDrain = 26, kBars = 27 };
+enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kSFree = 18, kPFull = 20, kPvDone = 22, kQFull = 24, kQFree = 25, kDrain = 26, kEdge = 27, kBars = 28 };
 
-template <class T, class C, int D>
-__global__ void __launch_bounds__(kThreads, 1)
-paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* counters, float* slots) {
-    using L = Layout<T, D>;
+template <class T, class C, int D, bool TMA>
+__global__ void __launch_bounds__(block_threads(TMA), 1)
+paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* counters,
+                   float* slots) {
+    using L = Layout<T, D, TMA>;
+    constexpr int kThreads = block_threads(TMA), kCopy = copy_threads(TMA);
     constexpr int NS = L::kSlots, CH = D / 8, SK = L::kScores, SUB = kTile / SK;
     constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
+    constexpr int kMma = 8 + kCopy / 32;              // the warp that issues the products
     extern __shared__ __align__(1024) char smem[];
     char* q_tile = smem;
     char* ring = smem + L::kQ;
@@ -181,14 +244,14 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     int* err = c.err;
-    const Schedule<kRows, kTile> sch{c, b, a.window, group};
+    const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1};
     const Span sp = find_span<kThreads>(sch, 2, scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
-            tc::mbar_init(&bars[kTileFull + i], 128);
+            tc::mbar_init(&bars[kTileFull + i], TMA ? 1 : kCopy);
             tc::mbar_init(&bars[kFree + i], 1);
         }
         for (int t = 0; t < 2; ++t) {
@@ -197,13 +260,14 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
             tc::mbar_init(&bars[kPFull + t], 128);
             tc::mbar_init(&bars[kPvDone + t], 1);
         }
-        tc::mbar_init(&bars[kQFull], 128);
+        tc::mbar_init(&bars[kQFull], kCopy);
         tc::mbar_init(&bars[kQFree], 1);
         tc::mbar_init(&bars[kDrain], 1);
+        tc::mbar_init(&bars[kEdge], 1);
         tc::fence_barrier_init();
         for (int i = 0; i < 8; ++i) flags[i] = 0;
     }
-    if (warp == 12) {
+    if (warp == kMma) {
         tc::tmem_alloc(reinterpret_cast<uint32_t*>(&flags[9]), 512);
         tc::tmem_relinquish();
     }
@@ -216,13 +280,139 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
     const auto p_col = [&](int t, int part) { return tmem + 256 * t + SK + part * (SK / 2); };
     const auto o_col = [&](int t) { return tmem + 256 * t + 256 - D; };
 
-    if (warp >= 8 && warp < 12) {
+    if (warp >= 8 && warp < kMma) {
         // ------------------------------------------------------------------------------------------- copies
         const int tid = threadIdx.x - 256;
         const uint32_t ring0 = tc::smem_u32(ring);
-        int issued = 0, done = 0, piece = 0, at = 0, g0 = sp.g;
+        int issued = 0, piece = 0, at = 0, g0 = sp.g;
         Item it = sp.it;
         bool good = true;
+        // queries of a piece, once the previous piece's products have read theirs
+        const auto load_queries = [&] {
+                                if (piece > 0 && good) good = all_ok(tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
+                                const int r0 = it.t * kRows;
+                                if constexpr (L::kSplit) {
+                                    for (int r = warp - 8; r < kRows; r += kCopy / 32) {
+                                        float x[D / 32], top = 0.f;
+                                        const int tok = int(group.div(r0 + r));
+                                        const float* src = static_cast<const float*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
+                                                           (it.h * G + (r0 + r - tok * G)) * D + lane * (D / 32);
+            #pragma unroll
+                                        for (int e = 0; e < D / 32; ++e) {
+                                            x[e] = r < it.rows ? src[e] : 0.f;
+                                            top = fmaxf(top, fabsf(x[e]));
+                                        }
+            #pragma unroll
+                                        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                                        int ex = 0;
+                                        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+                                        ex = min(max(11 - ex, -126), 126);
+                                        const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, ex);
+            #pragma unroll
+                                        for (int e = 0; e < D / 32; ++e) {
+                                            const float y = x[e] * by;
+                                            const __half hi = __float2half_rn(y);
+                                            const int d = lane * (D / 32) + e;
+                                            char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) + d % 8 * 2;
+                                            *reinterpret_cast<__half*>(p) = hi;
+                                            *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
+                                        }
+                                        if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
+                                    }
+                                } else {
+                                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+            #pragma unroll 8
+                                    for (int u = tid; u < kRows * CH; u += kCopy) {
+                                        const int r = u / CH, ch = u % CH, tok = int(group.div(r0 + r));
+                                        uint4 x = make_uint4(0, 0, 0, 0);
+                                        if (r < it.rows)
+                                            x = __ldg(reinterpret_cast<const uint4*>(
+                                                static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
+                                                (it.h * G + (r0 + r - tok * G)) * D + ch * 8));
+                                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                                        *reinterpret_cast<uint4*>(q_tile + (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch)) = x;
+                                    }
+                                }
+                                tc::fence_proxy_async_smem();
+                                tc::mbar_arrive(&bars[kQFull]);
+        };
+        // 16 bytes of values that some row must not see (NaN or infinity would reach it through a product)
+        const auto not_finite = [](const uint4& x) {
+            constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            bool bad = false;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || (w[k] >> 16 & e) == e;
+            return bad;
+        };
+        const auto wait_free = [&] {                  // until the ring's next place is free
+            if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1, err, kKvWait));
+        };
+        if constexpr (TMA) {
+            // lane x of the first copying warp brings box x of a tile: 2^box_log slots of one page, one copy per 64 dims
+            const int box = 1 << c.box_log, boxes = kTile >> c.box_log;
+            int id = -1, edges = 0;
+            const auto look_up = [&](int k0) {
+                const int pos = k0 + lane * box;
+                id = lane < boxes && pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride + c.page.div(pos)) : -1;
+            };
+            const auto issue = [&](const CUtensorMap* map, int k0, int page, uint64_t* bar) {
+                wait_free();
+                if (good && warp == 8) {
+                    const int pos = k0 + lane * box;
+                    const bool mine = lane < boxes && pos < it.hi;
+                    const int n = __popc(__ballot_sync(kFull, mine));
+                    if (lane == 0) tc::mbar_arrive_expect_tx(bar, uint32_t(n * box * D * 2));
+                    __syncwarp();
+                    if (mine) {
+                        const int slot = pos - int(c.page.div(pos) * c.page.d);
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h)
+                            tma_load_5d(ring0 + issued % NS * L::kTileBytes + h * (128 * 128) + lane * box * 128, map, h * 64,
+                                        it.h, slot, page, c.layer, tc::smem_u32(bar));
+                    }
+                    __syncwarp();
+                }
+                ++issued;
+            };
+            while (at < sp.len) {                     // after a failed wait: barriers only
+                const int g1 = min(it.n, g0 + sp.len - at);
+                const int lo_last = a.window ? max(0, it.p1 - a.window + 1) : 0;
+                look_up(it.lo + g0 * kTile);
+                for (int g = g0; g < g1; ++g) {
+                    const int k0 = it.lo + g * kTile;
+                    const bool edge = k0 + kTile > it.p0 + 1 || k0 < lo_last;
+                    const int page = id < 0 && !(lane < boxes && k0 + lane * box < it.hi) ? 0 : safe_page(id, c);
+                    issue(&maps.k, k0, page, &bars[kTileFull + issued % NS]);
+                    if (g + 1 < g1) look_up(k0 + kTile);
+                    if (g == g0) load_queries();
+                    const int slot = issued % NS;
+                    issue(&maps.v, k0, page, &bars[edge ? int(kEdge) : kTileFull + slot]);
+                    if (edge) {
+                        // some row does not see all of these values: slots past the sequence's end (whatever they hold)
+                        // become zeros, and the others are checked
+                        if (good) good = all_ok(tc::mbar_wait(&bars[kEdge], edges & 1, err, kKvWait + 1));
+                        ++edges;
+                        bool bad = false;
+                        for (int i = tid; i < kTile * CH && good; i += kCopy) {
+                            const int r = i / CH;
+                            uint4* x = reinterpret_cast<uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, i % CH));
+                            if (k0 + r >= it.hi) *x = make_uint4(0, 0, 0, 0);
+                            else bad |= not_finite(*x);
+                        }
+                        if (bad) flags[piece & 7] = piece + 1;
+                        tc::fence_proxy_async_smem();
+                        bar_copies<kCopy>();
+                        if (tid == 0 && good) tc::mbar_arrive(&bars[kTileFull + slot]);
+                    }
+                }
+                at += g1 - g0;
+                g0 = 0;
+                ++piece;
+                if (at < sp.len) sch.next(it);
+            }
+        } else {
+        int done = 0;
         constexpr int kLag = NS >= 5 ? 3 : 2;
         int check0 = 0, check1 = 0, check2 = 0;       // newest to oldest in flight: piece + 1 if its values are checked
         const auto complete = [&](int check) {        // the oldest tile in flight is complete for all threads
@@ -230,50 +420,57 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
             const int slot = done % NS;
             if (check) {
                 bool bad = false;
-                for (int i = 0; i < kTile * CH / 128; ++i) {
-                    const int r = i * (128 / CH) + tid / CH, ch = tid % CH;
-                    const uint4 x = *reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, ch));
-                    constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
-                    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || (w[k] >> 16 & e) == e;
+                for (int i = 0; i < kTile * CH / kCopy; ++i) {
+                    const int r = i * (kCopy / CH) + tid / CH, ch = tid % CH;
+                    bad |= not_finite(*reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, ch)));
                 }
                 if (bad) flags[(check - 1) & 7] = check;
             }
             tc::mbar_arrive(&bars[kTileFull + slot]);
             ++done;
         };
-        // thread k finds key k of a tile: page ids are read a tile ahead, byte offsets shared through row_off (K and V
-        // lie at the same offsets); -1: no such key, filled with zeros
-        int id = 0, pos = 0;
+        // thread k finds keys k and k + 64 of a tile: page ids are read a tile ahead, byte offsets shared through row_off
+        // (K and V lie at the same offsets); -1: no such key, filled with zeros
+        int id[kTile / kCopy], pos0 = 0;
         const auto look_up = [&](int k0) {
-            pos = k0 + tid;
-            id = pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride + c.page.div(pos)) : -1;
+            pos0 = k0 + tid;
+#pragma unroll
+            for (int i = 0; i < kTile / kCopy; ++i) {
+                const int pos = pos0 + i * kCopy;
+                id[i] = pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride + c.page.div(pos)) : -1;
+            }
         };
         const auto share = [&](int buf) {
-            long long off = -1;
-            if (pos < it.hi) {
-                if (unsigned(id) >= unsigned(c.num_pages)) {
-                    report(err, kKvBadPage);
-                    id = 0;
+#pragma unroll
+            for (int i = 0; i < kTile / kCopy; ++i) {
+                const int pos = pos0 + i * kCopy;
+                long long off = -1;
+                if (pos < it.hi) {
+                    if (unsigned(id[i]) >= unsigned(c.num_pages)) {
+                        report(err, kKvBadPage);
+                        id[i] = 0;
+                    }
+                    off = id[i] * c.page_stride + (pos - int(c.page.div(pos) * c.page.d)) * c.token_stride +
+                          it.h * c.head_stride;
                 }
-                off = id * c.page_stride + (pos - int(c.page.div(pos) * c.page.d)) * c.token_stride + it.h * c.head_stride;
+                row_off[buf * kTile + tid + i * kCopy] = off;
             }
-            row_off[buf * kTile + tid] = off;
-            bar_copies();
+            bar_copies<kCopy>();
         };
         const uint32_t my_dst = image_off<D>(tid / CH, tid % CH);
         const auto issue = [&](int buf, bool values, int check) {
-            if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1, err, kKvWait));
+            wait_free();
             if (!good) return;
             const char* base = (values ? c.v : c.k) + tid % CH * 16;
-            // rows 128 / CH apart: their chunks' places repeat every 8 rows
+            // rows kCopy / CH apart: a chunk's place repeats every 8 rows
+            constexpr int kStep = kCopy / CH;
             const uint32_t dst = ring0 + (issued % NS) * L::kTileBytes + my_dst;
             const long long* offs = row_off + buf * kTile + tid / CH;
 #pragma unroll
-            for (int i = 0; i < kTile * CH / 128; ++i) {
-                const long long off = offs[i * (128 / CH)];
-                cp_async16_zfill(dst + i * (128 / CH) * 128, base + (off < 0 ? 0 : off), off >= 0);
+            for (int i = 0; i < kTile / kStep; ++i) {
+                const long long off = offs[i * kStep];
+                const uint32_t to = kStep % 8 == 0 || i % 2 == 0 ? dst : dst ^ 64;   // four rows on: chunk ^ 4
+                cp_async16_zfill(to + i * kStep * 128, base + (off < 0 ? 0 : off), off >= 0);
             }
             cp_async_commit();
             check2 = check1;
@@ -295,58 +492,10 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                 share(g & 1);
                 if (g + 1 < g1) look_up(k0 + kTile);
                 issue(g & 1, false, 0);
-                if (g == g0) {
-                    // queries of this piece, once the previous piece's products have read theirs
-                    if (piece > 0 && good) good = all_ok(tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
-                    const int r0 = it.t * kRows;
-                    if constexpr (L::kSplit) {
-                        for (int r = warp - 8; r < kRows; r += 4) {
-                            float x[D / 32], top = 0.f;
-                            const int tok = int(group.div(r0 + r));
-                            const float* src = static_cast<const float*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
-                                               (it.h * G + (r0 + r - tok * G)) * D + lane * (D / 32);
-#pragma unroll
-                            for (int e = 0; e < D / 32; ++e) {
-                                x[e] = r < it.rows ? src[e] : 0.f;
-                                top = fmaxf(top, fabsf(x[e]));
-                            }
-#pragma unroll
-                            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-                            int ex = 0;
-                            if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-                            ex = min(max(11 - ex, -126), 126);
-                            const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, ex);
-#pragma unroll
-                            for (int e = 0; e < D / 32; ++e) {
-                                const float y = x[e] * by;
-                                const __half hi = __float2half_rn(y);
-                                const int d = lane * (D / 32) + e;
-                                char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) + d % 8 * 2;
-                                *reinterpret_cast<__half*>(p) = hi;
-                                *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
-                            }
-                            if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
-                        }
-                    } else {
-                        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-#pragma unroll 4
-                        for (int u = tid; u < kRows * CH; u += 128) {
-                            const int r = u / CH, ch = u % CH, tok = int(group.div(r0 + r));
-                            uint4 x = make_uint4(0, 0, 0, 0);
-                            if (r < it.rows)
-                                x = __ldg(reinterpret_cast<const uint4*>(
-                                    static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
-                                    (it.h * G + (r0 + r - tok * G)) * D + ch * 8));
-                            x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                            *reinterpret_cast<uint4*>(q_tile + (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch)) = x;
-                        }
-                    }
-                    tc::fence_proxy_async_smem();
-                    tc::mbar_arrive(&bars[kQFull]);
-                }
+                if (g == g0) load_queries();
                 issue(g & 1, true, edge ? piece + 1 : 0);
             }
-            bar_copies();                             // row_off is read before the next piece writes it
+            bar_copies<kCopy>();                             // row_off is read before the next piece writes it
             at += g1 - g0;
             g0 = 0;
             ++piece;
@@ -355,11 +504,14 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
         cp_async_wait_group<0>();
         if (good && issued - done == 2) complete(check1);
         if (good && issued - done == 1) complete(check0);
-    } else if (warp >= 12) {
+        }
+    } else if (warp >= kMma) {
         // ------------------------------------------------------------------------------------------- products
-        if (warp == 12 && tc::elect_one()) {
+        if (warp == kMma && tc::elect_one()) {
             constexpr uint32_t id_qk = idesc_f16(kBf16, false, 128, SK), id_pv = idesc_f16(kBf16, true, 128, D);
-            const uint32_t q0 = tc::smem_u32(q_tile), ring0 = tc::smem_u32(ring);
+            // low descriptor words; leading offset: unused (1) for the K-major ones, between 64-dim halves for V
+            const uint32_t q0 = tc::smem_u32(q_tile) >> 4 | 1u << 16, ring0 = tc::smem_u32(ring) >> 4;
+            constexpr uint32_t k_lead = 1u << 16, v_lead = (D == 64 ? 1024u : 128u * 128u) >> 4 << 16;
             int at = 0, g0 = sp.g, piece = 0, tile = 0;           // tile: ring position of the piece's first keys
             int made[2] = {0, 0}, used[2] = {0, 0};               // score tiles and weight tiles issued per half
             Item it = sp.it;
@@ -377,14 +529,14 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                     if (t == 0 && u % SUB == 0) wait(kTileFull + pos % NS, pos / NS, kKvWait + 3);
                     if (made[t] > 0) wait(kSFree + t, made[t] - 1, kKvWait + 4);
                     if (!good) return;
-                    const uint32_t kt = ring0 + pos % NS * L::kTileBytes + u % SUB * (SK * 128);
+                    const uint32_t kt = (ring0 | k_lead) + (pos % NS * L::kTileBytes + u % SUB * (SK * 128)) / 16;
 #pragma unroll
                     for (int part = 0; part < (L::kSplit ? 2 : 1); ++part) {
-                        const uint32_t q = q0 + (t * (L::kSplit ? 2 : 1) + part) * L::kTileBytes;
+                        const uint32_t q = q0 + (t * (L::kSplit ? 2 : 1) + part) * (L::kTileBytes / 16);
 #pragma unroll
                         for (int k = 0; k < D / 16; ++k) {
-                            const uint32_t off = (k / 4) * (128 * 128) + (k % 4) * 32;
-                            mma_ss(s_col(t), tc::desc_sw128(q + off), tc::desc_sw128(kt + off), id_qk, part + k > 0);
+                            const uint32_t off = ((k / 4) * (128 * 128) + (k % 4) * 32) / 16;
+                            mma_ss(s_col(t), desc_of(q + off), desc_of(kt + off), id_qk, part + k > 0);
                         }
                     }
                     tc::mma_commit(&bars[kSFull + t]);
@@ -399,14 +551,12 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                     if (t == 0 && u % SUB == 0) wait(kTileFull + pos % NS, pos / NS, kKvWait + 5);
                     wait(kPFull + t, used[t], kKvWait + 6);
                     if (!good) return;
-                    const uint32_t vt = ring0 + pos % NS * L::kTileBytes + u % SUB * (SK * 128);
+                    const uint32_t vt = (ring0 | v_lead) + (pos % NS * L::kTileBytes + u % SUB * (SK * 128)) / 16;
 #pragma unroll
                     for (int part = 0; part < (L::kSplit ? 2 : 1); ++part)
 #pragma unroll
                         for (int k = 0; k < SK / 16; ++k)
-                            mma_ts(o_col(t), p_col(t, part) + k * 8,
-                                   tc::smem_desc(vt + k * 2048, D == 64 ? 1024 : 128 * 128, 1024, 2), id_pv,
-                                   u > 0 || part + k > 0);
+                            mma_ts(o_col(t), p_col(t, part) + k * 8, desc_of(vt + k * 2048 / 16), id_pv, u > 0 || part + k > 0);
                     tc::mma_commit(&bars[kPvDone + t]);
                     ++used[t];
                     if (t == int(two) && u % SUB == SUB - 1) tc::mma_commit(&bars[kFree + pos % NS]);
@@ -491,15 +641,15 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
                         l *= f;
                     }
                     const float base = m == -INFINITY ? 0.f : m;
-                    l += weights<C, L::kSplit, SK>(x, sc, -base);
                     if (step > 0) good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
                     if (!good) break;
                     tc::tc_fence_after();             // the products have read the previous weights
-#pragma unroll
-                    for (int i = 0; i < SK / 2; i += 16) {
-                        tmem_st_x16(p_col(t, 0) + lanes + i, x + i);
-                        if constexpr (L::kSplit) tmem_st_x16(p_col(t, 1) + lanes + i, x + SK / 2 + i);
-                    }
+                    const uint32_t p_at = p_col(t, 0) + lanes, p_low = p_col(t, 1) + lanes;
+                    // a row without a key so far needs exact zeros
+                    if (L::kSplit || edge || __any_sync(kFull, m == -INFINITY))
+                        l += weights<C, L::kSplit, false, SK>(x, sc, -base, p_at, p_low);
+                    else
+                        l += weights<C, L::kSplit, true, SK>(x, sc, -base, p_at, p_low);
                     tmem_st_wait();
                     tc::tc_fence_before();
                     tc::mbar_arrive(&bars[kPFull + t]);
@@ -619,21 +769,27 @@ paged_tiles_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* cou
     }
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 12) tc::tmem_dealloc(tmem, 512);
+    if (warp == kMma) tc::tmem_dealloc(tmem, 512);
 }
 
 constexpr int kMaxCtas = 160;
 
-template <class T, class C, int D>
-void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
-    using L = Layout<T, D>;
-    static const cudaError_t attr = cudaFuncSetAttribute(paged_tiles_kernel<T, C, D>,
+template <class T, class C, int D, bool TMA>
+void launch(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    using L = Layout<T, D, TMA>;
+    static const cudaError_t attr = cudaFuncSetAttribute(paged_tiles_kernel<T, C, D, TMA>,
                                                          cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
     GPT_CHECK(attr);
-    paged_tiles_kernel<T, C, D><<<std::min(kMaxCtas, num_sms()), kThreads, L::kSmem, s>>>(
-        c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
+    paged_tiles_kernel<T, C, D, TMA><<<std::min(kMaxCtas, num_sms()), block_threads(TMA), L::kSmem, s>>>(
+        maps, c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
         reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes));
     check_launch("paged_attention");
+}
+
+template <class T, class C, int D>
+void by_copy(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    if (c.box_log >= 3) launch<T, C, D, true>(maps, c, b, a, ws, s);
+    else launch<T, C, D, false>(maps, c, b, a, ws, s);
 }
 
 }  // namespace
@@ -642,15 +798,16 @@ size_t paged_tiles_ws_bytes(int dim) {
     return kCounterBytes + kMaxCtas * 2 * sizeof(float) * (dim == 64 ? slot_floats<64>() : slot_floats<128>());
 }
 
-void launch_paged_tiles(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+void launch_paged_tiles(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
+                        cudaStream_t s) {
     if (c.dim == 64) {
-        if (a.type == kF32) launch<float, __half, 64>(c, b, a, ws, s);
-        else if (a.type == kF16) launch<__half, __half, 64>(c, b, a, ws, s);
-        else launch<__nv_bfloat16, __nv_bfloat16, 64>(c, b, a, ws, s);
+        if (a.type == kF32) by_copy<float, __half, 64>(m, c, b, a, ws, s);
+        else if (a.type == kF16) by_copy<__half, __half, 64>(m, c, b, a, ws, s);
+        else by_copy<__nv_bfloat16, __nv_bfloat16, 64>(m, c, b, a, ws, s);
     } else {
-        if (a.type == kF32) launch<float, __half, 128>(c, b, a, ws, s);
-        else if (a.type == kF16) launch<__half, __half, 128>(c, b, a, ws, s);
-        else launch<__nv_bfloat16, __nv_bfloat16, 128>(c, b, a, ws, s);
+        if (a.type == kF32) by_copy<float, __half, 128>(m, c, b, a, ws, s);
+        else if (a.type == kF16) by_copy<__half, __half, 128>(m, c, b, a, ws, s);
+        else by_copy<__nv_bfloat16, __nv_bfloat16, 128>(m, c, b, a, ws, s);
     }
 }
 

@@ -11,12 +11,15 @@
 #include "common.cuh"
 #include "gptoss.h"
 #include "paged.h"
+#include "tma.h"
 
 using gpt::abi_guard;
 using gpt::require;
 
 struct gptoss_kv_pool {
     gpt::KvPages pages{};
+    gpt::KvMaps maps{};
+    int box_log = 0;
     gpt::FastDiv div{};
     int type = 0, dim = 0, device = 0;
     int* err = nullptr;
@@ -36,6 +39,8 @@ struct gptoss_kv_pool {
         v.dim = dim;
         v.page = div;
         v.err = err;
+        v.layer = layer;
+        v.box_log = box_log;
         return v;
     }
     ~gptoss_kv_pool() {
@@ -141,6 +146,7 @@ gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, in
         p->type = type;
         p->dim = head_dim;
         p->div = gpt::FastDiv::of(uint32_t(page_size));
+        p->box_log = gpt::make_kv_maps(p->pages, head_dim, type == gpt::kBF16, &p->maps);
         GPT_CHECK(cudaGetDevice(&p->device));
         GPT_CHECK(cudaMalloc(&p->err, sizeof(int)));
         GPT_CHECK(cudaMemset(p->err, 0, sizeof(int)));
@@ -215,7 +221,7 @@ int gptoss_paged_attention(gptoss_kv_pool* p, int layer, const gptoss_kv_batch* 
                 "paged_attention: too many tokens in one call");
         check_device(p, "paged_attention");
         gpt::PagedAttnArgs a{q, out, sinks, q_stride, out_stride, type, p->type, q_heads, window, scale};
-        gpt::launch_paged_attention(p->view(layer), b, a, p->attn_ws, static_cast<cudaStream_t>(stream));
+        gpt::launch_paged_attention(p->maps, p->view(layer), b, a, p->attn_ws, static_cast<cudaStream_t>(stream));
     });
 }
 

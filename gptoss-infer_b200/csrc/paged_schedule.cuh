@@ -28,6 +28,7 @@ struct Schedule {
     const KvBatch& b;
     int window;
     FastDiv group;
+    int align;               // lo is a multiple of this (a power of two)
 
     __device__ __forceinline__ int row_tiles(int n) const { return (n * int(group.d) + R - 1) / R; }
 
@@ -36,7 +37,7 @@ struct Schedule {
         it.rows = min(R, it.s.n * int(group.d) - r0);
         it.p0 = it.s.len - it.s.n + int(group.div(r0));
         it.p1 = it.s.len - it.s.n + int(group.div(r0 + it.rows - 1));
-        it.lo = window ? max(0, it.p0 - window + 1) : 0;
+        it.lo = window ? max(0, it.p0 - window + 1) & -align : 0;
         it.hi = max(it.lo, it.p1 + 1);
         it.n = max(1, (it.hi - it.lo + UNIT - 1) / UNIT);
     }

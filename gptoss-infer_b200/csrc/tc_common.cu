@@ -12,6 +12,7 @@
 #include "kernels.h"
 #include "tc.cuh"
 #include "terms.cuh"
+#include "paged.h"
 #include "tma.h"
 
 namespace gpt {
@@ -83,6 +84,29 @@ CUtensorMap make_tmap_u8_swz_3d(const void* base, uint64_t row_bytes, uint64_t r
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled (3d) failed: " + std::to_string(int(r)));
     return m;
+}
+
+int make_kv_maps(const KvPages& p, int dim, bool bf16, KvMaps* maps) {
+    int log = 0;
+    while (log < 7 && p.page_size % (2 << log) == 0) ++log;
+    if (log < 3) return 0;
+    const cuuint64_t dims[5] = {cuuint64_t(dim), cuuint64_t(p.kv_heads), cuuint64_t(p.page_size), cuuint64_t(p.num_pages),
+                                cuuint64_t(p.layers)};
+    const long long bytes[4] = {p.head_stride, p.token_stride, p.page_stride, p.layer_stride};
+    cuuint64_t strides[4];
+    for (int i = 0; i < 4; ++i) {
+        if (dims[i + 1] > 1 && (bytes[i] <= 0 || bytes[i] >= (1ll << 40))) return 0;
+        strides[i] = dims[i + 1] > 1 ? cuuint64_t(bytes[i]) : 16;        // one element: never stepped
+    }
+    const cuuint32_t box[5] = {64, 1, 1u << log, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
+    for (CUtensorMap* m : {&maps->k, &maps->v}) {
+        const CUresult r = encoder()(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                                     m == &maps->k ? p.k : p.v, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_SUCCESS) return 0;
+    }
+    return log;
 }
 
 CUtensorMap make_tmap_u8_sw128_3d(const void* base, uint64_t row_bytes, uint64_t rows, uint64_t mats,

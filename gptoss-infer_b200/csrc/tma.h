@@ -25,4 +25,11 @@ CUtensorMap make_tmap_u8_swz(const void* base, uint64_t row_bytes, uint64_t rows
 CUtensorMap make_tmap_u8_swz_3d(const void* base, uint64_t row_bytes, uint64_t rows, uint64_t mats,
                                 uint32_t box_bytes, uint32_t box_rows, uint32_t swizzle_bytes);
 
+// Maps of a paged cache's keys and values (see KvMaps). Returns log2 of the slots of a box: the largest power of two up to
+// 128 that divides the page size; 0 where there can be no maps (page sizes that are no multiple of 8, strides that TMA
+// does not take).
+struct KvPages;
+struct KvMaps;
+int make_kv_maps(const KvPages& p, int dim, bool bf16, KvMaps* maps);
+
 }  // namespace gpt
