@@ -6,7 +6,7 @@
 //   P = exp2(S - m)      one thread per row, no exchange between threads
 //   O += P V             A operand P read from TMEM, V in shared memory as stored (rows = keys)
 // S is taken in tiles of 64 keys, read into registers and released at once, so the next scores are made while this
-// tile's exponentials run; the two halves run half a step apart.
+// tile's exponentials run; while one half waits for products the other computes.
 //
 // Bound: with heads of 64 the exponentials (128 x 128 per 4.2 MFLOP, 16 a clock and SM), with heads of 128 the products.
 //
@@ -32,10 +32,9 @@ constexpr int kRows = 256, kHalf = 128, kTile = 128;
 // Threads that bring in keys, values and queries: two warps with TMA, four without; one warp more issues the products.
 constexpr int copy_threads(bool tma) { return tma ? 64 : 128; }
 constexpr int block_threads(bool tma) { return tma ? 384 : 512; }
-#ifndef KMIX
-#define KMIX 3
-#endif
-constexpr int kMixed = KMIX;      // of 8 pairs of exponentials, those on the fp32 pipes
+// Of 8 pairs of exponentials, those computed on the fp32 pipes beside the special-function unit (2048 tokens over 16384,
+// heads of 64, bf16: 0 of 8 747 us, 2 748, 3 790; heads of 128: 551, 540, 546).
+constexpr int kMixed = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -75,7 +74,8 @@ __device__ __forceinline__ uint64_t desc_of(uint32_t low) {
     asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
     return d;
 }
-// D (+)= A B^T, A and B in shared memory.
+// D (+)= A B^T, A and B in shared memory. Issued by one thread; M = 128, K = 16 takes 48, 64 and 128 cycles for N = 64,
+// 128 and 256.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -83,7 +83,7 @@ __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint3
         "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(accumulate))
         : "memory");
 }
-// D (+)= A B, A in TMEM (one lane per row, two 16-bit values per column).
+// D (+)= A B, A in TMEM (one lane per row, two 16-bit values per column): 32 and 64 cycles for N = 64 and 128.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -102,6 +102,11 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // A wait's outcome as the whole warp's.
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(kFull, ok); }
+// One arrival for the whole warp, after all its lanes' work (32 arrivals on one barrier take turns).
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) tc::mbar_arrive(bar);
+}
 template <int N>
 __device__ __forceinline__ void bar_copies() { asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bar_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
@@ -214,7 +219,7 @@ struct Layout {
     static constexpr int kTileBytes = 128 * D * 2;                       // a tile of keys or of values
     static constexpr int kQ = 2 * kTileBytes * (kSplit ? 2 : 1);         // [half][part]
     static constexpr int kSlots = D == 64 ? 8 : (kSplit ? 3 : 5);
-    static constexpr int kSmem = kQ + kSlots * kTileBytes + 2 * kRows + 2 * kTile * 8 + 416;
+    static constexpr int kSmem = kQ + kSlots * kTileBytes + 2 * kRows + 2 * kTile * 8 + 512;
 };
 
 template <int D>
@@ -240,9 +245,9 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
     long long* row_off = reinterpret_cast<long long*>(row_exp + 2 * kRows);     // [2][key of the tile]
     uint64_t* bars = reinterpret_cast<uint64_t*>(row_off + 2 * kTile);
     int* flags = reinterpret_cast<int*>(bars + kBars);                   // [0..7] poisoned piece, [8] last, [9] TMEM
-    long long* scratch = reinterpret_cast<long long*>(reinterpret_cast<char*>(bars) + 256);
+    long long* scratch = reinterpret_cast<long long*>(reinterpret_cast<char*>(bars) + 352);
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = int(threadIdx.x / 32), lane = threadIdx.x % 32;
     int* err = c.err;
     const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1};
     const Span sp = find_span<kThreads>(sch, 2, scratch);
@@ -251,16 +256,16 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) {
-            tc::mbar_init(&bars[kTileFull + i], TMA ? 1 : kCopy);
+            tc::mbar_init(&bars[kTileFull + i], TMA ? 1 : kCopy / 32);
             tc::mbar_init(&bars[kFree + i], 1);
         }
         for (int t = 0; t < 2; ++t) {
             tc::mbar_init(&bars[kSFull + t], 1);
-            tc::mbar_init(&bars[kSFree + t], 128);
-            tc::mbar_init(&bars[kPFull + t], 128);
+            tc::mbar_init(&bars[kSFree + t], 4);
+            tc::mbar_init(&bars[kPFull + t], 4);
             tc::mbar_init(&bars[kPvDone + t], 1);
         }
-        tc::mbar_init(&bars[kQFull], kCopy);
+        tc::mbar_init(&bars[kQFull], kCopy / 32);
         tc::mbar_init(&bars[kQFree], 1);
         tc::mbar_init(&bars[kDrain], 1);
         tc::mbar_init(&bars[kEdge], 1);
@@ -289,52 +294,52 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
         bool good = true;
         // queries of a piece, once the previous piece's products have read theirs
         const auto load_queries = [&] {
-                                if (piece > 0 && good) good = all_ok(tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
-                                const int r0 = it.t * kRows;
-                                if constexpr (L::kSplit) {
-                                    for (int r = warp - 8; r < kRows; r += kCopy / 32) {
-                                        float x[D / 32], top = 0.f;
-                                        const int tok = int(group.div(r0 + r));
-                                        const float* src = static_cast<const float*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
-                                                           (it.h * G + (r0 + r - tok * G)) * D + lane * (D / 32);
-            #pragma unroll
-                                        for (int e = 0; e < D / 32; ++e) {
-                                            x[e] = r < it.rows ? src[e] : 0.f;
-                                            top = fmaxf(top, fabsf(x[e]));
-                                        }
-            #pragma unroll
-                                        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-                                        int ex = 0;
-                                        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-                                        ex = min(max(11 - ex, -126), 126);
-                                        const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, ex);
-            #pragma unroll
-                                        for (int e = 0; e < D / 32; ++e) {
-                                            const float y = x[e] * by;
-                                            const __half hi = __float2half_rn(y);
-                                            const int d = lane * (D / 32) + e;
-                                            char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) + d % 8 * 2;
-                                            *reinterpret_cast<__half*>(p) = hi;
-                                            *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
-                                        }
-                                        if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
-                                    }
-                                } else {
-                                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-            #pragma unroll 8
-                                    for (int u = tid; u < kRows * CH; u += kCopy) {
-                                        const int r = u / CH, ch = u % CH, tok = int(group.div(r0 + r));
-                                        uint4 x = make_uint4(0, 0, 0, 0);
-                                        if (r < it.rows)
-                                            x = __ldg(reinterpret_cast<const uint4*>(
-                                                static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
-                                                (it.h * G + (r0 + r - tok * G)) * D + ch * 8));
-                                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                                        *reinterpret_cast<uint4*>(q_tile + (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch)) = x;
-                                    }
-                                }
-                                tc::fence_proxy_async_smem();
-                                tc::mbar_arrive(&bars[kQFull]);
+                if (piece > 0 && good) good = all_ok(tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
+                const int r0 = it.t * kRows;
+                if constexpr (L::kSplit) {
+                    for (int r = warp - 8; r < kRows; r += kCopy / 32) {
+                        float x[D / 32], top = 0.f;
+                        const int tok = int(group.div(r0 + r));
+                        const float* src = static_cast<const float*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
+                                           (it.h * G + (r0 + r - tok * G)) * D + lane * (D / 32);
+#pragma unroll
+                        for (int e = 0; e < D / 32; ++e) {
+                            x[e] = r < it.rows ? src[e] : 0.f;
+                            top = fmaxf(top, fabsf(x[e]));
+                        }
+#pragma unroll
+                        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                        int ex = 0;
+                        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
+                        ex = min(max(11 - ex, -126), 126);
+                        const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, ex);
+#pragma unroll
+                        for (int e = 0; e < D / 32; ++e) {
+                            const float y = x[e] * by;
+                            const __half hi = __float2half_rn(y);
+                            const int d = lane * (D / 32) + e;
+                            char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) + d % 8 * 2;
+                            *reinterpret_cast<__half*>(p) = hi;
+                            *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
+                        }
+                        if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
+                    }
+                } else {
+                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll 8
+                    for (int u = tid; u < kRows * CH; u += kCopy) {
+                        const int r = u / CH, ch = u % CH, tok = int(group.div(r0 + r));
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (r < it.rows)
+                            x = __ldg(reinterpret_cast<const uint4*>(
+                                static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
+                                (it.h * G + (r0 + r - tok * G)) * D + ch * 8));
+                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
+                        *reinterpret_cast<uint4*>(q_tile + (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch)) = x;
+                    }
+                }
+                tc::fence_proxy_async_smem();
+                arrive_warp(&bars[kQFull]);
         };
         // 16 bytes of values that some row must not see (NaN or infinity would reach it through a product)
         const auto not_finite = [](const uint4& x) {
@@ -357,7 +362,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 id = lane < boxes && pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride + c.page.div(pos)) : -1;
             };
             const auto issue = [&](const CUtensorMap* map, int k0, int page, uint64_t* bar) {
-                wait_free();
+                // (the second warp must not wait here: nothing holds it within a phase of the first)
+                if (warp == 8) wait_free();
                 if (good && warp == 8) {
                     const int pos = k0 + lane * box;
                     const bool mine = lane < boxes && pos < it.hi;
@@ -426,7 +432,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 }
                 if (bad) flags[(check - 1) & 7] = check;
             }
-            tc::mbar_arrive(&bars[kTileFull + slot]);
+            arrive_warp(&bars[kTileFull + slot]);
             ++done;
         };
         // thread k finds keys k and k + 64 of a tile: page ids are read a tile ahead, byte offsets shared through row_off
@@ -612,7 +618,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                         tc::tmem_ld_32x32b_x32(s_col(t) + lanes + i, *reinterpret_cast<uint32_t(*)[32]>(x + i));
                     tc::tmem_ld_wait();
                     tc::tc_fence_before();
-                    tc::mbar_arrive(&bars[kSFree + t]);   // the next scores may be written
+                    arrive_warp(&bars[kSFree + t]);       // the next scores may be written
                     if (L::kSplit && g == g0 * SUB) sc *= __int_as_float((127 - row_exp[(piece & 1) * kRows + row]) << 23);
                     if (edge) mask<SK>(x, first - k0, p - k0);
                     float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -652,7 +658,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                         l += weights<C, L::kSplit, true, SK>(x, sc, -base, p_at, p_low);
                     tmem_st_wait();
                     tc::tc_fence_before();
-                    tc::mbar_arrive(&bars[kPFull + t]);
+                    arrive_warp(&bars[kPFull + t]);
                 }
                 if (good) good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
                 tc::tc_fence_after();
