@@ -3,6 +3,16 @@
 // score(r, v) = s_r + x_rv - lse_r with lse_r = log sum_v exp(x_rv), ranked by (score in fp64, lower flattened index
 // r * vocab + v first); a NaN logit counts as -inf, and candidates of score -inf or NaN are never picked. A finished
 // row's only candidate is done_token at the row's own score.
+//
+// Bound: the logits' bytes, read once. A CTA takes up to 16384 logits of one row into registers (16-byte loads, 32 per
+// thread, a thread's values 8 or 4 at a time), leaves their maximum and sum of exponentials, and its own best `picks`:
+// within a row the score orders as the logit does, so no sum is needed to choose them. The threads' own best values
+// give a threshold, their picks-th largest: at least `picks` values reach it, and only the `picks` threads whose best
+// does can hold any that do, so at most picks x 32 values go on; a list of those is ranked exactly. Keys (value, then
+// lower index first) are 64-bit words without ties. The last CTA of a request puts the rows' sums together in the order
+// of their parts and ranks the parts' picks in the same way, with scores in fp64: the result does not depend on timing.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace gpt {
@@ -10,86 +20,287 @@ namespace {
 
 using namespace paged;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kPer = 32, kPart = kThreads * kPer, kWarps = kThreads / 32, kMostPicks = 64;
+constexpr int kList = kMostPicks * kPer;
 
-struct Best {
-    double score;
-    int at;
+// fp32 bits in an order that compares as unsigned: the larger float is the larger word; NaN is not passed in.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) {
+    return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+struct Found {               // a part's result: its maximum, sum of exp(x - maximum), and keys in descending order
+    float top, sum;
 };
-__device__ __forceinline__ bool better(double s, int i, double t, int j) { return s > t || (s == t && i < j); }
+
+// The k-th largest (k from 1) of the block's keys, one per thread, none of them twice except 0 ("nothing"): each warp
+// sorts its own, then the warps' heads are taken off k times by the first warp. Returns 0 when fewer than k exist.
+__device__ __forceinline__ unsigned long long kth_largest(unsigned long long key, int k, unsigned long long* sorted,
+                                                          unsigned long long* out) {
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    // bitonic sort of the warp's 32 keys, descending
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int step = size >> 1; step; step >>= 1) {
+            const unsigned long long other = __shfl_xor_sync(kFull, key, step);
+            const bool down = (lane & size) == 0, lower = (lane & step) == 0;
+            key = (down == lower) == (key > other) ? key : other;
+        }
+    sorted[warp * 32 + lane] = key;
+    __syncthreads();
+    if (warp == 0) {
+        int at = 0;
+        unsigned long long best = 0;
+        for (int i = 0; i < k; ++i) {
+            const unsigned long long head = lane < kWarps && at < 32 ? sorted[lane * 32 + at] : 0;
+            best = head;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                const unsigned long long y = __shfl_xor_sync(kFull, best, o);
+                if (y > best) best = y;
+            }
+            if (best == 0) break;
+            if (head == best) ++at;
+        }
+        if (lane == 0) *out = best;
+    }
+    __syncthreads();
+    return *out;
+}
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 2)
+beam_select_kernel(BeamArgs a, int parts, int* counters, Found* found, unsigned long long* keys) {
+    __shared__ unsigned long long list[kList];
+    __shared__ unsigned long long threshold;
+    __shared__ float red[2 * kWarps];
     __shared__ double lse[64];
-    __shared__ Best part[kThreads / 32];
-    __shared__ Best last;
-    const int req = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const T* base = static_cast<const T*>(a.logits) + (long long)req * a.beams * a.row_stride;
-    for (int r = warp; r < a.beams; r += kThreads / 32) {
-        float m = -INFINITY, z = 0.f;
-        for (int v = lane; v < a.vocab; v += 32) {
-            float x = to_f32(base[r * a.row_stride + v]);
-            if (!(x == x)) x = -INFINITY;
-            if (x > m) {
-                z = z * expf(m - x) + 1.f;
-                m = x;
-            } else if (x > -INFINITY) {
-                z += expf(x - m);
+    __shared__ int count, last;
+    unsigned long long* sorted = list;                // the threshold is found before the list is filled
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const int row = blockIdx.x / parts, part = blockIdx.x % parts, req = row / a.beams;
+    const bool done = a.done && a.done[row];
+    const int v0 = part * kPart, n = min(kPart, a.vocab - v0);
+    if (threadIdx.x == 0) count = 0;
+    if (!done) {
+        // --- the part's values; x[] holds -inf where there is none
+        constexpr int W = 16 / int(sizeof(T));        // values of a 16-byte load
+        const T* src = static_cast<const T*>(a.logits) + (long long)row * a.row_stride + v0;
+        float x[kPer];
+        if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
+            uint4 raw[kPer / W];
+#pragma unroll
+            for (int i = 0; i < kPer / W; ++i) {
+                const int at = (i * kThreads + threadIdx.x) * W;
+                if (at + W <= n) raw[i] = __ldcs(reinterpret_cast<const uint4*>(src + at));
+            }
+#pragma unroll
+            for (int i = 0; i < kPer / W; ++i) {
+                const int at = (i * kThreads + threadIdx.x) * W;
+                const T* r = reinterpret_cast<const T*>(&raw[i]);
+#pragma unroll
+                for (int e = 0; e < W; ++e)
+                    x[i * W + e] = at + W <= n ? to_f32(r[e]) : at + e < n ? to_f32(src[at + e]) : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int at = (i / W * kThreads + threadIdx.x) * W + i % W;
+                x[i] = at < n ? to_f32(src[at]) : -INFINITY;
             }
         }
-        float mm = m;
-        for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(kFull, mm, o));
-        const double zz = warp_sum(m > -INFINITY ? double(z) * exp(double(m) - mm) : 0.0);
-        if (lane == 0) lse[r] = double(mm) + log(zz);
-    }
-    if (threadIdx.x == 0) last = {INFINITY, -1};
-    __syncthreads();
-    const int total = a.beams * a.vocab;
-    for (int pick = 0; pick < a.picks; ++pick) {
-        Best b{-INFINITY, 0x7fffffff};
-        const Best prev = last;
-        for (int i = threadIdx.x; i < total; i += kThreads) {
-            const int r = i / a.vocab, v = i - r * a.vocab;
-            double sc = a.scores[req * a.beams + r];
-            if (a.done && a.done[req * a.beams + r]) {
-                if (v != a.done_token) continue;
-            } else {
-                const float x = to_f32(base[r * a.row_stride + v]);
-                sc = sc + (double(x) - lse[r]);
+        // --- maximum and sum; the thread's largest value, the lowest index first
+        float top = -INFINITY;
+        int best = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (!(x[i] == x[i])) x[i] = -INFINITY;
+            if (x[i] > top) {
+                top = x[i];
+                best = i;
             }
-            if (!(sc > -INFINITY)) continue;
-            if (better(prev.score, prev.at, sc, i) && better(sc, i, b.score, b.at)) b = {sc, i};
         }
-        for (int o = 16; o; o >>= 1) {
-            const double s = __shfl_xor_sync(kFull, b.score, o);
-            const int j = __shfl_xor_sync(kFull, b.at, o);
-            if (better(s, j, b.score, b.at)) b = {s, j};
-        }
-        if (lane == 0) part[warp] = b;
+        const auto index = [&](int i) { return (i / W * kThreads + int(threadIdx.x)) * W + i % W; };
+        const auto key_of = [&](float value, int i) {
+            return value == -INFINITY ? 0ull
+                                      : (unsigned long long)ordered(value) << 32 | (0xffffffffu - uint32_t(v0 + index(i)));
+        };
+        float all = top;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFull, all, o));
+        if (lane == 0) red[warp] = all;
         __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) all = fmaxf(all, red[w]);
+        const float base = all == -INFINITY || all == INFINITY ? 0.f : all;
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum4[i & 3] += __expf(x[i] - base);
+        float sum = warp_sum((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        if (lane == 0) red[kWarps + warp] = sum;
+        // --- the picks
+        const unsigned long long least = kth_largest(key_of(top, best), a.picks, sorted, &threshold);
         if (threadIdx.x == 0) {
-            for (int w = 1; w < kThreads / 32; ++w)
-                if (better(part[w].score, part[w].at, b.score, b.at)) b = part[w];
-            const bool none = b.at == 0x7fffffff;
-            const int o = req * a.picks + pick;
-            a.out_scores[o] = none ? -INFINITY : float(b.score);
-            a.rows[o] = none ? -1 : req * a.beams + b.at / a.vocab;
-            a.tokens[o] = none ? -1 : b.at % a.vocab;
-            last = b;
+            float s = 0.f;
+            for (int w = 0; w < kWarps; ++w) s += red[kWarps + w];
+            found[blockIdx.x] = {all, s};
+        }
+        if (key_of(top, best) >= max(least, 1ull)) {
+            const float floor_value = unordered(uint32_t(least >> 32));
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+                if (least == 0 || x[i] >= floor_value) {
+                    const unsigned long long k = key_of(x[i], i);
+                    if (k && k >= least) list[atomicAdd(&count, 1)] = k;
+                }
+        }
+        __syncthreads();
+        const int m = count;
+        // rank of each listed key: how many are larger (keys differ from one another)
+        for (int i = warp; i < m; i += kWarps) {
+            const unsigned long long k = list[i];
+            int larger = 0;
+            for (int j = lane; j < m; j += 32) larger += list[j] > k;
+            larger = __reduce_add_sync(kFull, larger);
+            if (lane == 0 && larger < a.picks) keys[(long long)blockIdx.x * a.picks + larger] = k;
+        }
+        for (int i = m + threadIdx.x; i < a.picks; i += kThreads) keys[(long long)blockIdx.x * a.picks + i] = 0;
+    } else {
+        if (threadIdx.x == 0) found[blockIdx.x] = {0.f, 1.f};
+        for (int i = threadIdx.x; i < a.picks; i += kThreads)
+            keys[(long long)blockIdx.x * a.picks + i] =
+                part == 0 && i == 0 ? (unsigned long long)ordered(0.f) << 32 | (0xffffffffu - uint32_t(a.done_token)) : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const int c = arrive(&counters[req]);
+        last = c == a.beams * parts - 1;
+        if (last) counters[req] = 0;
+    }
+    __syncthreads();
+    if (!last) return;
+
+    // --- the request: log-sum-exp of its rows, then the best of all parts' picks
+    const int first = req * a.beams * parts;
+    for (int r = warp; r < a.beams; r += kWarps) {
+        const Found* f = found + first + r * parts;
+        float top = -INFINITY;
+        for (int p = lane; p < parts; p += 32) top = fmaxf(top, __ldcg(&f[p].top));
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+        double sum = 0.0;
+        for (int p = lane; p < parts; p += 32) {
+            const float t = __ldcg(&f[p].top);
+            if (t > -INFINITY) sum += double(__ldcg(&f[p].sum)) * (t == INFINITY ? 1.0 : exp(double(t) - double(top)));
+        }
+        sum = warp_sum(sum);
+        // a finished row's candidate has the key of 0: its score is the row's own
+        if (lane == 0) lse[r] = a.done && a.done[req * a.beams + r] ? 0.0 : double(top) + log(sum);
+    }
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    const int total = a.beams * parts * a.picks;
+    const unsigned long long* mine = keys + (long long)first * a.picks;
+    // score of a candidate, and its order word: fp64 in an order that compares as unsigned, 0: none
+    const auto score_of = [&](int i, unsigned long long k, int& flat) {
+        const int r = i / (parts * a.picks);
+        flat = r * a.vocab + int(0xffffffffu - uint32_t(k));
+        return double(a.scores[req * a.beams + r]) + (double(unordered(uint32_t(k >> 32))) - lse[r]);
+    };
+    const auto order_of = [&](int i, unsigned long long k) {
+        int flat;
+        if (k == 0) return 0ull;
+        const double s = score_of(i, k, flat);
+        if (!(s > -INFINITY)) return 0ull;
+        const unsigned long long b = __double_as_longlong(s + 0.0);
+        return b & 0x8000000000000000ull ? ~b : b | 0x8000000000000000ull;
+    };
+    // thread's largest, then the threshold: scores alone (ties share a word, so the list takes all that reach it). Each
+    // part's picks come in descending order, so only the first few of a part can matter: the list holds at most
+    // kList, and with more candidates than that at the threshold (ties by the hundred) they are ranked where they lie.
+    unsigned long long best = 0;
+    for (int i = threadIdx.x; i < total; i += kThreads) best = max(best, order_of(i, __ldcg(mine + i)));
+    const unsigned long long least = kth_largest(best, a.picks, sorted, &threshold);
+    int taken = 0;
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        const unsigned long long k = __ldcg(mine + i), o = order_of(i, k);
+        taken += o && o >= least;
+    }
+    if (taken) atomicAdd(&count, taken);
+    __syncthreads();
+    const int m = count;
+    __syncthreads();
+    int* at_list = reinterpret_cast<int*>(list);      // candidates' places
+    const bool listed = m <= kList;
+    if (listed) {
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < total; i += kThreads) {
+            const unsigned long long o = order_of(i, __ldcg(mine + i));
+            if (o && o >= least) at_list[atomicAdd(&count, 1)] = i;
         }
         __syncthreads();
     }
+    const int many = listed ? m : total, out = req * a.picks;
+    for (int i = warp; i < many; i += kWarps) {
+        const int ci = listed ? at_list[i] : i;
+        const unsigned long long ki = __ldcg(mine + ci), oi = order_of(ci, ki);
+        if (!oi || oi < least) continue;
+        int fi;
+        const double si = score_of(ci, ki, fi);
+        int larger = 0;
+        for (int j = lane; j < many; j += 32) {
+            const int cj = listed ? at_list[j] : j;
+            const unsigned long long kj = __ldcg(mine + cj), oj = order_of(cj, kj);
+            if (!oj || oj < oi) continue;
+            int fj;
+            score_of(cj, kj, fj);
+            larger += oj > oi || fj < fi;
+        }
+        larger = __reduce_add_sync(kFull, larger);
+        if (lane == 0 && larger < a.picks) {
+            a.out_scores[out + larger] = float(si);
+            a.rows[out + larger] = req * a.beams + fi / a.vocab;
+            a.tokens[out + larger] = fi % a.vocab;
+        }
+    }
+    for (int i = min(m, a.picks) + threadIdx.x; i < a.picks; i += kThreads) {
+        a.out_scores[out + i] = -INFINITY;
+        a.rows[out + i] = a.tokens[out + i] = -1;
+    }
+}
+
+int parts_of(const BeamArgs& a) { return (a.vocab + kPart - 1) / kPart; }
+size_t counter_bytes(const BeamArgs& a) { return (size_t(a.batch) * sizeof(int) + 255) / 256 * 256; }
+size_t found_bytes(const BeamArgs& a) {
+    return (size_t(a.batch) * a.beams * parts_of(a) * sizeof(Found) + 255) / 256 * 256;
+}
+
+template <class T>
+void launch(const BeamArgs& a, void* ws, cudaStream_t s) {
+    char* p = static_cast<char*>(ws);
+    const int parts = parts_of(a);
+    beam_select_kernel<T><<<a.batch * a.beams * parts, kThreads, 0, s>>>(
+        a, parts, reinterpret_cast<int*>(p), reinterpret_cast<Found*>(p + kBeamCounters),
+        reinterpret_cast<unsigned long long*>(p + kBeamCounters + found_bytes(a)));
+    check_launch("beam_select");
 }
 
 }  // namespace
 
-size_t beam_ws_bytes(const BeamArgs&) { return 16; }
+size_t beam_ws_bytes(const BeamArgs& a) {
+    require(counter_bytes(a) <= kBeamCounters, "beam_select: too many requests in one call");
+    return kBeamCounters + found_bytes(a) + size_t(a.batch) * a.beams * parts_of(a) * a.picks * 8;
+}
 
-void launch_beam_select(const BeamArgs& a, void*, cudaStream_t s) {
-    if (a.type == kF32) beam_select_kernel<float><<<a.batch, kThreads, 0, s>>>(a);
-    else if (a.type == kF16) beam_select_kernel<__half><<<a.batch, kThreads, 0, s>>>(a);
-    else beam_select_kernel<__nv_bfloat16><<<a.batch, kThreads, 0, s>>>(a);
-    check_launch("beam_select");
+void launch_beam_select(const BeamArgs& a, void* ws, cudaStream_t s) {
+    if (a.type == kF32) launch<float>(a, ws, s);
+    else if (a.type == kF16) launch<__half>(a, ws, s);
+    else launch<__nv_bfloat16>(a, ws, s);
 }
 
 }  // namespace gpt

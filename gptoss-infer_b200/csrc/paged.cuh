@@ -50,6 +50,14 @@ __device__ __forceinline__ int safe_page(int id, const KvView& c) {
     return 0;
 }
 
+// One more arrival at a counter, after everything this CTA wrote (the caller has passed a barrier since); what the
+// earlier arrivals wrote is visible to the CTA after its next barrier.
+__device__ __forceinline__ int arrive(int* counter) {
+    int old;
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
+    return old;
+}
+
 template <class T>
 __device__ __forceinline__ float to_f32(T x);
 template <>

@@ -94,6 +94,8 @@ struct BeamArgs {
     int *rows, *tokens;
     int type, done_token, batch, beams, vocab, picks;
 };
+// Workspace: a counter per request in the first kBeamCounters bytes (zeroed once, left at 0), then the parts' results.
+constexpr size_t kBeamCounters = 1 << 18;
 size_t beam_ws_bytes(const BeamArgs& a);
 void launch_beam_select(const BeamArgs& a, void* ws, cudaStream_t s);
 

@@ -233,7 +233,7 @@ int gptoss_beam_select(const void* logits, int type, long long row_stride, const
         require(batch >= 0 && beams >= 1 && beams <= 64 && picks >= 1 && picks <= 64,
                 "beam_select: batch >= 0, beams and picks in 1 .. 64");
         require(vocab >= 1 && (long long)beams * vocab < (1ll << 31), "beam_select: beams * vocab must be 1 .. 2^31 - 1");
-        require((long long)batch * beams < (1 << 24), "beam_select: too many rows");
+        require(batch <= (1 << 16), "beam_select: at most 65536 requests in one call");
         require(row_stride >= vocab || (long long)batch * beams <= 1, "beam_select: row_stride is shorter than a row");
         require(!done || (done_token >= 0 && done_token < vocab), "beam_select: done_token outside the vocabulary");
         if (batch == 0) return;

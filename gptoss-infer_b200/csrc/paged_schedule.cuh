@@ -229,14 +229,6 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
     return sp;
 }
 
-// One more arrival at a counter, after everything this CTA wrote (the caller has passed a barrier since); what the
-// earlier arrivals wrote is visible to the CTA after its next barrier.
-__device__ __forceinline__ int arrive(int* counter) {
-    int old;
-    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
-    return old;
-}
-
 // One query row over keys [k0, k1) of a sequence, by one warp, in plain fp32 arithmetic and with masked keys never
 // multiplied: the path taken when a value that some row of a tile must not see is NaN or infinite (a matrix product
 // would carry it into every row as 0 * NaN). m (base-2 logarithm), l and o (dims lane * E ..) are left unnormalised.
