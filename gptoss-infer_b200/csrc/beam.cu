@@ -6,11 +6,14 @@
 //
 // Bound: the logits' bytes, read once. A CTA takes up to 16384 logits of one row into registers (16-byte loads, 32 per
 // thread, a thread's values 8 or 4 at a time), leaves their maximum and sum of exponentials, and its own best `picks`:
-// within a row the score orders as the logit does, so no sum is needed to choose them. The threads' own best values
-// give a threshold, their picks-th largest: at least `picks` values reach it, and only the `picks` threads whose best
-// does can hold any that do, so at most picks x 32 values go on; a list of those is ranked exactly. Keys (value, then
-// lower index first) are 64-bit words without ties. The last CTA of a request puts the rows' sums together in the order
-// of their parts and ranks the parts' picks in the same way, with scores in fp64: the result does not depend on timing.
+// within a row the score orders as the logit does, so no sum is needed to choose them. A threshold comes from the
+// threads' own best values: the least over the 16 warps of the warp's j-th largest, 16 j >= picks, so at least `picks`
+// values reach it (about three times as many do when the values are in no particular order: 54 for 16 picks). Those go
+// on a list and are ranked exactly. Where they overflow it (sorted or constant rows), the exact picks-th largest of the
+// threads' best is taken instead: only the `picks` threads whose best reaches it can hold values that do, at most
+// picks x 32. Keys (value, then lower index first) are 64-bit words without ties. The last CTA of a request puts the
+// rows' sums together in the order of their parts and ranks the parts' picks in the same way, with scores in fp64: the
+// result does not depend on timing.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -37,7 +40,8 @@ struct Found {               // a part's result: its maximum, sum of exp(x - max
 };
 
 // The k-th largest (k from 1) of the block's keys, one per thread, none of them twice except 0 ("nothing"): each warp
-// sorts its own, then the warps' heads are taken off k times by the first warp. Returns 0 when fewer than k exist.
+// sorts its own, then every key finds its rank. Returns 0 when fewer than k exist. (Where keys may be equal, it returns 0
+// or a key that at least k reach: equal keys share a rank, and the one asked for may then be nobody's.)
 __device__ __forceinline__ unsigned long long kth_largest(unsigned long long key, int k, unsigned long long* sorted,
                                                           unsigned long long* out) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -51,43 +55,72 @@ __device__ __forceinline__ unsigned long long kth_largest(unsigned long long key
             key = (down == lower) == (key > other) ? key : other;
         }
     sorted[warp * 32 + lane] = key;
+    if (threadIdx.x == 0) *out = 0;
     __syncthreads();
-    if (warp == 0) {
-        int at = 0;
-        unsigned long long best = 0;
-        for (int i = 0; i < k; ++i) {
-            const unsigned long long head = lane < kWarps && at < 32 ? sorted[lane * 32 + at] : 0;
-            best = head;
+    // how many keys are larger: in its own warp's order, and by binary search in the other warps'
+    if (key) {
+        int larger = lane;
+#pragma unroll 4
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) continue;
+            int at = 0;
 #pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const unsigned long long y = __shfl_xor_sync(kFull, best, o);
-                if (y > best) best = y;
-            }
-            if (best == 0) break;
-            if (head == best) ++at;
+            for (int step = 16; step; step >>= 1)
+                if (sorted[w * 32 + at + step - 1] > key) at += step;
+            larger += at + (sorted[w * 32 + at] > key);
         }
-        if (lane == 0) *out = best;
+        if (larger == k - 1) *out = key;
     }
     __syncthreads();
-    return *out;
+    const unsigned long long found = *out;
+    __syncthreads();                                  // `sorted` and `out` may be written again
+    return found;
+}
+
+// Lists of keys by rank: eight lanes count the larger ones for each. f(rank, place in the list).
+template <class G, class F>
+__device__ __forceinline__ void by_rank(int m, G&& larger_than, F&& f) {
+    const int lane8 = threadIdx.x % 8;
+    for (int i0 = 0; i0 < m; i0 += kThreads / 8) {    // uniform over the warp: all lanes take part in the sum
+        const int i = i0 + threadIdx.x / 8;
+        int larger = 0;
+        if (i < m)
+            for (int j = lane8; j < m; j += 8) larger += larger_than(j, i);
+#pragma unroll
+        for (int o = 4; o; o >>= 1) larger += __shfl_xor_sync(kFull, larger, o);
+        if (i < m && lane8 == 0) f(larger, i);
+    }
+}
+
+// A warp's j-th largest word (0: fewer than j are not 0), equal ones counted apart.
+__device__ __forceinline__ uint32_t warp_jth(uint32_t u, int j) {
+    uint32_t w = 0;
+    for (int i = 0; i < j; ++i) {
+        w = __reduce_max_sync(kFull, u);
+        if (w == 0) break;
+        if (int(threadIdx.x % 32) == __ffs(__ballot_sync(kFull, u == w)) - 1) u = 0;
+    }
+    return w;
 }
 
 template <class T>
 __global__ void __launch_bounds__(kThreads, 2)
-beam_select_kernel(BeamArgs a, int parts, int* counters, Found* found, unsigned long long* keys) {
+beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found, unsigned long long* keys) {
     __shared__ unsigned long long list[kList];
     __shared__ unsigned long long threshold;
+    __shared__ int flat_list[kList];                  // of the request's candidates: row of the request * vocab + token
     __shared__ float red[2 * kWarps];
+    __shared__ uint32_t low[kWarps];
     __shared__ double lse[64];
     __shared__ int count, last;
     unsigned long long* sorted = list;                // the threshold is found before the list is filled
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     const int row = blockIdx.x / parts, part = blockIdx.x % parts, req = row / a.beams;
     const bool done = a.done && a.done[row];
-    const int v0 = part * kPart, n = min(kPart, a.vocab - v0);
+    const int v0 = part * size, n = max(0, min(size, a.vocab - v0));
     if (threadIdx.x == 0) count = 0;
     if (!done) {
-        // --- the part's values; x[] holds -inf where there is none
+        // --- the part's values; x[] holds -inf where there is none, or NaN (fmaxf drops it)
         constexpr int W = 16 / int(sizeof(T));        // values of a 16-byte load
         const T* src = static_cast<const T*>(a.logits) + (long long)row * a.row_stride + v0;
         float x[kPer];
@@ -104,26 +137,19 @@ beam_select_kernel(BeamArgs a, int parts, int* counters, Found* found, unsigned 
                 const T* r = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
                 for (int e = 0; e < W; ++e)
-                    x[i * W + e] = at + W <= n ? to_f32(r[e]) : at + e < n ? to_f32(src[at + e]) : -INFINITY;
+                    x[i * W + e] = fmaxf(at + W <= n ? to_f32(r[e]) : at + e < n ? to_f32(src[at + e]) : -INFINITY, -INFINITY);
             }
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int at = (i / W * kThreads + threadIdx.x) * W + i % W;
-                x[i] = at < n ? to_f32(src[at]) : -INFINITY;
+                x[i] = fmaxf(at < n ? to_f32(src[at]) : -INFINITY, -INFINITY);
             }
         }
-        // --- maximum and sum; the thread's largest value, the lowest index first
+        // --- maximum, threshold, sum
         float top = -INFINITY;
-        int best = 0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (!(x[i] == x[i])) x[i] = -INFINITY;
-            if (x[i] > top) {
-                top = x[i];
-                best = i;
-            }
-        }
+        for (int i = 0; i < kPer; i += 2) top = fmaxf(fmaxf(top, x[i]), x[i + 1]);
         const auto index = [&](int i) { return (i / W * kThreads + int(threadIdx.x)) * W + i % W; };
         const auto key_of = [&](float value, int i) {
             return value == -INFINITY ? 0ull
@@ -132,42 +158,68 @@ beam_select_kernel(BeamArgs a, int parts, int* counters, Found* found, unsigned 
         float all = top;
 #pragma unroll
         for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(kFull, all, o));
-        if (lane == 0) red[warp] = all;
+        const int holders = min(kWarps, (n + 32 * W - 1) / (32 * W));       // warps that have values
+        const uint32_t word = top == -INFINITY ? 0u : ordered(top);
+        const uint32_t jth = warp < holders ? warp_jth(word, (a.picks + holders - 1) / holders) : 0xffffffffu;
+        if (lane == 0) {
+            red[warp] = all;
+            low[warp] = jth;
+        }
         __syncthreads();
+        uint32_t reach = low[0];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) all = fmaxf(all, red[w]);
+        for (int w = 0; w < kWarps; ++w) {
+            all = fmaxf(all, red[w]);
+            reach = min(reach, low[w]);
+        }
+        // --- values that reach the threshold (read again: a register cannot be picked by number)
+        const auto collect = [&](unsigned long long least) {
+            if (word && word >= uint32_t(least >> 32)) {
+                const float floor_value = least == 0 ? -INFINITY : unordered(uint32_t(least >> 32));
+                uint32_t hits = 0;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) hits |= uint32_t(x[i] >= floor_value) << i;
+                for (; hits; hits &= hits - 1) {
+                    const int i = __ffs(hits) - 1, at = index(i);
+                    if (at >= n) continue;
+                    const unsigned long long k = key_of(fmaxf(to_f32(src[at]), -INFINITY), i);
+                    if (k && k >= least) {
+                        const int to = atomicAdd(&count, 1);
+                        if (to < kList) list[to] = k;
+                    }
+                }
+            }
+        };
+        collect((unsigned long long)reach << 32);
         const float base = all == -INFINITY || all == INFINITY ? 0.f : all;
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < kPer; ++i) sum4[i & 3] += __expf(x[i] - base);
-        float sum = warp_sum((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        const float sum = warp_sum((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
         if (lane == 0) red[kWarps + warp] = sum;
-        // --- the picks
-        const unsigned long long least = kth_largest(key_of(top, best), a.picks, sorted, &threshold);
-        if (threadIdx.x == 0) {
-            float s = 0.f;
-            for (int w = 0; w < kWarps; ++w) s += red[kWarps + w];
-            found[blockIdx.x] = {all, s};
-        }
-        if (key_of(top, best) >= max(least, 1ull)) {
-            const float floor_value = unordered(uint32_t(least >> 32));
-#pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (least == 0 || x[i] >= floor_value) {
-                    const unsigned long long k = key_of(x[i], i);
-                    if (k && k >= least) list[atomicAdd(&count, 1)] = k;
-                }
-        }
         __syncthreads();
-        const int m = count;
-        // rank of each listed key: how many are larger (keys differ from one another)
-        for (int i = warp; i < m; i += kWarps) {
-            const unsigned long long k = list[i];
-            int larger = 0;
-            for (int j = lane; j < m; j += 32) larger += list[j] > k;
-            larger = __reduce_add_sync(kFull, larger);
-            if (lane == 0 && larger < a.picks) keys[(long long)blockIdx.x * a.picks + larger] = k;
+        if (threadIdx.x == 0) {
+            float z = 0.f;
+            for (int w = 0; w < kWarps; ++w) z += red[kWarps + w];
+            found[blockIdx.x] = {all, z};
         }
+        int m = count;
+        if (m > kList) {
+            int best = 0;                             // the first of the thread's largest values
+#pragma unroll
+            for (int i = kPer - 1; i >= 0; --i)
+                if (x[i] == top) best = i;
+            const unsigned long long least = kth_largest(key_of(top, best), a.picks, sorted, &threshold);
+            if (threadIdx.x == 0) count = 0;
+            __syncthreads();
+            collect(least);
+            __syncthreads();
+            m = count;
+        }
+        // rank of each listed key: how many are larger (keys differ from one another)
+        by_rank(m, [&](int j, int i) { return list[j] > list[i]; }, [&](int rank, int i) {
+            if (rank < a.picks) keys[(long long)blockIdx.x * a.picks + rank] = list[i];
+        });
         for (int i = m + threadIdx.x; i < a.picks; i += kThreads) keys[(long long)blockIdx.x * a.picks + i] = 0;
     } else {
         if (threadIdx.x == 0) found[blockIdx.x] = {0.f, 1.f};
@@ -219,53 +271,57 @@ beam_select_kernel(BeamArgs a, int parts, int* counters, Found* found, unsigned 
         const unsigned long long b = __double_as_longlong(s + 0.0);
         return b & 0x8000000000000000ull ? ~b : b | 0x8000000000000000ull;
     };
-    // thread's largest, then the threshold: scores alone (ties share a word, so the list takes all that reach it). Each
-    // part's picks come in descending order, so only the first few of a part can matter: the list holds at most
-    // kList, and with more candidates than that at the threshold (ties by the hundred) they are ranked where they lie.
+    // The threshold is the picks-th largest of the threads' best words, made different from one another by the thread's
+    // number in the 9 lowest bits (which only lowers it). If the list does not hold what reaches it (equal scores by the
+    // hundred), the candidates are ranked where they lie.
     unsigned long long best = 0;
     for (int i = threadIdx.x; i < total; i += kThreads) best = max(best, order_of(i, __ldcg(mine + i)));
-    const unsigned long long least = kth_largest(best, a.picks, sorted, &threshold);
-    int taken = 0;
-    for (int i = threadIdx.x; i < total; i += kThreads) {
-        const unsigned long long k = __ldcg(mine + i), o = order_of(i, k);
-        taken += o && o >= least;
-    }
-    if (taken) atomicAdd(&count, taken);
+    const unsigned long long least = kth_largest(best ? (best & ~511ull) | threadIdx.x : 0, a.picks, sorted, &threshold) & ~511ull;
+    const auto collect = [&](unsigned long long least) {
+        if (best && best >= least)
+            for (int i = threadIdx.x; i < total; i += kThreads) {
+                const unsigned long long k = __ldcg(mine + i), o = order_of(i, k);
+                if (o && o >= least) {
+                    const int to = atomicAdd(&count, 1);
+                    if (to < kList) {
+                        list[to] = o;
+                        score_of(i, k, flat_list[to]);
+                    }
+                }
+            }
+    };
+    collect(least);
     __syncthreads();
     const int m = count;
-    __syncthreads();
-    int* at_list = reinterpret_cast<int*>(list);      // candidates' places
-    const bool listed = m <= kList;
-    if (listed) {
-        if (threadIdx.x == 0) count = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < total; i += kThreads) {
-            const unsigned long long o = order_of(i, __ldcg(mine + i));
-            if (o && o >= least) at_list[atomicAdd(&count, 1)] = i;
-        }
-        __syncthreads();
-    }
-    const int many = listed ? m : total, out = req * a.picks;
-    for (int i = warp; i < many; i += kWarps) {
-        const int ci = listed ? at_list[i] : i;
-        const unsigned long long ki = __ldcg(mine + ci), oi = order_of(ci, ki);
-        if (!oi || oi < least) continue;
-        int fi;
-        const double si = score_of(ci, ki, fi);
-        int larger = 0;
-        for (int j = lane; j < many; j += 32) {
-            const int cj = listed ? at_list[j] : j;
-            const unsigned long long kj = __ldcg(mine + cj), oj = order_of(cj, kj);
-            if (!oj || oj < oi) continue;
-            int fj;
-            score_of(cj, kj, fj);
-            larger += oj > oi || fj < fi;
-        }
-        larger = __reduce_add_sync(kFull, larger);
-        if (lane == 0 && larger < a.picks) {
-            a.out_scores[out + larger] = float(si);
-            a.rows[out + larger] = req * a.beams + fi / a.vocab;
-            a.tokens[out + larger] = fi % a.vocab;
+    const int out = req * a.picks;
+    const auto put = [&](int at, double score, int flat) {
+        a.out_scores[out + at] = float(score);
+        a.rows[out + at] = req * a.beams + flat / a.vocab;
+        a.tokens[out + at] = flat % a.vocab;
+    };
+    if (m <= kList) {
+        by_rank(m, [&](int j, int i) { return list[j] > list[i] || (list[j] == list[i] && flat_list[j] < flat_list[i]); },
+                [&](int rank, int i) {
+                    const unsigned long long o = list[i];
+                    if (rank < a.picks)
+                        put(rank, __longlong_as_double(o & 0x8000000000000000ull ? o & 0x7fffffffffffffffull : ~o), flat_list[i]);
+                });
+    } else {
+        for (int i = warp; i < total; i += kWarps) {
+            const unsigned long long ki = __ldcg(mine + i), oi = order_of(i, ki);
+            if (!oi || oi < least) continue;
+            int fi;
+            const double si = score_of(i, ki, fi);
+            int larger = 0;
+            for (int j = lane; j < total; j += 32) {
+                const unsigned long long kj = __ldcg(mine + j), oj = order_of(j, kj);
+                if (!oj || oj < oi) continue;
+                int fj;
+                score_of(j, kj, fj);
+                larger += oj > oi || fj < fi;
+            }
+            larger = __reduce_add_sync(kFull, larger);
+            if (lane == 0 && larger < a.picks) put(larger, si, fi);
         }
     }
     for (int i = min(m, a.picks) + threadIdx.x; i < a.picks; i += kThreads) {
@@ -283,9 +339,10 @@ size_t found_bytes(const BeamArgs& a) {
 template <class T>
 void launch(const BeamArgs& a, void* ws, cudaStream_t s) {
     char* p = static_cast<char*>(ws);
-    const int parts = parts_of(a);
+    // equal parts, of whole 64-byte runs
+    const int parts = parts_of(a), size = ((a.vocab + parts - 1) / parts + 31) / 32 * 32;
     beam_select_kernel<T><<<a.batch * a.beams * parts, kThreads, 0, s>>>(
-        a, parts, reinterpret_cast<int*>(p), reinterpret_cast<Found*>(p + kBeamCounters),
+        a, parts, size, reinterpret_cast<int*>(p), reinterpret_cast<Found*>(p + kBeamCounters),
         reinterpret_cast<unsigned long long*>(p + kBeamCounters + found_bytes(a)));
     check_launch("beam_select");
 }
