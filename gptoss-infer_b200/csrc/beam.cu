@@ -15,6 +15,7 @@
 // rows' sums together in the order of their parts and ranks the parts' picks in the same way, with scores in fp64: the
 // result does not depend on timing.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -35,13 +36,19 @@ __device__ __forceinline__ float unordered(uint32_t o) {
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
+template <class T>
+__device__ __forceinline__ T from_f32(float x) {
+    if constexpr (std::is_same<T, float>::value) return x;
+    else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+    else return __float2bfloat16_rn(x);
+}
+
 struct Found {               // a part's result: its maximum, sum of exp(x - maximum), and keys in descending order
     float top, sum;
 };
 
 // The k-th largest (k from 1) of the block's keys, one per thread, none of them twice except 0 ("nothing"): each warp
-// sorts its own, then every key finds its rank. Returns 0 when fewer than k exist. (Where keys may be equal, it returns 0
-// or a key that at least k reach: equal keys share a rank, and the one asked for may then be nobody's.)
+// sorts its own, then every key finds its rank. Returns 0 when fewer than k exist.
 __device__ __forceinline__ unsigned long long kth_largest(unsigned long long key, int k, unsigned long long* sorted,
                                                           unsigned long long* out) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -104,7 +111,7 @@ __device__ __forceinline__ uint32_t warp_jth(uint32_t u, int j) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 2 : 3)
 beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found, unsigned long long* keys) {
     __shared__ unsigned long long list[kList];
     __shared__ unsigned long long threshold;
@@ -120,37 +127,35 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
     const int v0 = part * size, n = max(0, min(size, a.vocab - v0));
     if (threadIdx.x == 0) count = 0;
     if (!done) {
-        // --- the part's values; x[] holds -inf where there is none, or NaN (fmaxf drops it)
+        // --- the part's values, in registers as they are stored (16-bit ones in half the registers: three CTAs share an
+        // SM), -inf past the end
         constexpr int W = 16 / int(sizeof(T));        // values of a 16-byte load
         const T* src = static_cast<const T*>(a.logits) + (long long)row * a.row_stride + v0;
-        float x[kPer];
+        const auto index = [&](int i) { return (i / W * kThreads + int(threadIdx.x)) * W + i % W; };
+        union {
+            uint4 quad[kPer / W];
+            T value[kPer];
+        } raw;
         if (reinterpret_cast<uintptr_t>(src) % 16 == 0) {
-            uint4 raw[kPer / W];
 #pragma unroll
-            for (int i = 0; i < kPer / W; ++i) {
-                const int at = (i * kThreads + threadIdx.x) * W;
-                if (at + W <= n) raw[i] = __ldcs(reinterpret_cast<const uint4*>(src + at));
-            }
+            for (int i = 0; i < kPer / W; ++i)
+                if (index(i * W) + W <= n) raw.quad[i] = __ldcs(reinterpret_cast<const uint4*>(src + index(i * W)));
 #pragma unroll
-            for (int i = 0; i < kPer / W; ++i) {
-                const int at = (i * kThreads + threadIdx.x) * W;
-                const T* r = reinterpret_cast<const T*>(&raw[i]);
+            for (int i = 0; i < kPer / W; ++i)
+                if (index(i * W) + W > n) {
 #pragma unroll
-                for (int e = 0; e < W; ++e)
-                    x[i * W + e] = fmaxf(at + W <= n ? to_f32(r[e]) : at + e < n ? to_f32(src[at + e]) : -INFINITY, -INFINITY);
-            }
+                    for (int e = 0; e < W; ++e)
+                        raw.value[i * W + e] = index(i * W) + e < n ? src[index(i * W) + e] : from_f32<T>(-INFINITY);
+                }
         } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int at = (i / W * kThreads + threadIdx.x) * W + i % W;
-                x[i] = fmaxf(at < n ? to_f32(src[at]) : -INFINITY, -INFINITY);
-            }
+            for (int i = 0; i < kPer; ++i) raw.value[i] = index(i) < n ? src[index(i)] : from_f32<T>(-INFINITY);
         }
+        const auto x = [&](int i) { return fmaxf(to_f32(raw.value[i]), -INFINITY); };   // NaN counts as -inf
         // --- maximum, threshold, sum
         float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2) top = fmaxf(fmaxf(top, x[i]), x[i + 1]);
-        const auto index = [&](int i) { return (i / W * kThreads + int(threadIdx.x)) * W + i % W; };
+        for (int i = 0; i < kPer; i += 2) top = fmaxf(fmaxf(top, x(i)), x(i + 1));
         const auto key_of = [&](float value, int i) {
             return value == -INFINITY ? 0ull
                                       : (unsigned long long)ordered(value) << 32 | (0xffffffffu - uint32_t(v0 + index(i)));
@@ -178,7 +183,7 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
                 const float floor_value = least == 0 ? -INFINITY : unordered(uint32_t(least >> 32));
                 uint32_t hits = 0;
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) hits |= uint32_t(x[i] >= floor_value) << i;
+                for (int i = 0; i < kPer; ++i) hits |= uint32_t(x(i) >= floor_value) << i;
                 for (; hits; hits &= hits - 1) {
                     const int i = __ffs(hits) - 1, at = index(i);
                     if (at >= n) continue;
@@ -194,7 +199,7 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
         const float base = all == -INFINITY || all == INFINITY ? 0.f : all;
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum4[i & 3] += __expf(x[i] - base);
+        for (int i = 0; i < kPer; ++i) sum4[i & 3] += __expf(x(i) - base);
         const float sum = warp_sum((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
         if (lane == 0) red[kWarps + warp] = sum;
         __syncthreads();
@@ -208,7 +213,7 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
             int best = 0;                             // the first of the thread's largest values
 #pragma unroll
             for (int i = kPer - 1; i >= 0; --i)
-                if (x[i] == top) best = i;
+                if (x(i) == top) best = i;
             const unsigned long long least = kth_largest(key_of(top, best), a.picks, sorted, &threshold);
             if (threadIdx.x == 0) count = 0;
             __syncthreads();
