@@ -9,42 +9,46 @@
 //          ascending order, so sources and destinations never overlap.
 //
 // The counting is whole-number arithmetic: atomics in any order give the same result.
+//
+// Bound: the copied pages' bytes, read and written; for a few beams, latency. Each is one cooperative launch whose phases
+// are separated by grid-wide barriers (four launches in a row took 23.9 us for a
+// fork of four beams, most of it on the host): fork counts references into a zeroed array, one CTA then gives out the free
+// pages (8192 a step), and all CTAs copy; compact plans on one CTA, then all copy and rewrite the tables.
 #include <algorithm>
 
 #include "paged.cuh"
+#include "kernels.h"
+#include "tc.cuh"
 
 namespace gpt {
 namespace {
 
 using namespace paged;
 
-constexpr int kScan = 1024;
+constexpr int kThreads = 512, kPer = 16, kScan = kThreads * kPer;    // pages of a scan step
 
-// Workspace words: [0] copies, [1] live pages / holes; then per-page ranks or moves, then per-child words.
-struct PageWs {
-    int* head;
-    int* page;               // free list, or movers' destinations
-    int2* moves;             // (source, destination)
-    int* first;              // first child of each parent is found through the children's own words
-    int4* child;             // per child: base length, kept pages, wanted pages, last page or -1
-};
+constexpr int kNoChild = 0x7fffffff;
 
-__host__ __device__ inline PageWs carve(void* ws, int num_pages, int children) {
-    char* p = static_cast<char*>(ws);
-    PageWs w;
-    w.head = reinterpret_cast<int*>(p);
-    p += 256;
-    w.page = reinterpret_cast<int*>(p);
-    p += (size_t(num_pages) * 4 + 255) / 256 * 256;
-    w.moves = reinterpret_cast<int2*>(p);
-    p += (size_t(num_pages > children ? num_pages : children) * 8 + 255) / 256 * 256;
-    w.child = reinterpret_cast<int4*>(p);
-    p += (size_t(children) * 16 + 255) / 256 * 256;
-    w.first = reinterpret_cast<int*>(p);
-    return w;
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// All CTAs of a cooperative launch meet. Bounded; after a wait that gave up the error word is set and the kernel goes on
+// (the arrays it reads are within bounds whatever they hold).
+__device__ __forceinline__ void grid_barrier(unsigned long long* barrier, int* err) {
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned long long old, now;
+        asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], 1;" : "=l"(old) : "l"(barrier) : "memory");
+        const unsigned long long target = (old / gridDim.x + 1) * gridDim.x;
+        uint32_t i = 0;
+        do {
+            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(barrier) : "memory");
+        } while (now < target && ++i < tc::kSpinLimit);
+        if (now < target) report(err, kKvWait + 9);
+    }
+    __syncthreads();
 }
 
-// Exclusive prefix sum over a block of kScan threads; *total gets the sum. Two barriers.
+// Exclusive prefix sum over the block; *total gets the sum. Three barriers.
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     int x = v;
@@ -53,20 +57,16 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
         const int y = __shfl_up_sync(kFull, x, o);
         if (lane >= o) x += y;
     }
+    __syncthreads();
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int s = warp_sums[lane];
+    int before = 0, all = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(kFull, s, o);
-            if (lane >= o) s += y;
-        }
-        warp_sums[lane] = s;
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w < warp) before += warp_sums[w];
+        all += warp_sums[w];
     }
-    __syncthreads();
-    const int before = warp ? warp_sums[warp - 1] : 0;
-    *total = warp_sums[31];
+    *total = all;
     return before + x - v;
 }
 
@@ -82,208 +82,262 @@ __device__ __forceinline__ int table_len(const int* lens, int i, int stride, int
     return len;
 }
 
-__global__ void fork_counts_kernel(KvPages p, ForkArgs a, void* ws, int pass) {
-    const PageWs w = carve(ws, p.num_pages, a.children);
-    const long long stride = (long long)gridDim.x * blockDim.x, t0 = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (pass == 0) {
-        if (a.refs_out != a.refs)
-            for (long long i = t0; i < p.num_pages; i += stride) a.refs_out[i] = a.refs[i];
-        for (long long m = t0; m < a.children; m += stride) {
-            // the first child of each parent: the lowest m among those that name it
-            const int par = a.parents[m];
-            int4 c = make_int4(0, 0, 0, -1);
-            if (par >= a.seqs || par < -1) report(p.err, kKvBadParent);
-            if (par >= 0 && par < a.seqs) {
-                const int len = table_len(a.lens, par, a.stride, p.page_size, p.err), full = len / p.page_size;
-                bool first = true;
-                for (int i = 0; i < m; ++i) first = first && a.parents[i] != par;
-                c.x = len;
-                c.y = full;
-                if (len % p.page_size) {
-                    const int id = a.tables[(long long)par * a.stride + full];
-                    if (unsigned(id) >= unsigned(p.num_pages)) report(p.err, kKvBadPage);
-                    else if (first && a.refs[id] == 1) c.y = full + 1;
-                    else c.w = id;
-                }
-                long long want = (long long)len + (a.extra ? max(a.extra[m], 0) : 0);
-                const long long cap = (long long)a.stride * p.page_size;
-                if (want > cap) {
-                    report(p.err, kKvBadLength);
-                    want = cap;
-                }
-                c.z = int(want);
+// Copies the pages of `moves` in all layers, K and V: pieces of 16 KB, one per CTA and step. Where a page is one run of
+// memory (slot-major or head-major without gaps) a piece is eight 16-byte loads per thread in flight; otherwise rows.
+__device__ __forceinline__ void copy_pages(const KvPages& p, int n, const int2* moves) {
+    const int rows = p.page_size * p.kv_heads, chunks = p.row_bytes / 16;
+    const bool run = (p.head_stride == p.row_bytes && p.token_stride == (long long)p.row_bytes * p.kv_heads) ||
+                     (p.token_stride == p.row_bytes && p.head_stride == (long long)p.row_bytes * p.page_size);
+    const long long total = (long long)rows * chunks;               // 16-byte chunks of a page
+    constexpr int kPiece = kThreads * 4;
+    const long long pieces = (total + kPiece - 1) / kPiece;
+    const long long work = n * 2ll * p.layers * pieces;
+    for (long long it = blockIdx.x; it < work; it += gridDim.x) {
+        const long long mv = it / pieces;
+        const int piece = int(it - mv * pieces), plane = int(mv % (2 * p.layers)), m = int(mv / (2 * p.layers));
+        const int2 move = __ldcg(moves + m);
+        char* base = (plane & 1 ? p.v : p.k) + (plane >> 1) * p.layer_stride;
+        const char* src = base + move.x * p.page_stride;
+        char* dst = base + move.y * p.page_stride;
+        uint4 x[4];
+        long long off[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long u = (long long)piece * kPiece + i * kThreads + threadIdx.x;
+            if (run) {
+                off[i] = u * 16;
+            } else {
+                const int row = int(u / chunks), h = row % p.kv_heads, t = row / p.kv_heads;
+                off[i] = t * p.token_stride + h * p.head_stride + u % chunks * 16;
             }
-            w.child[m] = c;
+            if (u < total) x[i] = __ldcs(reinterpret_cast<const uint4*>(src + off[i]));
+            else off[i] = -1;
         }
-        return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (off[i] >= 0) __stcs(reinterpret_cast<uint4*>(dst + off[i]), x[i]);
     }
-    const long long n_in = (long long)a.seqs * a.stride, n_out = (long long)a.children * a.stride;
-    for (long long i = t0; i < n_in; i += stride) {
-        const int s = int(i / a.stride), j = int(i % a.stride);
+}
+
+__global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArgs a, PageWs w) {
+    __shared__ int sums[kThreads / 32];
+    const long long step = (long long)gridDim.x * kThreads, t0 = (long long)blockIdx.x * kThreads + threadIdx.x;
+    // --- references dropped and added (full pages), each sequence's first child
+    for (long long i = t0, n = (long long)a.seqs * a.stride; i < n; i += step) {
+        const int s = int(i / a.stride), j = int(i - (long long)s * a.stride);
         if (j >= pages_of(table_len(a.lens, s, a.stride, p.page_size, p.err), p.page_size)) continue;
         const int id = a.tables[i];
-        if (unsigned(id) < unsigned(p.num_pages)) atomicSub(&a.refs_out[id], 1);
+        if (unsigned(id) < unsigned(p.num_pages)) atomicSub(&w.delta[id], 1);
         else report(p.err, kKvBadPage);
     }
-    for (long long i = t0; i < n_out; i += stride) {
-        const int m = int(i / a.stride), j = int(i % a.stride);
+    for (long long i = t0, n = (long long)a.children * a.stride; i < n; i += step) {
+        const int m = int(i / a.stride), j = int(i - (long long)m * a.stride), par = a.parents[m];
         int id = -1;
-        if (j < w.child[m].y) {
-            id = a.tables[(long long)a.parents[m] * a.stride + j];
-            if (unsigned(id) < unsigned(p.num_pages)) atomicAdd(&a.refs_out[id], 1);
+        if (par >= 0 && par < a.seqs && j < table_len(a.lens, par, a.stride, p.page_size, p.err) / p.page_size) {
+            id = a.tables[(long long)par * a.stride + j];
+            if (unsigned(id) < unsigned(p.num_pages)) atomicAdd(&w.delta[id], 1);
         }
         a.tables_out[i] = id;
     }
-}
-
-__global__ void __launch_bounds__(kScan) fork_alloc_kernel(KvPages p, ForkArgs a, void* ws) {
-    __shared__ int sums[32];
-    const PageWs w = carve(ws, p.num_pages, a.children);
-    int free_pages = 0;
-    for (int i0 = 0; i0 < p.num_pages; i0 += kScan) {
-        const int i = i0 + threadIdx.x;
-        const bool f = i < p.num_pages && a.refs_out[i] == 0;
-        int total;
-        const int at = block_scan(f, sums, &total);
-        if (f) w.page[free_pages + at] = i;
-        free_pages += total;
-        __syncthreads();
+    for (long long m = t0; m < a.children; m += step) {
+        const int par = a.parents[m];
+        if (par >= 0 && par < a.seqs) atomicMin(&w.first[par], int(m));
+        else if (par != -1) report(p.err, kKvBadParent);
     }
-    int used = 0, copies = 0;
-    for (int m0 = 0; m0 < a.children; m0 += kScan) {
-        const int m = m0 + threadIdx.x;
-        int4 c = m < a.children ? w.child[m] : make_int4(0, 0, 0, -1);
-        const int want = pages_of(c.z, p.page_size), n = max(0, want - c.y);
-        int total;
-        const int at = used + block_scan(n, sums, &total);
-        __syncthreads();
-        const int got = max(0, min(n, free_pages - at));
-        const bool copy = c.w >= 0 && got > 0;
-        int total_copies;
-        const int slot = copies + block_scan(copy, sums, &total_copies);
-        if (m < a.children) {
-            if (got < n) report(p.err, kKvOutOfPages);
-            for (int i = 0; i < got; ++i) {
-                const int id = w.page[at + i];
-                a.tables_out[(long long)m * a.stride + c.y + i] = id;
-                a.refs_out[id] = 1;
+    grid_barrier(w.barrier, p.err);
+    if (blockIdx.x == 0) {
+        // --- the last pages that stay
+        for (int m = threadIdx.x; m < a.children; m += kThreads) {
+            const int par = a.parents[m];
+            if (par < 0 || par >= a.seqs || __ldcg(&w.first[par]) != m) continue;
+            const int len = table_len(a.lens, par, a.stride, p.page_size, p.err), full = len / p.page_size;
+            if (len % p.page_size == 0) continue;
+            const int id = a.tables[(long long)par * a.stride + full];
+            if (unsigned(id) < unsigned(p.num_pages) && a.refs[id] == 1) {
+                atomicAdd(&w.delta[id], 1);
+                a.tables_out[(long long)m * a.stride + full] = id;
             }
-            a.lens_out[m] = got < n ? min((long long)c.z, (long long)(c.y + got) * p.page_size) : c.z;
-            if (copy) w.moves[slot] = make_int2(c.w, w.page[at]);
         }
-        used += total;
-        copies += total_copies;
         __syncthreads();
+        // --- new counts, free pages in ascending order
+        int free_pages = 0;
+        for (int i0 = 0; i0 < p.num_pages; i0 += kScan) {
+            const int i = i0 + threadIdx.x * kPer;
+            unsigned is_free = 0;
+            int r[kPer];
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) r[e] = i + e < p.num_pages ? a.refs[i + e] : 1;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (i + e < p.num_pages) r[e] += __ldcg(&w.delta[i + e]);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e)
+                if (i + e < p.num_pages) {
+                    w.delta[i + e] = 0;
+                    a.refs_out[i + e] = r[e];
+                    is_free |= unsigned(r[e] == 0) << e;
+                }
+            int total;
+            int at = free_pages + block_scan(__popc(is_free), sums, &total);
+            for (unsigned f = is_free; f; f &= f - 1) w.free_page[at++] = i + __ffs(f) - 1;
+            free_pages += total;
+        }
+        __syncthreads();
+        // --- fresh pages, in the order of the children
+        int used = 0, copies = 0;
+        for (int m0 = 0; m0 < a.children; m0 += kThreads) {
+            const int m = m0 + threadIdx.x;
+            int have = 0, want_len = 0, src = -1;
+            if (m < a.children) {
+                const int par = a.parents[m];
+                if (par >= 0 && par < a.seqs) {
+                    const int len = table_len(a.lens, par, a.stride, p.page_size, p.err);
+                    have = len / p.page_size;
+                    if (len % p.page_size) {
+                        const int id = a.tables[(long long)par * a.stride + have];
+                        if (unsigned(id) >= unsigned(p.num_pages)) report(p.err, kKvBadPage);
+                        else if (__ldcg(&a.tables_out[(long long)m * a.stride + have]) >= 0) ++have;
+                        else src = id;
+                    }
+                    const long long want = (long long)len + (a.extra ? max(a.extra[m], 0) : 0);
+                    const long long cap = (long long)a.stride * p.page_size;
+                    if (want > cap) report(p.err, kKvBadLength);
+                    want_len = int(min(want, cap));
+                }
+            }
+            const int n = max(0, pages_of(want_len, p.page_size) - have);
+            int total, total_copies;
+            const int at = used + block_scan(n, sums, &total);
+            const int got = max(0, min(n, free_pages - at));
+            const bool copy = src >= 0 && got > 0;
+            const int slot = copies + block_scan(copy, sums, &total_copies);
+            if (m < a.children) {
+                if (got < n) report(p.err, kKvOutOfPages);
+                for (int i = 0; i < got; ++i) {
+                    const int id = w.free_page[at + i];
+                    a.tables_out[(long long)m * a.stride + have + i] = id;
+                    a.refs_out[id] = 1;
+                }
+                a.lens_out[m] = got < n ? int(min((long long)want_len, (long long)(have + got) * p.page_size)) : want_len;
+                if (copy) w.moves[slot] = make_int2(src, w.free_page[at]);
+            }
+            used += total;
+            copies += total_copies;
+        }
+        if (threadIdx.x == 0) *w.count = copies;
+        for (int i = threadIdx.x; i < a.seqs; i += kThreads) w.first[i] = kNoChild;
     }
-    if (threadIdx.x == 0) w.head[0] = copies;
+    grid_barrier(w.barrier, p.err);
+    copy_pages(p, __ldcg(w.count), w.moves);
 }
 
-// One CTA column per (layer, K or V); rows of row_bytes (128 or 256), 16 bytes per thread.
-__global__ void copy_pages_kernel(KvPages p, const int* count, const int2* moves) {
-    const int n = *count, chunks = p.row_bytes / 16;
-    const long long per_page = (long long)p.page_size * p.kv_heads * chunks;
-    const int plane = blockIdx.y, layer = plane >> 1;
-    char* base = (plane & 1 ? p.v : p.k) + layer * p.layer_stride;
-    for (int i = blockIdx.x; i < n; i += gridDim.x) {
-        const char* src = base + moves[i].x * p.page_stride;
-        char* dst = base + moves[i].y * p.page_stride;
-        for (long long u = threadIdx.x; u < per_page; u += blockDim.x) {
-            const int c = int(u % chunks), h = int(u / chunks % p.kv_heads), t = int(u / chunks / p.kv_heads);
-            const long long off = t * p.token_stride + h * p.head_stride + c * 16;
-            *reinterpret_cast<uint4*>(dst + off) = *reinterpret_cast<const uint4*>(src + off);
+__global__ void __launch_bounds__(kThreads, 2) kv_compact_kernel(KvPages p, CompactArgs a, PageWs w) {
+    __shared__ int sums[kThreads / 32];
+    if (blockIdx.x == 0) {
+        int live = 0;
+        for (int i = threadIdx.x; i < p.num_pages; i += kThreads) live += a.refs[i] > 0;
+        int total;
+        block_scan(live, sums, &total);
+        live = total;
+        // holes below the live count and live pages from it on, both in ascending order: as many of the one as of the other
+        int holes = 0, movers = 0;
+        for (int i0 = 0; i0 < p.num_pages; i0 += kScan) {
+            const int i = i0 + threadIdx.x * kPer;
+            unsigned hole = 0, mover = 0;
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const int r = i + e < p.num_pages ? a.refs[i + e] : 0;
+                if (i + e < p.num_pages) a.remap[i + e] = r > 0 ? i + e : -1;
+                if (i + e < live) hole |= unsigned(r <= 0) << e;
+                else mover |= unsigned(r > 0) << e;
+            }
+            int n_holes, n_movers;
+            int at = holes + block_scan(__popc(hole), sums, &n_holes);
+            for (; hole; hole &= hole - 1) w.moves[at++].y = i + __ffs(hole) - 1;
+            at = movers + block_scan(__popc(mover), sums, &n_movers);
+            for (; mover; mover &= mover - 1) w.moves[at++].x = i + __ffs(mover) - 1;
+            holes += n_holes;
+            movers += n_movers;
+        }
+        __syncthreads();
+        // counts: the movers' go to their holes; pages past the live count are free
+        if (a.refs_out != a.refs)
+            for (int i = threadIdx.x; i < min(live, p.num_pages); i += kThreads) a.refs_out[i] = max(a.refs[i], 0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < movers; i += kThreads) {
+            const int2 v = w.moves[i];
+            a.remap[v.x] = v.y;
+            a.refs_out[v.y] = a.refs[v.x];
+        }
+        __syncthreads();
+        for (int i = live + threadIdx.x; i < p.num_pages; i += kThreads) a.refs_out[i] = 0;
+        if (threadIdx.x == 0) {
+            *w.count = movers;
+            *a.live = live;
         }
     }
-}
-
-__global__ void __launch_bounds__(kScan) compact_plan_kernel(KvPages p, CompactArgs a, void* ws) {
-    __shared__ int sums[32];
-    const PageWs w = carve(ws, p.num_pages, 0);
-    int live = 0;
-    for (int i0 = 0; i0 < p.num_pages; i0 += kScan) {
-        const int i = i0 + threadIdx.x;
-        int total;
-        block_scan(i < p.num_pages && a.refs[i] > 0, sums, &total);
-        live += total;
-        __syncthreads();
-    }
-    int holes = 0;
-    for (int i0 = 0; i0 < live; i0 += kScan) {
-        const int i = i0 + threadIdx.x;
-        const bool f = i < live && a.refs[i] <= 0;
-        int total;
-        const int at = holes + block_scan(f, sums, &total);
-        if (f) w.moves[at].y = i;
-        holes += total;
-        __syncthreads();
-    }
-    int movers = 0;
-    for (int i0 = live; i0 < p.num_pages; i0 += kScan) {
-        const int i = i0 + threadIdx.x;
-        const int r = i < p.num_pages ? a.refs[i] : 0;
-        int total;
-        const int at = movers + block_scan(r > 0, sums, &total);
-        if (r > 0) w.moves[at].x = i;
-        movers += total;
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < p.num_pages; i += kScan) {
-        const int r = a.refs[i];
-        a.remap[i] = r > 0 ? i : -1;
-        a.refs_out[i] = r > 0 && i < live ? r : i < live ? 0 : (a.refs_out == a.refs ? r : 0);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < movers; i += kScan) {
-        const int2 v = w.moves[i];
-        a.remap[v.x] = v.y;
-        a.refs_out[v.y] = a.refs[v.x];
-    }
-    __syncthreads();
-    if (a.refs_out == a.refs)
-        for (int i = live + threadIdx.x; i < p.num_pages; i += kScan) a.refs_out[i] = 0;
-    if (threadIdx.x == 0) {
-        w.head[0] = movers;
-        *a.live = live;
-    }
-}
-
-__global__ void compact_tables_kernel(KvPages p, CompactArgs a) {
+    grid_barrier(w.barrier, p.err);
     const long long n = (long long)a.seqs * a.stride;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long long)gridDim.x * blockDim.x) {
-        const int s = int(i / a.stride), j = int(i % a.stride);
+    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
+        const int s = int(i / a.stride), j = int(i - (long long)s * a.stride);
         int id = -1;
         if (j < pages_of(table_len(a.lens, s, a.stride, p.page_size, p.err), p.page_size)) {
             const int old = a.tables[i];
-            if (unsigned(old) < unsigned(p.num_pages)) id = a.remap[old];
+            if (unsigned(old) < unsigned(p.num_pages)) id = __ldcg(a.remap + old);
             else report(p.err, kKvBadPage);
         }
         a.tables_out[i] = id;
     }
+    copy_pages(p, __ldcg(w.count), w.moves);
 }
 
-int grid_for(long long n) { return int(std::min<long long>(592, std::max<long long>(1, (n + 255) / 256))); }
+__global__ void init_first_kernel(int* first, int n) {
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) first[i] = kNoChild;
+}
+
+// CTAs for so many table entries and bytes of pages that may have to be copied.
+int grid_for(long long entries, long long bytes) {
+    const long long want = std::max((entries + 2 * kThreads - 1) / (2 * kThreads), (bytes + 32767) / 32768);
+    return int(std::min<long long>(2 * num_sms(), std::max<long long>(1, want)));
+}
+long long page_bytes(const KvPages& p) { return 2ll * p.layers * p.page_size * p.kv_heads * p.row_bytes; }
 
 }  // namespace
 
-size_t kv_pages_ws_bytes(int num_pages, int children) {
-    return 256 + (size_t(num_pages) * 4 + 256) + (size_t(std::max(num_pages, children)) * 8 + 256) +
-           (size_t(children) * 20 + 512);
+size_t kv_pages_ws_bytes(int num_pages, int children, int seqs) {
+    return 256 + 2 * up256(size_t(num_pages) * 4) + up256(size_t(std::max(num_pages, children)) * 8) + size_t(seqs) * 4;
 }
 
-void launch_kv_fork(const KvPages& p, const ForkArgs& a, void* ws, cudaStream_t s) {
-    const PageWs w = carve(ws, p.num_pages, a.children);
-    fork_counts_kernel<<<grid_for(std::max(p.num_pages, a.children)), 256, 0, s>>>(p, a, ws, 0);
-    fork_counts_kernel<<<grid_for((long long)std::max(a.seqs, a.children) * a.stride), 256, 0, s>>>(p, a, ws, 1);
-    fork_alloc_kernel<<<1, kScan, 0, s>>>(p, a, ws);
-    copy_pages_kernel<<<dim3(std::min(std::max(1, a.children), 256), 2 * p.layers), 256, 0, s>>>(p, w.head, w.moves);
-    check_launch("kv_fork");
+PageWs make_kv_pages_ws(void* ws, int num_pages, int children, int seqs) {
+    char* p = static_cast<char*>(ws);
+    PageWs w;
+    w.barrier = reinterpret_cast<unsigned long long*>(p);
+    w.count = reinterpret_cast<int*>(p + 128);
+    w.delta = reinterpret_cast<int*>(p += 256);
+    w.free_page = reinterpret_cast<int*>(p += up256(size_t(num_pages) * 4));
+    w.moves = reinterpret_cast<int2*>(p += up256(size_t(num_pages) * 4));
+    w.first = reinterpret_cast<int*>(p + up256(size_t(std::max(num_pages, children)) * 8));
+    if (seqs > 0) init_first_kernel<<<(seqs + 255) / 256, 256>>>(w.first, seqs);
+    check_launch("kv_pages workspace");
+    return w;
 }
 
-void launch_kv_compact(const KvPages& p, const CompactArgs& a, void* ws, cudaStream_t s) {
-    const PageWs w = carve(ws, p.num_pages, 0);
-    compact_plan_kernel<<<1, kScan, 0, s>>>(p, a, ws);
-    copy_pages_kernel<<<dim3(std::min(p.num_pages, 1024), 2 * p.layers), 256, 0, s>>>(p, w.head, w.moves);
-    compact_tables_kernel<<<grid_for((long long)a.seqs * a.stride), 256, 0, s>>>(p, a);
-    check_launch("kv_compact");
+void launch_kv_fork(const KvPages& p, const ForkArgs& a, const PageWs& w, cudaStream_t s) {
+    const int grid = grid_for((long long)std::max(a.seqs, a.children) * a.stride, a.children * page_bytes(p));
+    KvPages pp = p;
+    ForkArgs aa = a;
+    PageWs ww = w;
+    void* args[] = {&pp, &aa, &ww};
+    GPT_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kv_fork_kernel), dim3(grid), dim3(kThreads), args, 0, s));
+}
+
+void launch_kv_compact(const KvPages& p, const CompactArgs& a, const PageWs& w, cudaStream_t s) {
+    const int grid = grid_for((long long)a.seqs * a.stride, p.num_pages * page_bytes(p) / 4);
+    KvPages pp = p;
+    CompactArgs aa = a;
+    PageWs ww = w;
+    void* args[] = {&pp, &aa, &ww};
+    GPT_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kv_compact_kernel), dim3(grid), dim3(kThreads), args, 0, s));
 }
 
 }  // namespace gpt

@@ -116,8 +116,19 @@ struct KvPages {
     int layers, num_pages, page_size, kv_heads, row_bytes;
     int* err;
 };
-size_t kv_pages_ws_bytes(int num_pages, int children);
-void launch_kv_fork(const KvPages& p, const ForkArgs& a, void* ws, cudaStream_t s);
-void launch_kv_compact(const KvPages& p, const CompactArgs& a, void* ws, cudaStream_t s);
+// Workspace of both, for up to so many children and sequences of a call: zeroed memory, laid out and prepared once by
+// make_kv_pages_ws (on the legacy default stream). The kernels leave it as they found it.
+struct PageWs {
+    unsigned long long* barrier;   // arrivals, ever: a launch leaves a multiple of its grid size
+    int* count;                    // [0] moves
+    int* delta;                    // [num_pages] change of the counts; left at 0
+    int* free_page;                // [num_pages]
+    int2* moves;                   // (source, destination)
+    int* first;                    // [seqs] first child of each sequence; left at the largest int
+};
+size_t kv_pages_ws_bytes(int num_pages, int children, int seqs);
+PageWs make_kv_pages_ws(void* ws, int num_pages, int children, int seqs);
+void launch_kv_fork(const KvPages& p, const ForkArgs& a, const PageWs& w, cudaStream_t s);
+void launch_kv_compact(const KvPages& p, const CompactArgs& a, const PageWs& w, cudaStream_t s);
 
 }  // namespace gpt

@@ -24,8 +24,9 @@ struct gptoss_kv_pool {
     int type = 0, dim = 0, device = 0;
     int* err = nullptr;
     void* attn_ws = nullptr;
-    void* page_ws = nullptr;
-    size_t page_ws_bytes = 0;
+    void* page_mem = nullptr;                 // of page_ws, made for so many children and sequences
+    gpt::PageWs page_ws{};
+    int page_children = 0, page_seqs = 0;
 
     gpt::KvView view(int layer) const {
         gpt::KvView v{};
@@ -46,7 +47,7 @@ struct gptoss_kv_pool {
     ~gptoss_kv_pool() {
         cudaFree(err);
         cudaFree(attn_ws);
-        cudaFree(page_ws);
+        cudaFree(page_mem);
     }
 };
 
@@ -113,6 +114,25 @@ struct ThreadWs {
 };
 thread_local ThreadWs g_beam_ws;
 
+// The pool's page workspace, made anew when a call needs more than it was made for.
+const gpt::PageWs& page_ws(gptoss_kv_pool* p, int children, int seqs) {
+    if (!p->page_mem || p->page_children < children || p->page_seqs < seqs) {
+        children = std::max(children, p->page_children);
+        seqs = std::max(seqs, p->page_seqs);
+        if (p->page_mem) GPT_CHECK(cudaFree(p->page_mem));
+        p->page_mem = nullptr;
+        p->page_children = p->page_seqs = 0;
+        const size_t n = gpt::kv_pages_ws_bytes(p->pages.num_pages, children, seqs);
+        GPT_CHECK(cudaMalloc(&p->page_mem, n));
+        GPT_CHECK(cudaMemset(p->page_mem, 0, n));
+        p->page_ws = gpt::make_kv_pages_ws(p->page_mem, p->pages.num_pages, children, seqs);
+        GPT_CHECK(cudaDeviceSynchronize());
+        p->page_children = children;
+        p->page_seqs = seqs;
+    }
+    return p->page_ws;
+}
+
 }  // namespace
 
 extern "C" {
@@ -155,6 +175,7 @@ gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, in
         GPT_CHECK(cudaMalloc(&p->attn_ws, n));
         GPT_CHECK(cudaMemset(p->attn_ws, 0, n));
         GPT_CHECK(cudaDeviceSynchronize());
+        page_ws(p.get(), 256, 256);
         made = p.release();
     });
     return rc == 0 ? made : nullptr;
@@ -245,24 +266,6 @@ int gptoss_beam_select(const void* logits, int type, long long row_stride, const
     });
 }
 
-namespace {
-
-void* page_ws(gptoss_kv_pool* p, int children) {
-    const size_t n = gpt::kv_pages_ws_bytes(p->pages.num_pages, children);
-    if (p->page_ws_bytes < n) {
-        if (p->page_ws) GPT_CHECK(cudaFree(p->page_ws));
-        p->page_ws = nullptr;
-        p->page_ws_bytes = 0;
-        GPT_CHECK(cudaMalloc(&p->page_ws, n));
-        GPT_CHECK(cudaMemset(p->page_ws, 0, n));
-        GPT_CHECK(cudaDeviceSynchronize());
-        p->page_ws_bytes = n;
-    }
-    return p->page_ws;
-}
-
-}  // namespace
-
 int gptoss_kv_fork(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tables, const int32_t* lens, int seqs,
                    const int32_t* parents, const int32_t* extra, int children, int table_stride, int32_t* refs_out,
                    int32_t* tables_out, int32_t* lens_out, void* stream) {
@@ -277,7 +280,7 @@ int gptoss_kv_fork(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tables
                 "kv_fork: the children's tables and lengths need arrays of their own");
         check_device(p, "kv_fork");
         gpt::ForkArgs a{refs, tables, lens, parents, extra, refs_out, tables_out, lens_out, seqs, children, table_stride};
-        gpt::launch_kv_fork(p->pages, a, page_ws(p, children), static_cast<cudaStream_t>(stream));
+        gpt::launch_kv_fork(p->pages, a, page_ws(p, children, seqs), static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -291,7 +294,7 @@ int gptoss_kv_compact(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tab
         require(seqs == 0 || table_stride == 0 || (tables && lens && tables_out), "kv_compact: null tables or lengths");
         check_device(p, "kv_compact");
         gpt::CompactArgs a{refs, tables, lens, refs_out, tables_out, remap, live, seqs, table_stride};
-        gpt::launch_kv_compact(p->pages, a, page_ws(p, 0), static_cast<cudaStream_t>(stream));
+        gpt::launch_kv_compact(p->pages, a, page_ws(p, 0, 0), static_cast<cudaStream_t>(stream));
     });
 }
 
