@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "paged.h"
 
@@ -83,21 +85,25 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool half) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Eight consecutive values, 16-byte aligned (32-byte for fp32 pairs of loads).
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+// Eight consecutive values as loaded: one 16-byte word of 16-bit ones, two of fp32.
+template <class T, int Q>
+__device__ __forceinline__ void unpack8(const uint4 (&a)[Q], float (&x)[8]) {
     if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x[4 * i] = __uint_as_float(a[i].x);
+            x[4 * i + 1] = __uint_as_float(a[i].y);
+            x[4 * i + 2] = __uint_as_float(a[i].z);
+            x[4 * i + 3] = __uint_as_float(a[i].w);
+        }
     } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        const uint32_t w[4] = {a[0].x, a[0].y, a[0].z, a[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (std::is_same<T, __half>::value) {
                 const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                x[2 * i] = f.x; x[2 * i + 1] = f.y;
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
             } else {
                 x[2 * i] = __uint_as_float(w[i] << 16);
                 x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);

@@ -76,6 +76,7 @@ struct PagedAttnArgs {
     long long q_stride, out_stride;          // elements between tokens
     int type, kv_type, q_heads, window;
     float scale;
+    int rows_from, rows_to;                  // sequences with so many query rows per key/value head; others are left out
 };
 // Workspace of launch_paged_attention: counters and partial results; zeroed once, the kernels leave the counters at 0.
 // The two kernels share it (their counters are the same words).

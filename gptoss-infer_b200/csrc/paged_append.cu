@@ -4,8 +4,8 @@
 // (a cos - b sin, b cos + a sin) with the table's row p; pairs are (j, j + rot/2) or, interleaved, (2j, 2j + 1); the
 // dims from rot on pass through. All arithmetic is fp32; a value is rounded once, to the type it is stored in.
 //
-// Bound: bytes (each value read once and written once; nothing is reused but the token's cos/sin row, which stays in
-// registers). A work item is 16 values of one head: 8 pairs, so both halves of a pair are in one thread.
+// Bound: bytes (each value read once and written once; nothing is reused but the token's cos/sin row, which the heads find
+// in L1). A work item is two runs of eight values of one head with whole pairs in them.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -17,15 +17,31 @@ using namespace paged;
 
 constexpr int kThreads = 256;
 constexpr int kTokens = 8;       // tokens per CTA, at most: one warp looks up each
+// Items of a thread in flight: more of them cost more in resident threads than they bring (16383 bf16 tokens of 48 heads
+// of 128: 1 item 70 us, 2 75 us, 4 91 us).
+constexpr int kBatch = 1;
 
 struct Place {
     char *k, *v;                 // the token's cache rows (head 0), or null: not stored
     int pos;                     // row of the cos/sin table, or -1: token not in a sequence or out of range
 };
 
+__device__ __forceinline__ void turn(float& a, float& b, float cs, float sn) {
+    const float p = a, r = b;
+    a = p * cs - r * sn;
+    b = r * cs + p * sn;
+}
+__device__ __forceinline__ void turn_pairs(float (&x)[8], const float* cs, const float* sn) {
+    const float4 c4 = __ldg(reinterpret_cast<const float4*>(cs)), s4 = __ldg(reinterpret_cast<const float4*>(sn));
+    turn(x[0], x[1], c4.x, s4.x);
+    turn(x[2], x[3], c4.y, s4.y);
+    turn(x[4], x[5], c4.z, s4.z);
+    turn(x[6], x[7], c4.w, s4.w);
+}
+
 // VEC: every run of eight values is 16-byte aligned in memory and pairs do not straddle a run.
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b, AppendArgs a, int per_cta) {
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b, AppendArgs a, int per_cta, FastDiv per_token) {
     __shared__ Place place[kTokens];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int t0 = blockIdx.x * per_cta, nt = min(per_cta, b.tokens - t0);
@@ -58,68 +74,97 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b
     const int per_head = VEC ? c.dim / 16 : c.dim / 2, heads = a.q_heads + 2 * c.kv_heads;
     const int half = a.rot / 2, q_bytes = a.q_type == kF32 ? 4 : 2;
     const int items = heads * per_head;
-    // blockDim is a multiple of per_head: a thread keeps its dims over the heads, and its cos/sin values per token
-    const int j = threadIdx.x % per_head;
-    for (int u = 0; u < nt; ++u) {
-        const Place w = place[u];
-        if (w.pos < 0) continue;
-        const long long t = t0 + u;
-        const T* q = static_cast<const T*>(a.q) + t * a.q_stride;
-        const T* k = static_cast<const T*>(a.k) + t * a.kv_stride;
-        const T* v = static_cast<const T*>(a.v) + t * a.kv_stride;
-        char* qo = static_cast<char*>(a.q_out) + t * a.q_heads * c.dim * q_bytes;
-        const long long tab = (long long)w.pos * half;
-        if constexpr (VEC) {
-            const bool turned = j * 16 < a.rot;
-            float cs[8], sn[8];
-            if (turned) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    cs[i] = __ldg(a.cos_t + tab + j * 8 + i);
-                    sn[i] = __ldg(a.sin_t + tab + j * 8 + i);
-                }
+    if constexpr (VEC) {
+        constexpr int Q = sizeof(T) == 4 ? 2 : 1;     // 16-byte loads of eight values
+        // First dims of an item's two runs: the halves of the rotated dims in the half layout, and of what passes behind
+        // them; the halves of the head otherwise. Neighbouring threads take neighbouring runs.
+        const auto runs_of = [&](int j, bool is_v, int& d0, int& d1) {
+            if (is_v || a.interleaved) {
+                d0 = j * 8;
+                d1 = c.dim / 2 + j * 8;
+            } else if (j * 16 < a.rot) {
+                d0 = j * 8;
+                d1 = half + j * 8;
+            } else {
+                d0 = a.rot + (j - a.rot / 16) * 8;
+                d1 = d0 + (c.dim - a.rot) / 2;
             }
-            for (int it = threadIdx.x; it < items; it += kThreads) {
-                const int h = it / per_head;
+        };
+        // kBatch items of a thread have their loads in flight before the first is worked on
+        for (int i0 = threadIdx.x; i0 < nt * items; i0 += kBatch * kThreads) {
+            uint4 raw[kBatch][2][Q];
+            int what[kBatch];                         // token << 16 | head, or -1
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                const int i = i0 + n * kThreads;
+                what[n] = -1;
+                if (i >= nt * items) continue;
+                const int u = int(per_token.div(i)), it = i - u * items, h = it / per_head, j = it % per_head;
+                if (place[u].pos < 0) continue;
+                const long long t = t0 + u;
                 const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + c.kv_heads;
-                const int hk = is_q ? 0 : is_v ? h - a.q_heads - c.kv_heads : h - a.q_heads;
-                const T* src = is_q ? q + h * c.dim : (is_v ? v : k) + hk * c.dim;
-                const bool rot = turned && !is_v;
-                // first and second run of eight
-                const int d0 = rot && !a.interleaved ? j * 8 : j * 16;
-                const int d1 = rot && !a.interleaved ? half + j * 8 : j * 16 + 8;
+                const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_stride + h * c.dim
+                                    : static_cast<const T*>(is_v ? a.v : a.k) + t * a.kv_stride +
+                                          (h - a.q_heads - (is_v ? c.kv_heads : 0)) * c.dim;
+                int d0, d1;
+                runs_of(j, is_v, d0, d1);
+#pragma unroll
+                for (int e = 0; e < Q; ++e) {
+                    raw[n][0][e] = __ldg(reinterpret_cast<const uint4*>(src + d0) + e);
+                    raw[n][1][e] = __ldg(reinterpret_cast<const uint4*>(src + d1) + e);
+                }
+                what[n] = u << 16 | h;
+            }
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n) {
+                if (what[n] < 0) continue;
+                const int u = what[n] >> 16, h = what[n] & 0xffff, j = (i0 + n * kThreads) % per_head;
+                const Place w = place[u];
+                const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + c.kv_heads;
+                int d0, d1;
+                runs_of(j, is_v, d0, d1);
                 float x[8], y[8];
-                load8(src + d0, x);
-                load8(src + d1, y);
-                if (rot) {
-                    if (a.interleaved) {
+                unpack8<T>(raw[n][0], x);
+                unpack8<T>(raw[n][1], y);
+                const long long tab = (long long)w.pos * half;
+                if (!is_v && a.interleaved) {         // each run: four pairs of its own
+                    if (d0 < a.rot) turn_pairs(x, a.cos_t + tab + d0 / 2, a.sin_t + tab + d0 / 2);
+                    if (d1 < a.rot) turn_pairs(y, a.cos_t + tab + d1 / 2, a.sin_t + tab + d1 / 2);
+                } else if (!is_v && j * 16 < a.rot) { // eight pairs across the runs
+                    const float4* ct = reinterpret_cast<const float4*>(a.cos_t + tab + d0);
+                    const float4* st = reinterpret_cast<const float4*>(a.sin_t + tab + d0);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = x[2 * i], r = x[2 * i + 1], s = y[2 * i], z = y[2 * i + 1];
-                            x[2 * i] = p * cs[i] - r * sn[i];
-                            x[2 * i + 1] = r * cs[i] + p * sn[i];
-                            y[2 * i] = s * cs[4 + i] - z * sn[4 + i];
-                            y[2 * i + 1] = z * cs[4 + i] + s * sn[4 + i];
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float p = x[i], r = y[i];
-                            x[i] = p * cs[i] - r * sn[i];
-                            y[i] = r * cs[i] + p * sn[i];
-                        }
+                    for (int e = 0; e < 2; ++e) {
+                        const float4 c4 = __ldg(ct + e), s4 = __ldg(st + e);
+                        turn(x[4 * e], y[4 * e], c4.x, s4.x);
+                        turn(x[4 * e + 1], y[4 * e + 1], c4.y, s4.y);
+                        turn(x[4 * e + 2], y[4 * e + 2], c4.z, s4.z);
+                        turn(x[4 * e + 3], y[4 * e + 3], c4.w, s4.w);
                     }
                 }
                 if (is_q) {
-                    store8(qo + (long long)(h * c.dim + d0) * q_bytes, x, a.q_type);
-                    store8(qo + (long long)(h * c.dim + d1) * q_bytes, y, a.q_type);
+                    char* qo = static_cast<char*>(a.q_out) + ((t0 + u) * (long long)a.q_heads + h) * c.dim * q_bytes;
+                    store8(qo + d0 * q_bytes, x, a.q_type);
+                    store8(qo + d1 * q_bytes, y, a.q_type);
                 } else if (w.k) {
-                    char* dst = (is_v ? w.v : w.k) + hk * c.head_stride;
+                    char* dst = (is_v ? w.v : w.k) + (h - a.q_heads - (is_v ? c.kv_heads : 0)) * c.head_stride;
                     store8(dst + d0 * 2, x, a.kv_type);
                     store8(dst + d1 * 2, y, a.kv_type);
                 }
             }
-        } else {
+        }
+    } else {
+        // blockDim is a multiple of per_head: a thread keeps its pair's number over the heads
+        const int j = threadIdx.x % per_head;
+        for (int u = 0; u < nt; ++u) {
+            const Place w = place[u];
+            if (w.pos < 0) continue;
+            const long long t = t0 + u;
+            const T* q = static_cast<const T*>(a.q) + t * a.q_stride;
+            const T* k = static_cast<const T*>(a.k) + t * a.kv_stride;
+            const T* v = static_cast<const T*>(a.v) + t * a.kv_stride;
+            char* qo = static_cast<char*>(a.q_out) + t * a.q_heads * c.dim * q_bytes;
+            const long long tab = (long long)w.pos * half;
             const bool turned = j < half;
             const float cs = turned ? __ldg(a.cos_t + tab + j) : 1.f, sn = turned ? __ldg(a.sin_t + tab + j) : 0.f;
             for (int it = threadIdx.x; it < items; it += kThreads) {
@@ -153,11 +198,12 @@ void launch(const KvView& c, const KvBatch& b, const AppendArgs& a, cudaStream_t
     const auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const int run = 16 / int(sizeof(T));
     const bool vec = al(a.q) && al(a.k) && al(a.v) && al(a.q_out) && a.q_stride % run == 0 && a.kv_stride % run == 0 &&
-                     a.rot % 16 == 0;
+                     a.rot % 16 == 0 && al(a.cos_t) && al(a.sin_t);
     const int per = b.tokens >= 148 * 8 * kTokens ? kTokens : 1;
     const int grid = (b.tokens + per - 1) / per;
-    if (vec) kv_append_kernel<T, true><<<grid, kThreads, 0, s>>>(c, b, a, per);
-    else kv_append_kernel<T, false><<<grid, kThreads, 0, s>>>(c, b, a, per);
+    const FastDiv div = FastDiv::of(uint32_t((a.q_heads + 2 * c.kv_heads) * (c.dim / 16)));
+    if (vec) kv_append_kernel<T, true><<<grid, kThreads, 0, s>>>(c, b, a, per, div);
+    else kv_append_kernel<T, false><<<grid, kThreads, 0, s>>>(c, b, a, per, div);
     check_launch("kv_append");
 }
 

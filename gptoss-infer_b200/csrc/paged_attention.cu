@@ -137,7 +137,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
     __shared__ long long scratch[kWarps + 2];
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Schedule<R, kGroup> sch{c, b, a.window, group, 1};
+    const Schedule<R, kGroup> sch{c, b, a.window, group, 1, a.rows_from, a.rows_to};
     const Span sp = find_span<kThreads>(sch, kWarps * (NS - 1), scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
@@ -586,6 +586,15 @@ void by_shape(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* w
     }
 }
 
+// Query rows per key/value head up to which the kernel of this file takes a sequence.
+constexpr int kFewRows = 64;
+
+void few_rows(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+    if (a.type == kF32) by_shape<float, __half>(c, b, a, ws, s);
+    else if (a.type == kF16) by_shape<__half, __half>(c, b, a, ws, s);
+    else by_shape<__nv_bfloat16, __nv_bfloat16>(c, b, a, ws, s);
+}
+
 }  // namespace
 
 size_t paged_attention_ws_bytes(int dim) {
@@ -593,10 +602,21 @@ size_t paged_attention_ws_bytes(int dim) {
 }
 
 void launch_paged_attention(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
-    if ((long long)b.max_new * (a.q_heads / c.kv_heads) > 64) return launch_paged_tiles(maps, c, b, a, ws, s);
-    if (a.type == kF32) by_shape<float, __half>(c, b, a, ws, s);
-    else if (a.type == kF16) by_shape<__half, __half>(c, b, a, ws, s);
-    else by_shape<__nv_bfloat16, __nv_bfloat16>(c, b, a, ws, s);
+    const long long most = (long long)b.max_new * (a.q_heads / c.kv_heads);
+    if (most <= kFewRows) return few_rows(c, b, a, ws, s);
+    // Chunks go to the tensor-core tiles. Where sequences differ in length (the batch's tokens say so), those of few rows,
+    // decoding beside a chunk, are left out of that launch and take one of their own.
+    const bool mixed = b.tokens < (long long)b.seqs * b.max_new && b.seqs > 1;
+    PagedAttnArgs part = a;
+    if (mixed) part.rows_from = kFewRows + 1;
+    launch_paged_tiles(maps, c, b, part, ws, s);
+    if (!mixed) return;
+    part.rows_from = 0;
+    part.rows_to = kFewRows;
+    KvBatch few = b;
+    // (their mean length, the longest sequence aside, steers the choice of tile)
+    few.max_new = std::max(1, (b.tokens - b.max_new + b.seqs - 2) / (b.seqs - 1));
+    few_rows(c, few, part, ws, s);
 }
 
 }  // namespace gpt

@@ -249,7 +249,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
 
     const int warp = int(threadIdx.x / 32), lane = threadIdx.x % 32;
     int* err = c.err;
-    const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1};
+    const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1, a.rows_from, a.rows_to};
     const Span sp = find_span<kThreads>(sch, 2, scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
@@ -296,12 +296,16 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
         const auto load_queries = [&] {
                 if (piece > 0 && good) good = all_ok(tc::mbar_wait(&bars[kQFree], (piece - 1) & 1, err, kKvWait + 1));
                 const int r0 = it.t * kRows;
+                const auto query = [&](int r) {       // row r's query
+                    const int tok = int(group.div(r0 + r));
+                    return static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride + (it.h * G + (r0 + r - tok * G)) * D;
+                };
+                const auto q_off = [&](int r, int ch) { return (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch); };
                 if constexpr (L::kSplit) {
+#pragma unroll 4
                     for (int r = warp - 8; r < kRows; r += kCopy / 32) {
                         float x[D / 32], top = 0.f;
-                        const int tok = int(group.div(r0 + r));
-                        const float* src = static_cast<const float*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
-                                           (it.h * G + (r0 + r - tok * G)) * D + lane * (D / 32);
+                        const float* src = reinterpret_cast<const float*>(query(r < it.rows ? r : 0)) + lane * (D / 32);
 #pragma unroll
                         for (int e = 0; e < D / 32; ++e) {
                             x[e] = r < it.rows ? src[e] : 0.f;
@@ -325,30 +329,33 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                         if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
                     }
                 } else {
-                    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+                    if (a.scale < 0.f) {
+                        // the sign goes to the queries, so that the largest product is the largest score
+                        for (int u = tid; u < kRows * CH; u += kCopy) {
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (u / CH < it.rows) x = *reinterpret_cast<const uint4*>(query(u / CH) + u % CH * 8);
+                            x.x ^= 0x80008000u; x.y ^= 0x80008000u; x.z ^= 0x80008000u; x.w ^= 0x80008000u;
+                            *reinterpret_cast<uint4*>(q_tile + q_off(u / CH, u % CH)) = x;
+                        }
+                    } else {
+                        const uint32_t q_at = tc::smem_u32(q_tile);
 #pragma unroll 8
-                    for (int u = tid; u < kRows * CH; u += kCopy) {
-                        const int r = u / CH, ch = u % CH, tok = int(group.div(r0 + r));
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (r < it.rows)
-                            x = __ldg(reinterpret_cast<const uint4*>(
-                                static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride +
-                                (it.h * G + (r0 + r - tok * G)) * D + ch * 8));
-                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                        *reinterpret_cast<uint4*>(q_tile + (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch)) = x;
+                        for (int u = tid; u < kRows * CH; u += kCopy) {
+                            const bool ok = u / CH < it.rows;
+                            cp_async16_zfill(q_at + q_off(u / CH, u % CH), query(ok ? u / CH : 0) + u % CH * 8, ok);
+                        }
+                        cp_async_commit();
+                        cp_async_wait_group<0>();
                     }
                 }
                 tc::fence_proxy_async_smem();
                 arrive_warp(&bars[kQFull]);
         };
-        // 16 bytes of values that some row must not see (NaN or infinity would reach it through a product)
-        const auto not_finite = [](const uint4& x) {
-            constexpr uint32_t e = kBf16 ? 0x7f80u : 0x7c00u;
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            bool bad = false;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) bad |= (w[k] & e) == e || (w[k] >> 16 & e) == e;
-            return bad;
+        // Bits 15 and 31 of the result: one of the eight values is NaN or infinite (an exponent of all ones, which one more
+        // carries into the sign's place). Values that some row must not see are checked: a product would carry them there.
+        const auto exponents = [](const uint4& x) {
+            constexpr uint32_t one = kBf16 ? 0x00800080u : 0x04000400u, rest = 0x7fff7fffu;
+            return ((x.x & rest) + one) | ((x.y & rest) + one) | ((x.z & rest) + one) | ((x.w & rest) + one);
         };
         const auto wait_free = [&] {                  // until the ring's next place is free
             if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1, err, kKvWait));
@@ -384,29 +391,39 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
             while (at < sp.len) {                     // after a failed wait: barriers only
                 const int g1 = min(it.n, g0 + sp.len - at);
                 const int lo_last = a.window ? max(0, it.p1 - a.window + 1) : 0;
+                const auto page_of = [&](int k0) {
+                    return lane < boxes && k0 + lane * box < it.hi ? safe_page(id, c) : 0;
+                };
                 look_up(it.lo + g0 * kTile);
+                int page = page_of(it.lo + g0 * kTile);
+                issue(&maps.k, it.lo + g0 * kTile, page, &bars[kTileFull + issued % NS]);
+                if (g0 + 1 < g1) look_up(it.lo + (g0 + 1) * kTile);
+                load_queries();
                 for (int g = g0; g < g1; ++g) {
-                    const int k0 = it.lo + g * kTile;
+                    const int k0 = it.lo + g * kTile, slot = issued % NS;
                     const bool edge = k0 + kTile > it.p0 + 1 || k0 < lo_last;
-                    const int page = id < 0 && !(lane < boxes && k0 + lane * box < it.hi) ? 0 : safe_page(id, c);
-                    issue(&maps.k, k0, page, &bars[kTileFull + issued % NS]);
-                    if (g + 1 < g1) look_up(k0 + kTile);
-                    if (g == g0) load_queries();
-                    const int slot = issued % NS;
                     issue(&maps.v, k0, page, &bars[edge ? int(kEdge) : kTileFull + slot]);
+                    if (g + 1 < g1) {                 // the next keys are on their way while the values are checked
+                        page = page_of(k0 + kTile);
+                        issue(&maps.k, k0 + kTile, page, &bars[kTileFull + issued % NS]);
+                        if (g + 2 < g1) look_up(k0 + 2 * kTile);
+                    }
                     if (edge) {
                         // some row does not see all of these values: slots past the sequence's end (whatever they hold)
                         // become zeros, and the others are checked
                         if (good) good = all_ok(tc::mbar_wait(&bars[kEdge], edges & 1, err, kKvWait + 1));
                         ++edges;
-                        bool bad = false;
-                        for (int i = tid; i < kTile * CH && good; i += kCopy) {
-                            const int r = i / CH;
-                            uint4* x = reinterpret_cast<uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, i % CH));
-                            if (k0 + r >= it.hi) *x = make_uint4(0, 0, 0, 0);
-                            else bad |= not_finite(*x);
+                        char* v = ring + slot * L::kTileBytes;
+                        const int valid = min(kTile, it.hi - k0);
+                        uint32_t seen = 0;
+                        if (good) {
+                            for (int i = tid + valid * CH; i < kTile * CH; i += kCopy)
+                                *reinterpret_cast<uint4*>(v + image_off<D>(i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
+#pragma unroll 8
+                            for (int i = tid; i < valid * CH; i += kCopy)
+                                seen |= exponents(*reinterpret_cast<const uint4*>(v + image_off<D>(i / CH, i % CH)));
                         }
-                        if (bad) flags[piece & 7] = piece + 1;
+                        if (seen & 0x80008000u) flags[piece & 7] = piece + 1;
                         tc::fence_proxy_async_smem();
                         bar_copies<kCopy>();
                         if (tid == 0 && good) tc::mbar_arrive(&bars[kTileFull + slot]);
@@ -425,12 +442,12 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
             tc::fence_proxy_async_smem();
             const int slot = done % NS;
             if (check) {
-                bool bad = false;
+                uint32_t seen = 0;
                 for (int i = 0; i < kTile * CH / kCopy; ++i) {
                     const int r = i * (kCopy / CH) + tid / CH, ch = tid % CH;
-                    bad |= not_finite(*reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, ch)));
+                    seen |= exponents(*reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, ch)));
                 }
-                if (bad) flags[(check - 1) & 7] = check;
+                if (seen & 0x80008000u) flags[(check - 1) & 7] = check;
             }
             arrive_warp(&bars[kTileFull + slot]);
             ++done;

@@ -241,7 +241,7 @@ int gptoss_paged_attention(gptoss_kv_pool* p, int layer, const gptoss_kv_batch* 
         require((long long)b.tokens * q_heads < (1ll << 31) && b.tokens < (1 << 24),
                 "paged_attention: too many tokens in one call");
         check_device(p, "paged_attention");
-        gpt::PagedAttnArgs a{q, out, sinks, q_stride, out_stride, type, p->type, q_heads, window, scale};
+        gpt::PagedAttnArgs a{q, out, sinks, q_stride, out_stride, type, p->type, q_heads, window, scale, 0, 0x7fffffff};
         gpt::launch_paged_attention(p->maps, p->view(layer), b, a, p->attn_ws, static_cast<cudaStream_t>(stream));
     });
 }

@@ -29,7 +29,14 @@ struct Schedule {
     int window;
     FastDiv group;
     int align;               // lo is a multiple of this (a power of two)
+    int rows_from, rows_to;  // only sequences with so many rows (new tokens x group) have items
 
+    __device__ __forceinline__ Seq seq(int i) const {
+        Seq s = load_seq(b, c.page, i, c.err);
+        const int rows = s.n * int(group.d);
+        if (rows < rows_from || rows > rows_to) s.n = 0;
+        return s;
+    }
     __device__ __forceinline__ int row_tiles(int n) const { return (n * int(group.d) + R - 1) / R; }
 
     __device__ __forceinline__ void fill(Item& it) const {
@@ -58,7 +65,7 @@ struct Schedule {
     // First item at or after (b, 0, 0); false past the last sequence.
     __device__ __forceinline__ bool open(Item& it, int i) const {
         for (; i < b.seqs; ++i) {
-            it.s = load_seq(b, c.page, i, c.err);
+            it.s = seq(i);
             it.nt = row_tiles(it.s.n);
             if (it.nt > 0) {
                 it.b = i;
@@ -139,7 +146,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
     if (seqs <= 32) {                                 // each warp for itself, a lane per sequence
         const int lane = threadIdx.x % 32;
         Seq s{0, 0, 0};
-        if (lane < seqs) s = load_seq(sch.b, sch.c.page, lane, sch.c.err);
+        if (lane < seqs) s = sch.seq(lane);
         int units = sch.head_groups(s, 1);
         long long total = (long long)units * kvh;
         int items = sch.row_tiles(s.n) * kvh;
@@ -186,7 +193,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
     long long total = 0, mine = 0, before = 0;
     for (int i0 = 0; i0 < seqs; i0 += NT) {
         const int i = i0 + threadIdx.x;
-        mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err), 1) * kvh : 0;
+        mine = i < seqs ? (long long)sch.head_groups(sch.seq(i), 1) * kvh : 0;
         long long sum;
         before = total + block_prefix<NT>(mine, scratch, &sum);
         total += sum;
@@ -201,7 +208,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
         long long base = 0;
         for (int i0 = 0; i0 < seqs; i0 += NT) {
             const int i = i0 + threadIdx.x;
-            mine = i < seqs ? (long long)sch.head_groups(load_seq(sch.b, sch.c.page, i, sch.c.err), 1) * kvh : 0;
+            mine = i < seqs ? (long long)sch.head_groups(sch.seq(i), 1) * kvh : 0;
             long long sum;
             before = base + block_prefix<NT>(mine, scratch, &sum);
             base += sum;
