@@ -111,12 +111,19 @@ template <int N>
 __device__ __forceinline__ void bar_copies() { asm volatile("bar.sync 2, %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bar_rows() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-// Scores outside [from, to] become -infinity.
+// Scores outside [from, to] become -infinity: a word of bits per run of 32, tested bit by bit (branches around the
+// scores' registers made them spill).
 template <int N>
 __device__ __forceinline__ void mask(uint32_t (&x)[N], int from, int to) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (i < from || i > to) x[i] = 0xff800000u;
+    for (int r = 0; r < N; r += 32) {
+        const int lo = min(max(from - r, 0), 32), hi = min(max(to - r + 1, 0), 32);      // seen: [lo, hi)
+        const uint32_t below_hi = hi == 32 ? ~0u : (1u << hi) - 1, below_lo = lo == 32 ? ~0u : (1u << lo) - 1;
+        const uint32_t seen = below_hi & ~below_lo;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (!(seen & (1u << i))) x[r + i] = 0xff800000u;
+    }
 }
 
 // Two fp32 values in a register pair: one instruction for both.
@@ -617,6 +624,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
             const int head = it.h * G + (r0 + rr - tok * G);
             const int p = it.s.len - it.s.n + tok, first = a.window ? p - a.window + 1 : 0;
             const bool mine = t < halves && good, valid = row < it.rows && good;   // after a failed wait: barriers only
+            const float sink = a.sinks ? a.sinks[head] * kLog2e : -INFINITY;
             float m = -INFINITY, l = 0.f, sc = fabsf(a.scale) * kLog2e;
             if (mine) {
                 // first and last position of this half's rows: between them some tiles are partly masked
@@ -696,7 +704,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 }
             };
             const auto inverse = [&](float mm, float z) {
-                if (a.sinks && z > 0.f) z += ex2(a.sinks[head] * kLog2e - mm);
+                if (z > 0.f) z += ex2(sink - mm);
                 return z == 0.f ? 0.f : 1.f / z;
             };
             if (mine && good && flags[piece & 7] == piece + 1) {

@@ -49,17 +49,52 @@ struct Schedule {
         it.n = max(1, (it.hi - it.lo + UNIT - 1) / UNIT);
     }
 
-    // Groups of one key/value head of a sequence, each item's rounded up to a multiple of pad.
-    __device__ __forceinline__ int head_groups(const Seq& s, int pad) const {
+    // Groups of tile t of a sequence, rounded up to a multiple of pad.
+    __device__ __forceinline__ int tile_groups(const Seq& s, int t, int pad) const {
         Item it;
         it.s = s;
-        it.nt = row_tiles(s.n);
+        it.t = t;
+        fill(it);
+        return pad == 1 ? it.n : (it.n + pad - 1) / pad * pad;
+    }
+    // Groups of one key/value head of each lane's sequence: a few tiles by the lane itself, more by the whole warp, a lane
+    // per tile (64 tiles by one lane took 4 us). All lanes call it.
+    __device__ __forceinline__ int head_groups(const Seq& s, int pad) const {
+        const int lane = threadIdx.x % 32, nt = row_tiles(s.n);
         int sum = 0;
-        for (it.t = 0; it.t < it.nt; ++it.t) {
-            fill(it);
-            sum += pad == 1 ? it.n : (it.n + pad - 1) / pad * pad;
+        if (nt <= 2)
+            for (int t = 0; t < nt; ++t) sum += tile_groups(s, t, pad);
+        for (unsigned many = __ballot_sync(kFull, nt > 2); many; many &= many - 1) {
+            const int src = __ffs(many) - 1;
+            const Seq q{__shfl_sync(kFull, s.row0, src), __shfl_sync(kFull, s.n, src), __shfl_sync(kFull, s.len, src)};
+            int part = 0;
+            for (int t = lane; t < row_tiles(q.n); t += 32) part += tile_groups(q, t, pad);
+            part = __reduce_add_sync(kFull, part);
+            if (lane == src) sum = part;
         }
         return sum;
+    }
+    // The tile of the item's head that holds group `off` of it; off becomes the group within the tile. All lanes call it.
+    __device__ __forceinline__ void find_tile(Item& it, int& off, int pad) const {
+        const int lane = threadIdx.x % 32;
+        for (int t0 = 0;; t0 += 32) {
+            const int n = t0 + lane < it.nt ? tile_groups(it.s, t0 + lane, pad) : 0;
+            int end = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(kFull, end, o);
+                if (lane >= o) end += y;
+            }
+            const unsigned holds = __ballot_sync(kFull, off < end);
+            if (holds || t0 + 32 >= it.nt) {
+                const int src = holds ? __ffs(holds) - 1 : 0;
+                it.t = t0 + src;
+                off -= __shfl_sync(kFull, end - n, src);
+                break;
+            }
+            off -= __shfl_sync(kFull, end, 31);
+        }
+        fill(it);
     }
 
     // First item at or after (b, 0, 0); false past the last sequence.
@@ -181,11 +216,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
         it.nt = sch.row_tiles(it.s.n);
         it.h = in_seq >> 31 ? int(in_seq / units) : int(unsigned(in_seq) / unsigned(units));
         int off = int(in_seq - (long long)it.h * units);
-        it.t = 0;
-        for (sch.fill(it); off >= (it.n + pad - 1) / pad * pad; sch.fill(it)) {
-            off -= (it.n + pad - 1) / pad * pad;
-            ++it.t;
-        }
+        sch.find_tile(it, off, pad);
         sp.g = off;
         sp.len = whole ? min(sp.per, it.n - off) : int(min((long long)sp.per, total - sp.start));
         return sp;
@@ -193,7 +224,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
     long long total = 0, mine = 0, before = 0;
     for (int i0 = 0; i0 < seqs; i0 += NT) {
         const int i = i0 + threadIdx.x;
-        mine = i < seqs ? (long long)sch.head_groups(sch.seq(i), 1) * kvh : 0;
+        mine = (long long)sch.head_groups(i < seqs ? sch.seq(i) : Seq{0, 0, 0}, 1) * kvh;
         long long sum;
         before = total + block_prefix<NT>(mine, scratch, &sum);
         total += sum;
@@ -208,7 +239,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
         long long base = 0;
         for (int i0 = 0; i0 < seqs; i0 += NT) {
             const int i = i0 + threadIdx.x;
-            mine = i < seqs ? (long long)sch.head_groups(sch.seq(i), 1) * kvh : 0;
+            mine = (long long)sch.head_groups(i < seqs ? sch.seq(i) : Seq{0, 0, 0}, 1) * kvh;
             long long sum;
             before = base + block_prefix<NT>(mine, scratch, &sum);
             base += sum;
@@ -227,11 +258,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
     const int per_head = sch.head_groups(sp.it.s, 1);
     sp.it.h = in_seq >> 31 ? int(in_seq / per_head) : int(unsigned(in_seq) / unsigned(per_head));
     int off = int(in_seq - (long long)sp.it.h * per_head);
-    while (off >= sp.it.n) {
-        off -= sp.it.n;
-        ++sp.it.t;
-        sch.fill(sp.it);
-    }
+    sch.find_tile(sp.it, off, 1);
     sp.g = off;
     return sp;
 }
