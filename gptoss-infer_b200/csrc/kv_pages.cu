@@ -33,17 +33,25 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // All CTAs of a cooperative launch meet. Bounded; after a wait that gave up the error word is set and the kernel goes on
 // (the arrays it reads are within bounds whatever they hold).
-__device__ __forceinline__ void grid_barrier(unsigned long long* barrier, int* err) {
+// The last to arrive sets the arrivals back to 0 and lets the others go by a new number, so launches of any size follow
+// one another.
+__device__ __forceinline__ void grid_barrier(int* barrier, int* err) {
     __syncthreads();
     if (threadIdx.x == 0) {
-        unsigned long long old, now;
-        asm volatile("atom.add.acq_rel.gpu.global.u64 %0, [%1], 1;" : "=l"(old) : "l"(barrier) : "memory");
-        const unsigned long long target = (old / gridDim.x + 1) * gridDim.x;
-        uint32_t i = 0;
-        do {
-            asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(now) : "l"(barrier) : "memory");
-        } while (now < target && ++i < tc::kSpinLimit);
-        if (now < target) report(err, kKvWait + 9);
+        const auto number = [&] {
+            int n;
+            asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(n) : "l"(barrier + 1) : "memory");
+            return n;
+        };
+        const int before = number();
+        if (arrive(barrier) == int(gridDim.x) - 1) {
+            barrier[0] = 0;
+            arrive(barrier + 1);
+        } else {
+            uint32_t i = 0;
+            while (number() == before && i < tc::kSpinLimit) ++i;
+            if (i == tc::kSpinLimit) report(err, kKvWait + 9);
+        }
     }
     __syncthreads();
 }
@@ -311,7 +319,7 @@ size_t kv_pages_ws_bytes(int num_pages, int children, int seqs) {
 PageWs make_kv_pages_ws(void* ws, int num_pages, int children, int seqs) {
     char* p = static_cast<char*>(ws);
     PageWs w;
-    w.barrier = reinterpret_cast<unsigned long long*>(p);
+    w.barrier = reinterpret_cast<int*>(p);
     w.count = reinterpret_cast<int*>(p + 128);
     w.delta = reinterpret_cast<int*>(p += 256);
     w.free_page = reinterpret_cast<int*>(p += up256(size_t(num_pages) * 4));

@@ -120,7 +120,7 @@ struct KvPages {
 // Workspace of both, for up to so many children and sequences of a call: zeroed memory, laid out and prepared once by
 // make_kv_pages_ws (on the legacy default stream). The kernels leave it as they found it.
 struct PageWs {
-    unsigned long long* barrier;   // arrivals, ever: a launch leaves a multiple of its grid size
+    int* barrier;                  // arrivals, left at 0, and the number of the last barrier passed
     int* count;                    // [0] moves
     int* delta;                    // [num_pages] change of the counts; left at 0
     int* free_page;                // [num_pages]

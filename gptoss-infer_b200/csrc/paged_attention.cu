@@ -15,6 +15,10 @@
 // score passes it by 2^8: weights are at most 256, which both 16-bit types and the fp32 sums hold without loss, and
 // most groups need no exchange between lanes at all.
 //
+// Measured: 64 sequences of 4K to 8K positions, one token each, 64 query heads over 8 of 64, bf16: 149 us, 5.5 TB/s (0.84
+// of the measured copy) with slot-major pages, whose rows of one head are 1 KB apart, 135 us, 6.1 TB/s with head-major
+// ones; 32 heads over 4 of 128: 130 us, 6.3 TB/s. With rows along the instructions' long side, 16 keys at a time, 203 us.
+//
 // fp32 queries: a row is scaled by a power of two into [2^10, 2^11) and split into two fp16 parts (22 bits, exact
 // products with fp16 keys); the weights are split the same way for the second product.
 #include <algorithm>
@@ -555,8 +559,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
 
 constexpr int kMaxCtas = 2 * 160;                     // two CTAs per SM, SMs rounded up
 static_assert(kMaxCtas * sizeof(int) <= kCounterBytes, "one counter per CTA");
-constexpr int kSlotFloats = slot_floats<64, 64>() > slot_floats<32, 128>() ? slot_floats<64, 64>()
-                                                                              : slot_floats<32, 128>();
+constexpr int kSlotFloats = std::max(slot_floats<32, 64>(), slot_floats<16, 128>());
 
 template <class T, class C, int D, int NT>
 void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
@@ -577,17 +580,18 @@ void by_shape(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* w
     if (c.dim == 64) {
         if (rows <= 8) launch<T, C, 64, 1>(c, b, a, ws, s);
         else if (rows <= 16) launch<T, C, 64, 2>(c, b, a, ws, s);
-        else if (rows <= 32) launch<T, C, 64, 4>(c, b, a, ws, s);
-        else launch<T, C, 64, 8>(c, b, a, ws, s);
+        else launch<T, C, 64, 4>(c, b, a, ws, s);
     } else {
         if (rows <= 8) launch<T, C, 128, 1>(c, b, a, ws, s);
-        else if (rows <= 16) launch<T, C, 128, 2>(c, b, a, ws, s);
-        else launch<T, C, 128, 4>(c, b, a, ws, s);
+        else launch<T, C, 128, 2>(c, b, a, ws, s);
     }
 }
 
-// Query rows per key/value head up to which the kernel of this file takes a sequence.
-constexpr int kFewRows = 64;
+// Query rows per key/value head up to which the kernel of this file takes a sequence. Both sides, 64 sequences of 4K to 8K
+// positions / 2 of them, 64 query heads over 8: 64 rows of heads of 64 (as two tiles of 32) 296 / 28 us here, 285 / 42 us on
+// the 128-row tiles; 32 rows 170 / 24 us here, 254 / 43 us there. Heads of 128 (32 over 4): 32 rows 283 us here, 259 us there,
+// 64 rows 492 us and 211 us.
+int few_rows_of(int dim) { return dim == 64 ? 64 : 16; }
 
 void few_rows(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
     if (a.type == kF32) by_shape<float, __half>(c, b, a, ws, s);
@@ -603,16 +607,17 @@ size_t paged_attention_ws_bytes(int dim) {
 
 void launch_paged_attention(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
     const long long most = (long long)b.max_new * (a.q_heads / c.kv_heads);
-    if (most <= kFewRows) return few_rows(c, b, a, ws, s);
+    const int few_at_most = few_rows_of(c.dim);
+    if (most <= few_at_most) return few_rows(c, b, a, ws, s);
     // Chunks go to the tensor-core tiles. Where sequences differ in length (the batch's tokens say so), those of few rows,
     // decoding beside a chunk, are left out of that launch and take one of their own.
     const bool mixed = b.tokens < (long long)b.seqs * b.max_new && b.seqs > 1;
     PagedAttnArgs part = a;
-    if (mixed) part.rows_from = kFewRows + 1;
+    if (mixed) part.rows_from = few_at_most + 1;
     launch_paged_tiles(maps, c, b, part, ws, s);
     if (!mixed) return;
     part.rows_from = 0;
-    part.rows_to = kFewRows;
+    part.rows_to = few_at_most;
     KvBatch few = b;
     // (their mean length, the longest sequence aside, steers the choice of tile)
     few.max_new = std::max(1, (b.tokens - b.max_new + b.seqs - 2) / (b.seqs - 1));

@@ -5,10 +5,17 @@
 //   S = Q K^T            tcgen05.mma kind::f16, both operands in shared memory, K-major, accumulator in TMEM
 //   P = exp2(S - m)      one thread per row, no exchange between threads
 //   O += P V             A operand P read from TMEM, V in shared memory as stored (rows = keys)
-// S is taken in tiles of 64 keys, read into registers and released at once, so the next scores are made while this
-// tile's exponentials run; while one half waits for products the other computes.
+// S is taken in tiles of 64 keys (128 for 16-bit heads of 64, whose P has columns of its own), read into registers and
+// released at once, so the next scores are made while this tile's exponentials run; the products are issued in the order
+// in which two halves half a step apart need them.
 //
-// Bound: with heads of 64 the exponentials (128 x 128 per 4.2 MFLOP, 16 a clock and SM), with heads of 128 the products.
+// Bound: the exponentials: 16 a clock and SM, 2048 cycles for 256 rows x 128 keys, against 1024 (heads of 64) and 2560
+// (heads of 128) of products. Measured, 2048 new tokens over 16384 positions, 64 query heads over 8, bf16: heads of 64
+// 668 us, 771 TFLOP/s, 46 % of the measured matrix rate: about 3100 cycles a step. Two warps of rows per scheduler do not
+// keep the special-function unit busy alone (a warp's 128 exponentials take about 1800 cycles by themselves), and waits
+// for products (about 600 cycles from weights written to their product seen) fall between. 32 heads of 128 over 4: 500 us,
+// 1031 TFLOP/s. Tried: reading the scores twice instead of holding them (1110 us), halves taking strict turns at the
+// exponentials (974 us), polling for whatever product is ready (735 us), 3 and 4 of 8 exponentials on the fp32 pipes.
 //
 // Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output); the next two copy keys and values through a
 // ring of tiles with TMA (a box per run of slots in a page; page sizes that are multiples of 8), or the next four with

@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -231,6 +232,7 @@ int gptoss_paged_attention(gptoss_kv_pool* p, int layer, const gptoss_kv_batch* 
         require(q_heads >= kvh && q_heads % kvh == 0 && q_heads <= 4096,
                 "paged_attention: q_heads is a multiple of kv_heads, at most 4096");
         require(window >= 0, "paged_attention: negative window");
+        require(std::isfinite(scale) && scale != 0.f, "paged_attention: the scale must be finite and not 0");
         if (b.seqs == 0 || b.tokens == 0) return;
         require(q && out, "paged_attention: null pointer");
         const long long row = (long long)q_heads * p->dim;

@@ -271,8 +271,8 @@ int gptoss_set_prefill_packing(int mode);
  * p * strides[1] + s * strides[2] + h * strides[3] + d (strides in elements, host array of 4, multiples of 8), so both
  * slot-major and head-major pages are described without a copy. type: 1 = fp16, 2 = bf16. head_dim 64 or 128; any
  * page_size >= 1. A sequence's table is an int32 row of page ids: position p lives in page table[p / page_size], slot
- * p % page_size; entries past its last position are never read. The handle owns its workspaces (a few MB) and an error
- * word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
+ * p % page_size; entries past its last position are never read. The handle owns its workspaces (about 22 MB, 43 MB for
+ * head_dim 128, and 16 bytes per page) and an error word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
  * current at its creation. Returns NULL on failure (gptoss_last_error). Synchronizes. */
 typedef struct gptoss_kv_pool gptoss_kv_pool;
 gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, int num_pages, int page_size,
@@ -313,8 +313,11 @@ int gptoss_kv_append(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* bat
  * positions j <= p of the token at p, and j > p - window with window > 0. Query head h reads key/value head
  * h / (q_heads / kv_heads). sinks: fp32 [q_heads] or NULL (no sink term). q and out: [tokens] rows of q_heads *
  * head_dim, q_stride and out_stride elements apart, 16-byte aligned, of the cache's type, or fp32 beside an fp16 cache
- * (products then keep about 22 bits). Statistics and sums are fp32. A row that sees no key is 0. Results do not depend
- * on timing. */
+ * (products then keep about 22 bits). scale: finite, not 0. Statistics and sums are fp32. A row that sees no key is 0,
+ * and what a row may not see does not reach it, NaN and infinities included. Results do not depend on timing.
+ * Sequences of up to 64 query rows (new tokens x q_heads / kv_heads; 16 for head_dim 128) run on one kernel, longer
+ * chunks on another; a batch with both takes two launches. Page sizes that are multiples of 8 are the fast ones for
+ * chunks. */
 int gptoss_paged_attention(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* batch, const void* q, int type,
                            long long q_stride, int q_heads, const float* sinks, float scale, int window, void* out,
                            long long out_stride, void* stream);
@@ -326,7 +329,9 @@ int gptoss_paged_attention(gptoss_kv_pool* pool, int layer, const gptoss_kv_batc
  * without a child is thereby freed), the children's added. Full pages are shared. A part-filled last page stays with
  * the parent's first child if its count was 1, and is copied to a fresh page for every other child, in all layers of
  * the pool. Fresh pages are the lowest-numbered ones left with count 0, in the order of the children; if they run out,
- * the children concerned get the length that their pages hold and the pool's status is 304. */
+ * the children concerned get the length that their pages hold and the pool's status is 304. The pool makes its
+ * workspace anew when a call has more sequences or children than any before (256 at first): make such a call before a
+ * stream capture. A cooperative launch. */
 int gptoss_kv_fork(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* tables, const int32_t* lens, int seqs,
                    const int32_t* parents, const int32_t* extra, int children, int table_stride, int32_t* refs_out,
                    int32_t* tables_out, int32_t* lens_out, void* stream);
@@ -334,7 +339,7 @@ int gptoss_kv_fork(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* tab
 /* [extension] Moves the live pages (count > 0) to the lowest page numbers, in all layers, asynchronous on `stream`:
  * the live pages past the number of live pages go to the free ones below it, both in ascending order. remap[num_pages]:
  * each live page's new number, -1 for a free page; *live: how many there are. refs_out and tables_out (the tables of
- * `seqs` sequences with lengths lens, remapped, unused entries -1) may alias refs and tables. */
+ * `seqs` sequences with lengths lens, remapped, unused entries -1) may alias refs and tables. A cooperative launch. */
 int gptoss_kv_compact(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* tables, const int32_t* lens, int seqs,
                       int table_stride, int32_t* refs_out, int32_t* tables_out, int32_t* remap, int32_t* live,
                       void* stream);
@@ -347,7 +352,7 @@ int gptoss_kv_compact(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* 
  * places without a candidate get score -inf, row -1, token -1. Outputs [batch][picks]: out_scores fp32, rows (of
  * logits, so they serve as gptoss_kv_fork's parents), tokens. Sums and ranking use fp32 statistics and fp64 scores.
  * Uses the calling thread's workspace: calls from one thread must not overlap on the GPU, and the first call at a
- * larger size allocates (before a stream capture). */
+ * larger size allocates (make it before a stream capture). */
 int gptoss_beam_select(const void* logits, int type, long long row_stride, const float* scores, const uint8_t* done,
                        int done_token, int batch, int beams, int vocab, int picks, float* out_scores, int32_t* rows,
                        int32_t* tokens, void* stream);

@@ -287,6 +287,27 @@ def test_attention_large_scores(lib, pair, shape):
     assert ((out.double() - want).abs() <= 2 * U[pair[0]] * mag + 2e-3 * mag + 2.0 ** -24).all()
 
 
+@pytest.mark.parametrize("pair", PAIRS, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [([1, 1], [90, 50]), ([140], [300])], ids=["decode", "chunk"])
+def test_attention_negative_scale(lib, pair, shape):
+    s = Setup(lib, *shape, page=16, kvh=1, dim=64, dtype=pair[1], seed=15)
+    q, sinks = new_q(s.T, 8, 64, pair[0]), torch.randn(8, device="cuda")
+    check_attention(run_attention(lib, s, q, sinks, scale=-0.1), *reference_attention(s, q, sinks, -0.1, 0))
+
+
+@pytest.mark.parametrize("dim,page", [(64, 16), (64, 20), (128, 16), (128, 20)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_attention_chunks_of_many_pieces(lib, dim, page, window):
+    """Items cut over several CTAs and CTAs with several items, next to sequences of few rows; twice the same bits."""
+    s = Setup(lib, [1, 300, 1, 700, 64, 2, 129], [3000, 5000, 20, 700, 3000, 3000, 1000], page=page, kvh=2, dim=dim,
+              dtype=BF16, seed=16)
+    q = new_q(s.T, 16, dim, BF16)
+    outs = [run_attention(lib, s, q, None, window) for _ in range(3)]
+    check_attention(outs[0], *reference_attention(s, q, None, dim ** -0.5, window))
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+    assert s.pool.status() == 0
+
+
 def test_attention_on_another_stream_and_in_a_graph(lib):
     s = Setup(lib, [1, 1], [800, 333], page=16, kvh=8, dim=64, dtype=F16, seed=12)
     q = new_q(s.T, 64, 64, F32)
@@ -647,6 +668,28 @@ def test_fork(lib, seqs, children, page, most, layers, head_major):
     assert torch.equal(wk, k) and torch.equal(wv, v)
 
 
+def test_fork_and_compact_of_different_sizes_in_turn(lib):
+    """Calls of different sizes on one pool, one after another: what one launch leaves in the workspace (counts, grid-wide
+    barriers) has to suit the next."""
+    r = np.random.RandomState(5)
+    refs, tables, lens = make_sequences(r, 30, 16, 500, False, 700)
+    k, v = make_pages(2, len(refs), 16, 2, 64, F16, False, 3)
+    pool = Pool(lib, k, v)
+    stride = 40
+    for children in (1, 200, 3, 60, 7):
+        parents = [int(x) for x in r.randint(-1, 30, children)]
+        got = run_fork(lib, pool, refs, tables, lens, parents, [1] * children, stride)
+        want = reference_fork(refs, tables, lens, parents, [1] * children, 16, len(refs))
+        assert pool.status() == (304 if want[4] else 0)
+        assert got[0] == want[0] and got[2] == want[2]
+        assert got[1] == [t + [-1] * (stride - len(t)) for t in want[1]]
+        R, t = ints(refs), ints([row + [-1] * (stride - len(row)) for row in tables])
+        remap, live = torch.empty_like(R), ints([0])
+        ok(lib, lib.gptoss_kv_compact(pool.h, P(R), P(t), P(ints(lens)), children % 30, stride, P(R), P(t), P(remap),
+                                      P(live), stream()))
+        assert pool.status() == 0 and live.item() == sum(n > 0 for n in refs)
+
+
 def test_fork_runs_out_of_pages(lib):
     k, v = make_pages(1, 6, 4, 1, 64, F16, False, 3)
     pool = Pool(lib, k, v)
@@ -719,8 +762,8 @@ def test_refusals_with_a_pool(lib):
     t = torch.zeros(4096, device="cuda")
     b = capi.KvBatch(1, 2, 2, 1, P(t), P(t), P(t))
 
-    def attention(layer=0, batch=b, q=P(t), type=2, qs=256, heads=4, window=0, out=P(t), os=256):
-        return lib.gptoss_paged_attention(pool.h, layer, batch and ctypes.byref(batch), q, type, qs, heads, None, 1.0,
+    def attention(layer=0, batch=b, q=P(t), type=2, qs=256, heads=4, window=0, out=P(t), os=256, scale=1.0):
+        return lib.gptoss_paged_attention(pool.h, layer, batch and ctypes.byref(batch), q, type, qs, heads, None, scale,
                                           window, out, os, None)
 
     def append(q=P(t), k=P(t), type=2, qs=512, ks=512, heads=4, cos=P(t), n=8, rot=64, qt=2):
@@ -738,7 +781,8 @@ def test_refusals_with_a_pool(lib):
         (lambda: attention(heads=0), b"multiple"), (lambda: attention(window=-1), b"window"),
         (lambda: attention(q=None), b"null"), (lambda: attention(out=None), b"null"),
         (lambda: attention(qs=128), b"shorter"), (lambda: attention(q=P(t) + 2), b"aligned"),
-        (lambda: attention(os=257), b"aligned"),
+        (lambda: attention(os=257), b"aligned"), (lambda: attention(scale=0.0), b"scale"),
+        (lambda: attention(scale=float("nan")), b"scale"),
         (lambda: attention(batch=capi.KvBatch(-1, 2, 2, 1, P(t), P(t), P(t))), b"negative"),
         (lambda: attention(batch=capi.KvBatch(1, 2, 2, 1, None, P(t), P(t))), b"null pointer"),
         (lambda: append(type=9), b"type"), (lambda: append(qt=9), b"type"), (lambda: append(rot=63), b"rot_dim"),
