@@ -127,8 +127,8 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
     const int v0 = part * size, n = max(0, min(size, a.vocab - v0));
     if (threadIdx.x == 0) count = 0;
     if (!done) {
-        // --- the part's values, in registers as they are stored (16-bit ones in half the registers: three CTAs share an
-        // SM), -inf past the end
+        // --- the part's values, in registers as they are stored (16-bit ones in half the registers: three CTAs share
+        // an SM), -inf past the end
         constexpr int W = 16 / int(sizeof(T));        // values of a 16-byte load
         const T* src = static_cast<const T*>(a.logits) + (long long)row * a.row_stride + v0;
         const auto index = [&](int i) { return (i / W * kThreads + int(threadIdx.x)) * W + i % W; };
@@ -158,7 +158,8 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
         for (int i = 0; i < kPer; i += 2) top = fmaxf(fmaxf(top, x(i)), x(i + 1));
         const auto key_of = [&](float value, int i) {
             return value == -INFINITY ? 0ull
-                                      : (unsigned long long)ordered(value) << 32 | (0xffffffffu - uint32_t(v0 + index(i)));
+                                      : (unsigned long long)ordered(value) << 32 | (0xffffffffu - uint32_t(v0 +
+                                          index(i)));
         };
         float all = top;
 #pragma unroll
@@ -277,11 +278,12 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
         return b & 0x8000000000000000ull ? ~b : b | 0x8000000000000000ull;
     };
     // The threshold is the picks-th largest of the threads' best words, made different from one another by the thread's
-    // number in the 9 lowest bits (which only lowers it). If the list does not hold what reaches it (equal scores by the
-    // hundred), the candidates are ranked where they lie.
+    // number in the 9 lowest bits (which only lowers it). If the list does not hold what reaches it (equal scores by
+    // the hundred), the candidates are ranked where they lie.
     unsigned long long best = 0;
     for (int i = threadIdx.x; i < total; i += kThreads) best = max(best, order_of(i, __ldcg(mine + i)));
-    const unsigned long long least = kth_largest(best ? (best & ~511ull) | threadIdx.x : 0, a.picks, sorted, &threshold) & ~511ull;
+    const unsigned long long least = kth_largest(best ? (best & ~511ull) | threadIdx.x : 0, a.picks, sorted,
+        &threshold) & ~511ull;
     const auto collect = [&](unsigned long long least) {
         if (best && best >= least)
             for (int i = threadIdx.x; i < total; i += kThreads) {
@@ -305,11 +307,13 @@ beam_select_kernel(BeamArgs a, int parts, int size, int* counters, Found* found,
         a.tokens[out + at] = flat % a.vocab;
     };
     if (m <= kList) {
-        by_rank(m, [&](int j, int i) { return list[j] > list[i] || (list[j] == list[i] && flat_list[j] < flat_list[i]); },
+        by_rank(m, [&](int j, int i) { return list[j] > list[i] || (list[j] == list[i] &&
+            flat_list[j] < flat_list[i]); },
                 [&](int rank, int i) {
                     const unsigned long long o = list[i];
                     if (rank < a.picks)
-                        put(rank, __longlong_as_double(o & 0x8000000000000000ull ? o & 0x7fffffffffffffffull : ~o), flat_list[i]);
+                        put(rank, __longlong_as_double(o & 0x8000000000000000ull ? o & 0x7fffffffffffffffull : ~o),
+                            flat_list[i]);
                 });
     } else {
         for (int i = warp; i < total; i += kWarps) {

@@ -10,10 +10,10 @@
 //
 // The counting is whole-number arithmetic: atomics in any order give the same result.
 //
-// Bound: the copied pages' bytes, read and written; for a few beams, latency. Each is one cooperative launch whose phases
-// are separated by grid-wide barriers (four launches in a row took 23.9 us for a
-// fork of four beams, most of it on the host): fork counts references into a zeroed array, one CTA then gives out the free
-// pages (8192 a step), and all CTAs copy; compact plans on one CTA, then all copy and rewrite the tables.
+// Bound: the copied pages' bytes, read and written; for a few beams, latency. Each is one cooperative launch whose
+// phases are separated by grid-wide barriers (four launches in a row took 23.9 us for a fork of four beams, most of it
+// on the host): fork counts references into a zeroed array, one CTA then gives out the free pages (8192 a step), and
+// all CTAs copy; compact plans on one CTA, then all copy and rewrite the tables.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -31,10 +31,9 @@ constexpr int kNoChild = 0x7fffffff;
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// All CTAs of a cooperative launch meet. Bounded; after a wait that gave up the error word is set and the kernel goes on
-// (the arrays it reads are within bounds whatever they hold).
-// The last to arrive sets the arrivals back to 0 and lets the others go by a new number, so launches of any size follow
-// one another.
+// All CTAs of a cooperative launch meet. Bounded; after a wait that gave up the error word is set and the kernel goes
+// on (the arrays it reads are within bounds whatever they hold). The last to arrive sets the arrivals back to 0 and
+// lets the others go by a new number, so launches of any size follow one another.
 __device__ __forceinline__ void grid_barrier(int* barrier, int* err) {
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -226,7 +225,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
                     a.tables_out[(long long)m * a.stride + have + i] = id;
                     a.refs_out[id] = 1;
                 }
-                a.lens_out[m] = got < n ? int(min((long long)want_len, (long long)(have + got) * p.page_size)) : want_len;
+                a.lens_out[m] = got < n ? int(min((long long)want_len, (long long)(have +
+                    got) * p.page_size)) : want_len;
                 if (copy) w.moves[slot] = make_int2(src, w.free_page[at]);
             }
             used += total;
@@ -247,7 +247,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_compact_kernel(KvPages p, Comp
         int total;
         block_scan(live, sums, &total);
         live = total;
-        // holes below the live count and live pages from it on, both in ascending order: as many of the one as of the other
+        // holes below the live count and live pages from it on, both in ascending order: as many of the one as of the
+        // other
         int holes = 0, movers = 0;
         for (int i0 = 0; i0 < p.num_pages; i0 += kScan) {
             const int i = i0 + threadIdx.x * kPer;
@@ -336,7 +337,8 @@ void launch_kv_fork(const KvPages& p, const ForkArgs& a, const PageWs& w, cudaSt
     ForkArgs aa = a;
     PageWs ww = w;
     void* args[] = {&pp, &aa, &ww};
-    GPT_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kv_fork_kernel), dim3(grid), dim3(kThreads), args, 0, s));
+    GPT_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kv_fork_kernel), dim3(grid), dim3(kThreads),
+        args, 0, s));
 }
 
 void launch_kv_compact(const KvPages& p, const CompactArgs& a, const PageWs& w, cudaStream_t s) {
@@ -345,7 +347,8 @@ void launch_kv_compact(const KvPages& p, const CompactArgs& a, const PageWs& w, 
     CompactArgs aa = a;
     PageWs ww = w;
     void* args[] = {&pp, &aa, &ww};
-    GPT_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kv_compact_kernel), dim3(grid), dim3(kThreads), args, 0, s));
+    GPT_CHECK(cudaLaunchCooperativeKernel(reinterpret_cast<const void*>(kv_compact_kernel), dim3(grid),
+        dim3(kThreads), args, 0, s));
 }
 
 }  // namespace gpt

@@ -47,7 +47,8 @@ struct KvView {
     int layer, box_log;      // coordinates of KvMaps: the layer, 2^box_log slots per box (below 3: no maps)
 };
 
-// Tensor maps of a pool, [layer][page][slot][head][dim] in boxes of 2^box_log slots x 64 dims with the 128-byte swizzle.
+// Tensor maps of a pool, [layer][page][slot][head][dim] in boxes of 2^box_log slots x 64 dims with the 128-byte
+// swizzle.
 struct KvMaps {
     CUtensorMap k, v;
 };
@@ -83,8 +84,10 @@ struct PagedAttnArgs {
 constexpr size_t kCounterBytes = 2048;            // of both kernels, before the partial results
 size_t paged_attention_ws_bytes(int dim);
 size_t paged_tiles_ws_bytes(int dim);
-void launch_paged_tiles(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
-void launch_paged_attention(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s);
+void launch_paged_tiles(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
+    cudaStream_t s);
+void launch_paged_attention(const KvMaps& m, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
+    cudaStream_t s);
 
 struct BeamArgs {
     const void* logits;

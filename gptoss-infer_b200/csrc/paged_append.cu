@@ -4,8 +4,8 @@
 // (a cos - b sin, b cos + a sin) with the table's row p; pairs are (j, j + rot/2) or, interleaved, (2j, 2j + 1); the
 // dims from rot on pass through. All arithmetic is fp32; a value is rounded once, to the type it is stored in.
 //
-// Bound: bytes (each value read once and written once; nothing is reused but the token's cos/sin row, which the heads find
-// in L1). A work item is two runs of eight values of one head with whole pairs in them.
+// Bound: bytes (each value read once and written once; nothing is reused but the token's cos/sin row, which the heads
+// find in L1). A work item is two runs of eight values of one head with whole pairs in them.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -17,8 +17,8 @@ using namespace paged;
 
 constexpr int kThreads = 256;
 constexpr int kTokens = 8;       // tokens per CTA, at most: one warp looks up each
-// Items of a thread in flight: more of them cost more in resident threads than they bring (16383 bf16 tokens of 48 heads
-// of 128: 1 item 70 us, 2 75 us, 4 91 us).
+// Items of a thread in flight: more of them cost more in resident threads than they bring (16383 bf16 tokens of 48
+// heads of 128: 1 item 70 us, 2 75 us, 4 91 us).
 constexpr int kBatch = 1;
 
 struct Place {
@@ -31,17 +31,54 @@ __device__ __forceinline__ void turn(float& a, float& b, float cs, float sn) {
     a = p * cs - r * sn;
     b = r * cs + p * sn;
 }
-__device__ __forceinline__ void turn_pairs(float (&x)[8], const float* cs, const float* sn) {
-    const float4 c4 = __ldg(reinterpret_cast<const float4*>(cs)), s4 = __ldg(reinterpret_cast<const float4*>(sn));
-    turn(x[0], x[1], c4.x, s4.x);
-    turn(x[2], x[3], c4.y, s4.y);
-    turn(x[4], x[5], c4.z, s4.z);
-    turn(x[6], x[7], c4.w, s4.w);
+template <int RUN>
+__device__ __forceinline__ void turn_pairs(float (&x)[RUN], const float* cs, const float* sn) {
+    if constexpr (RUN == 8) {
+        const float4 c4 = __ldg(reinterpret_cast<const float4*>(cs)), s4 = __ldg(reinterpret_cast<const float4*>(sn));
+        turn(x[0], x[1], c4.x, s4.x);
+        turn(x[2], x[3], c4.y, s4.y);
+        turn(x[4], x[5], c4.z, s4.z);
+        turn(x[6], x[7], c4.w, s4.w);
+    }
 }
 
-// VEC: every run of eight values is 16-byte aligned in memory and pairs do not straddle a run.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b, AppendArgs a, int per_cta, FastDiv per_token) {
+// RUN values of a run as loaded, unpacked and stored: 8 (16 bytes of 16-bit values) or 4.
+template <class T, int RUN, int Q>
+__device__ __forceinline__ void load_run(const T* p, uint4 (&raw)[Q]) {
+    if constexpr (RUN * sizeof(T) == 8) {
+        const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+        raw[0].x = x.x;
+        raw[0].y = x.y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < Q; ++e) raw[e] = __ldg(reinterpret_cast<const uint4*>(p) + e);
+    }
+}
+template <class T, int RUN, int Q>
+__device__ __forceinline__ void unpack_run(const uint4 (&raw)[Q], float (&x)[RUN]) {
+    if constexpr (RUN == 8) {
+        unpack8<T>(raw, x);
+    } else {
+        const uint4 both[2] = {raw[0], raw[0]};
+        float y[8];
+        if constexpr (sizeof(T) == 4) unpack8<T>(both, y);
+        else unpack8<T>(raw, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = y[i];
+    }
+}
+template <int RUN>
+__device__ __forceinline__ void store_run(char* p, const float (&x)[RUN], int type) {
+    if constexpr (RUN == 8) store8(p, x, type);
+    else if (type == kF32) *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack2(x[0], x[1], type == kF16), pack2(x[2], x[3], type == kF16));
+}
+
+// RUN 8 or 4: runs of so many values are aligned to their loads and pairs lie in one run or in the two of an item (4: a
+// rotated half that is a multiple of 4 only); RUN 1: one pair at a time.
+template <class T, int RUN>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b, AppendArgs a, int per_cta,
+    FastDiv per_token) {
     __shared__ Place place[kTokens];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int t0 = blockIdx.x * per_cta, nt = min(per_cta, b.tokens - t0);
@@ -71,22 +108,22 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b
         }
     }
     __syncthreads();
-    const int per_head = VEC ? c.dim / 16 : c.dim / 2, heads = a.q_heads + 2 * c.kv_heads;
+    const int per_head = RUN > 1 ? c.dim / (2 * RUN) : c.dim / 2, heads = a.q_heads + 2 * c.kv_heads;
     const int half = a.rot / 2, q_bytes = a.q_type == kF32 ? 4 : 2;
     const int items = heads * per_head;
-    if constexpr (VEC) {
-        constexpr int Q = sizeof(T) == 4 ? 2 : 1;     // 16-byte loads of eight values
-        // First dims of an item's two runs: the halves of the rotated dims in the half layout, and of what passes behind
-        // them; the halves of the head otherwise. Neighbouring threads take neighbouring runs.
+    if constexpr (RUN > 1) {
+        constexpr int Q = RUN * sizeof(T) > 16 ? 2 : 1;   // loads of a run
+        // First dims of an item's two runs: the halves of the rotated dims in the half layout, and of what passes
+        // behind them; the halves of the head otherwise. Neighbouring threads take neighbouring runs.
         const auto runs_of = [&](int j, bool is_v, int& d0, int& d1) {
             if (is_v || a.interleaved) {
-                d0 = j * 8;
-                d1 = c.dim / 2 + j * 8;
-            } else if (j * 16 < a.rot) {
-                d0 = j * 8;
-                d1 = half + j * 8;
+                d0 = j * RUN;
+                d1 = c.dim / 2 + j * RUN;
+            } else if (j * 2 * RUN < a.rot) {
+                d0 = j * RUN;
+                d1 = half + j * RUN;
             } else {
-                d0 = a.rot + (j - a.rot / 16) * 8;
+                d0 = a.rot + (j - a.rot / (2 * RUN)) * RUN;
                 d1 = d0 + (c.dim - a.rot) / 2;
             }
         };
@@ -108,11 +145,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b
                                           (h - a.q_heads - (is_v ? c.kv_heads : 0)) * c.dim;
                 int d0, d1;
                 runs_of(j, is_v, d0, d1);
-#pragma unroll
-                for (int e = 0; e < Q; ++e) {
-                    raw[n][0][e] = __ldg(reinterpret_cast<const uint4*>(src + d0) + e);
-                    raw[n][1][e] = __ldg(reinterpret_cast<const uint4*>(src + d1) + e);
-                }
+                load_run<T, RUN>(src + d0, raw[n][0]);
+                load_run<T, RUN>(src + d1, raw[n][1]);
                 what[n] = u << 16 | h;
             }
 #pragma unroll
@@ -123,18 +157,18 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b
                 const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + c.kv_heads;
                 int d0, d1;
                 runs_of(j, is_v, d0, d1);
-                float x[8], y[8];
-                unpack8<T>(raw[n][0], x);
-                unpack8<T>(raw[n][1], y);
+                float x[RUN], y[RUN];
+                unpack_run<T, RUN>(raw[n][0], x);
+                unpack_run<T, RUN>(raw[n][1], y);
                 const long long tab = (long long)w.pos * half;
-                if (!is_v && a.interleaved) {         // each run: four pairs of its own
-                    if (d0 < a.rot) turn_pairs(x, a.cos_t + tab + d0 / 2, a.sin_t + tab + d0 / 2);
-                    if (d1 < a.rot) turn_pairs(y, a.cos_t + tab + d1 / 2, a.sin_t + tab + d1 / 2);
-                } else if (!is_v && j * 16 < a.rot) { // eight pairs across the runs
+                if (RUN == 8 && !is_v && a.interleaved) {   // each run: four pairs of its own
+                    if (d0 < a.rot) turn_pairs<RUN>(x, a.cos_t + tab + d0 / 2, a.sin_t + tab + d0 / 2);
+                    if (d1 < a.rot) turn_pairs<RUN>(y, a.cos_t + tab + d1 / 2, a.sin_t + tab + d1 / 2);
+                } else if (!is_v && j * 2 * RUN < a.rot) {  // RUN pairs across the runs
                     const float4* ct = reinterpret_cast<const float4*>(a.cos_t + tab + d0);
                     const float4* st = reinterpret_cast<const float4*>(a.sin_t + tab + d0);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
+                    for (int e = 0; e < RUN / 4; ++e) {
                         const float4 c4 = __ldg(ct + e), s4 = __ldg(st + e);
                         turn(x[4 * e], y[4 * e], c4.x, s4.x);
                         turn(x[4 * e + 1], y[4 * e + 1], c4.y, s4.y);
@@ -144,12 +178,12 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b
                 }
                 if (is_q) {
                     char* qo = static_cast<char*>(a.q_out) + ((t0 + u) * (long long)a.q_heads + h) * c.dim * q_bytes;
-                    store8(qo + d0 * q_bytes, x, a.q_type);
-                    store8(qo + d1 * q_bytes, y, a.q_type);
+                    store_run<RUN>(qo + d0 * q_bytes, x, a.q_type);
+                    store_run<RUN>(qo + d1 * q_bytes, y, a.q_type);
                 } else if (w.k) {
                     char* dst = (is_v ? w.v : w.k) + (h - a.q_heads - (is_v ? c.kv_heads : 0)) * c.head_stride;
-                    store8(dst + d0 * 2, x, a.kv_type);
-                    store8(dst + d1 * 2, y, a.kv_type);
+                    store_run<RUN>(dst + d0 * 2, x, a.kv_type);
+                    store_run<RUN>(dst + d1 * 2, y, a.kv_type);
                 }
             }
         }
@@ -197,13 +231,17 @@ template <class T>
 void launch(const KvView& c, const KvBatch& b, const AppendArgs& a, cudaStream_t s) {
     const auto al = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
     const int run = 16 / int(sizeof(T));
-    const bool vec = al(a.q) && al(a.k) && al(a.v) && al(a.q_out) && a.q_stride % run == 0 && a.kv_stride % run == 0 &&
-                     a.rot % 16 == 0 && al(a.cos_t) && al(a.sin_t);
+    const bool even = al(a.q) && al(a.k) && al(a.v) && al(a.q_out) && al(a.cos_t) && al(a.sin_t) && a.rot % 8 == 0 &&
+        a.q_stride % run == 0 && a.kv_stride % run == 0;
     const int per = b.tokens >= 148 * 8 * kTokens ? kTokens : 1;
-    const int grid = (b.tokens + per - 1) / per;
-    const FastDiv div = FastDiv::of(uint32_t((a.q_heads + 2 * c.kv_heads) * (c.dim / 16)));
-    if (vec) kv_append_kernel<T, true><<<grid, kThreads, 0, s>>>(c, b, a, per, div);
-    else kv_append_kernel<T, false><<<grid, kThreads, 0, s>>>(c, b, a, per, div);
+    const int grid = (b.tokens + per - 1) / per, heads = a.q_heads + 2 * c.kv_heads;
+    const auto div = [&](int n) { return FastDiv::of(uint32_t(heads * (c.dim / n))); };
+    if (even && (a.interleaved || a.rot % 16 == 0))
+        kv_append_kernel<T, 8><<<grid, kThreads, 0, s>>>(c, b, a, per, div(16));
+    else if (even)
+        kv_append_kernel<T, 4><<<grid, kThreads, 0, s>>>(c, b, a, per, div(8));
+    else
+        kv_append_kernel<T, 1><<<grid, kThreads, 0, s>>>(c, b, a, per, div(2));
     check_launch("kv_append");
 }
 

@@ -1,7 +1,7 @@
 // Attention of new tokens over the paged cache: few rows per key/value head (decode).
 //
-// out = sum_j w_j v_j / (sum_j w_j [+ exp(sink)]), w_j = exp(scale q.k_j) over the positions max(0, p - window + 1) .. p
-// of the token at p; one pass with a running maximum and sum (base 2, fp32).
+// out = sum_j w_j v_j / (sum_j w_j [+ exp(sink)]), w_j = exp(scale q.k_j) over the positions max(0, p - window + 1) ..
+// p of the token at p; one pass with a running maximum and sum (base 2, fp32).
 //
 // Bound: the keys' and values' bytes, read once. A CTA is four warps that never wait for one another inside an item:
 // each warp owns every fourth group of keys, copies it into its own ring of shared memory (16-byte asynchronous copies,
@@ -15,9 +15,10 @@
 // score passes it by 2^8: weights are at most 256, which both 16-bit types and the fp32 sums hold without loss, and
 // most groups need no exchange between lanes at all.
 //
-// Measured: 64 sequences of 4K to 8K positions, one token each, 64 query heads over 8 of 64, bf16: 149 us, 5.5 TB/s (0.84
-// of the measured copy) with slot-major pages, whose rows of one head are 1 KB apart, 135 us, 6.1 TB/s with head-major
-// ones; 32 heads over 4 of 128: 130 us, 6.3 TB/s. With rows along the instructions' long side, 16 keys at a time, 203 us.
+// Measured: 64 sequences of 4K to 8K positions, one token each, 64 query heads over 8 of 64, bf16: 149 us, 5.5 TB/s
+// (0.84 of the measured copy) with slot-major pages, whose rows of one head are 1 KB apart, 135 us, 6.1 TB/s with
+// head-major ones; 32 heads over 4 of 128: 130 us, 6.3 TB/s. With rows along the instructions' long side, 16 keys at a
+// time, 203 us.
 //
 // fp32 queries: a row is scaled by a power of two into [2^10, 2^11) and split into two fp16 parts (22 bits, exact
 // products with fp16 keys); the weights are split the same way for the second product.
@@ -142,7 +143,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const Schedule<R, kGroup> sch{c, b, a.window, group, 1, a.rows_from, a.rows_to};
-    const Span sp = find_span<kThreads>(sch, kWarps * (NS - 1), scratch);
+    const Span sp = find_span<kThreads>(sch, kWarps, scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
 
@@ -299,7 +300,8 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
 #pragma unroll
                 for (int x = 0; x < KT; ++x)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) ldsm4(kt + tile_off<D>(x * 16 + lane % 16, 2 * (k + y) + lane / 16), ka[x][y]);
+                    for (int y = 0; y < 2; ++y) ldsm4(kt + tile_off<D>(x * 16 + lane % 16, 2 * (k + y) + lane / 16),
+                        ka[x][y]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     uint32_t q[4];
@@ -587,10 +589,10 @@ void by_shape(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* w
     }
 }
 
-// Query rows per key/value head up to which the kernel of this file takes a sequence. Both sides, 64 sequences of 4K to 8K
-// positions / 2 of them, 64 query heads over 8: 64 rows of heads of 64 (as two tiles of 32) 296 / 28 us here, 285 / 42 us on
-// the 128-row tiles; 32 rows 170 / 24 us here, 254 / 43 us there. Heads of 128 (32 over 4): 32 rows 283 us here, 259 us there,
-// 64 rows 492 us and 211 us.
+// Query rows per key/value head up to which the kernel of this file takes a sequence. Both sides, 64 sequences of 4K to
+// 8K positions / 2 of them, 64 query heads over 8: 64 rows of heads of 64 (as two tiles of 32) 296 / 28 us here, 285 /
+// 42 us on the 128-row tiles; 32 rows 170 / 24 us here, 254 / 43 us there. Heads of 128 (32 over 4): 32 rows 283 us
+// here, 259 us there, 64 rows 492 us and 211 us.
 int few_rows_of(int dim) { return dim == 64 ? 64 : 16; }
 
 void few_rows(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
@@ -605,12 +607,13 @@ size_t paged_attention_ws_bytes(int dim) {
     return std::max(kCounterBytes + kMaxCtas * 2 * sizeof(float) * kSlotFloats, paged_tiles_ws_bytes(dim));
 }
 
-void launch_paged_attention(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
+void launch_paged_attention(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
+    cudaStream_t s) {
     const long long most = (long long)b.max_new * (a.q_heads / c.kv_heads);
     const int few_at_most = few_rows_of(c.dim);
     if (most <= few_at_most) return few_rows(c, b, a, ws, s);
-    // Chunks go to the tensor-core tiles. Where sequences differ in length (the batch's tokens say so), those of few rows,
-    // decoding beside a chunk, are left out of that launch and take one of their own.
+    // Chunks go to the tensor-core tiles. Where sequences differ in length (the batch's tokens say so), those of few
+    // rows, decoding beside a chunk, are left out of that launch and take one of their own.
     const bool mixed = b.tokens < (long long)b.seqs * b.max_new && b.seqs > 1;
     PagedAttnArgs part = a;
     if (mixed) part.rows_from = few_at_most + 1;

@@ -6,20 +6,21 @@
 //   P = exp2(S - m)      one thread per row, no exchange between threads
 //   O += P V             A operand P read from TMEM, V in shared memory as stored (rows = keys)
 // S is taken in tiles of 64 keys (128 for 16-bit heads of 64, whose P has columns of its own), read into registers and
-// released at once, so the next scores are made while this tile's exponentials run; the products are issued in the order
-// in which two halves half a step apart need them.
+// released at once, so the next scores are made while this tile's exponentials run; the products are issued in the
+// order in which two halves half a step apart need them.
 //
 // Bound: the exponentials: 16 a clock and SM, 2048 cycles for 256 rows x 128 keys, against 1024 (heads of 64) and 2560
 // (heads of 128) of products. Measured, 2048 new tokens over 16384 positions, 64 query heads over 8, bf16: heads of 64
-// 668 us, 771 TFLOP/s, 46 % of the measured matrix rate: about 3100 cycles a step. Two warps of rows per scheduler do not
-// keep the special-function unit busy alone (a warp's 128 exponentials take about 1800 cycles by themselves), and waits
-// for products (about 600 cycles from weights written to their product seen) fall between. 32 heads of 128 over 4: 500 us,
-// 1031 TFLOP/s. Tried: reading the scores twice instead of holding them (1110 us), halves taking strict turns at the
-// exponentials (974 us), polling for whatever product is ready (735 us), 3 and 4 of 8 exponentials on the fp32 pipes.
+// 668 us, 771 TFLOP/s, 46 % of the measured matrix rate: about 3100 cycles a step. Two warps of rows per scheduler do
+// not keep the special-function unit busy alone (a warp's 128 exponentials take about 1800 cycles by themselves), and
+// waits for products (about 600 cycles from weights written to their product seen) fall between. 32 heads of 128 over
+// 4: 500 us, 1031 TFLOP/s. Tried: reading the scores twice instead of holding them (1110 us), halves taking strict
+// turns at the exponentials (974 us), polling for whatever product is ready (735 us), 3 and 4 of 8 exponentials on the
+// fp32 pipes.
 //
-// Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output); the next two copy keys and values through a
-// ring of tiles with TMA (a box per run of slots in a page; page sizes that are multiples of 8), or the next four with
-// 16-byte asynchronous copies (any page size); one more issues the products. The running maximum moves only when
+// Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output); the next two copy keys and values through
+// a ring of tiles with TMA (a box per run of slots in a page; page sizes that are multiples of 8), or the next four
+// with 16-byte asynchronous copies (any page size); one more issues the products. The running maximum moves only when
 // it grows by more than 2^8, so the accumulator in TMEM is rescaled rarely (weights stay at most 256).
 //
 // fp32 queries: two fp16 parts of a row scaled by a power of two, and two of the weights, as in paged_attention.cu.
@@ -39,8 +40,8 @@ constexpr int kRows = 256, kHalf = 128, kTile = 128;
 // Threads that bring in keys, values and queries: two warps with TMA, four without; one warp more issues the products.
 constexpr int copy_threads(bool tma) { return tma ? 64 : 128; }
 constexpr int block_threads(bool tma) { return tma ? 384 : 512; }
-// Of 8 pairs of exponentials, those computed on the fp32 pipes beside the special-function unit (2048 tokens over 16384,
-// heads of 64, bf16: 0 of 8 747 us, 2 748, 3 790; heads of 128: 551, 540, 546).
+// Of 8 pairs of exponentials, those computed on the fp32 pipes beside the special-function unit (2048 tokens over
+// 16384, heads of 64, bf16: 0 of 8 747 us, 2 748, 3 790; heads of 128: 551, 540, 546).
 constexpr int kMixed = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -220,7 +221,8 @@ __device__ __forceinline__ float weights(const uint32_t (&x)[N], float sc, float
 }
 
 // Shared-memory image of 128 rows of D 16-bit values: halves of 64 columns, each in the 128-byte swizzled layout. As a
-// K-major operand the rows are M or N; as V the rows are K (8-row groups 1024 bytes apart, 64-column halves 16 KB apart).
+// K-major operand the rows are M or N; as V the rows are K (8-row groups 1024 bytes apart, 64-column halves 16 KB
+// apart).
 template <int D>
 __device__ __forceinline__ uint32_t image_off(int r, int chunk) {
     return uint32_t((chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
@@ -241,11 +243,13 @@ __host__ __device__ constexpr int slot_floats() {
     return kRows * D + 2 * kRows;                                        // sums [dim][row], maxima, sums of weights
 }
 
-enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kSFree = 18, kPFull = 20, kPvDone = 22, kQFull = 24, kQFree = 25, kDrain = 26, kEdge = 27, kBars = 28 };
+enum Bars { kTileFull = 0, kFree = 8, kSFull = 16, kSFree = 18, kPFull = 20, kPvDone = 22, kQFull = 24, kQFree = 25,
+    kDrain = 26, kEdge = 27, kBars = 28 };
 
 template <class T, class C, int D, bool TMA>
 __global__ void __launch_bounds__(block_threads(TMA), 1)
-paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* counters,
+paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, PagedAttnArgs a, FastDiv group,
+    int* counters,
                    float* slots) {
     using L = Layout<T, D, TMA>;
     constexpr int kThreads = block_threads(TMA), kCopy = copy_threads(TMA);
@@ -264,7 +268,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
     const int warp = int(threadIdx.x / 32), lane = threadIdx.x % 32;
     int* err = c.err;
     const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1, a.rows_from, a.rows_to};
-    const Span sp = find_span<kThreads>(sch, 2, scratch);
+    const Span sp = find_span<kThreads>(sch, 4, scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
 
@@ -312,9 +316,11 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 const int r0 = it.t * kRows;
                 const auto query = [&](int r) {       // row r's query
                     const int tok = int(group.div(r0 + r));
-                    return static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride + (it.h * G + (r0 + r - tok * G)) * D;
+                    return static_cast<const T*>(a.q) + (long long)(it.s.row0 + tok) * a.q_stride + (it.h * G + (r0 +
+                        r - tok * G)) * D;
                 };
-                const auto q_off = [&](int r, int ch) { return (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf, ch); };
+                const auto q_off = [&](int r, int ch) { return (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf,
+                    ch); };
                 if constexpr (L::kSplit) {
 #pragma unroll 4
                     for (int r = warp - 8; r < kRows; r += kCopy / 32) {
@@ -336,7 +342,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                             const float y = x[e] * by;
                             const __half hi = __float2half_rn(y);
                             const int d = lane * (D / 32) + e;
-                            char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) + d % 8 * 2;
+                            char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) +
+                                d % 8 * 2;
                             *reinterpret_cast<__half*>(p) = hi;
                             *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
                         }
@@ -365,22 +372,26 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 tc::fence_proxy_async_smem();
                 arrive_warp(&bars[kQFull]);
         };
-        // Bits 15 and 31 of the result: one of the eight values is NaN or infinite (an exponent of all ones, which one more
-        // carries into the sign's place). Values that some row must not see are checked: a product would carry them there.
+        // Bits 15 and 31 of the result: one of the eight values is NaN or infinite (an exponent of all ones, which one
+        // more carries into the sign's place). Values that some row must not see are checked: a product would carry
+        // them there.
         const auto exponents = [](const uint4& x) {
             constexpr uint32_t one = kBf16 ? 0x00800080u : 0x04000400u, rest = 0x7fff7fffu;
             return ((x.x & rest) + one) | ((x.y & rest) + one) | ((x.z & rest) + one) | ((x.w & rest) + one);
         };
         const auto wait_free = [&] {                  // until the ring's next place is free
-            if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1, err, kKvWait));
+            if (issued >= NS) good = all_ok(good && tc::mbar_wait(&bars[kFree + issued % NS], (issued / NS - 1) & 1,
+                err, kKvWait));
         };
         if constexpr (TMA) {
-            // lane x of the first copying warp brings box x of a tile: 2^box_log slots of one page, one copy per 64 dims
+            // lane x of the first copying warp brings box x of a tile: 2^box_log slots of one page, one copy per 64
+            // dims
             const int box = 1 << c.box_log, boxes = kTile >> c.box_log;
             int id = -1, edges = 0;
             const auto look_up = [&](int k0) {
                 const int pos = k0 + lane * box;
-                id = lane < boxes && pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride + c.page.div(pos)) : -1;
+                id = lane < boxes && pos < it.hi ? __ldg(b.tables + (long long)it.b * b.table_stride +
+                    c.page.div(pos)) : -1;
             };
             const auto issue = [&](const CUtensorMap* map, int k0, int page, uint64_t* bar) {
                 // (the second warp must not wait here: nothing holds it within a phase of the first)
@@ -395,7 +406,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                         const int slot = pos - int(c.page.div(pos) * c.page.d);
 #pragma unroll
                         for (int h = 0; h < D / 64; ++h)
-                            tma_load_5d(ring0 + issued % NS * L::kTileBytes + h * (128 * 128) + lane * box * 128, map, h * 64,
+                            tma_load_5d(ring0 + issued % NS * L::kTileBytes + h * (128 * 128) + lane * box * 128, map,
+                                h * 64,
                                         it.h, slot, page, c.layer, tc::smem_u32(bar));
                     }
                     __syncwarp();
@@ -459,15 +471,16 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 uint32_t seen = 0;
                 for (int i = 0; i < kTile * CH / kCopy; ++i) {
                     const int r = i * (kCopy / CH) + tid / CH, ch = tid % CH;
-                    seen |= exponents(*reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r, ch)));
+                    seen |= exponents(*reinterpret_cast<const uint4*>(ring + slot * L::kTileBytes + image_off<D>(r,
+                        ch)));
                 }
                 if (seen & 0x80008000u) flags[(check - 1) & 7] = check;
             }
             arrive_warp(&bars[kTileFull + slot]);
             ++done;
         };
-        // thread k finds keys k and k + 64 of a tile: page ids are read a tile ahead, byte offsets shared through row_off
-        // (K and V lie at the same offsets); -1: no such key, filled with zeros
+        // thread k finds keys k and k + 64 of a tile: page ids are read a tile ahead, byte offsets shared through
+        // row_off (K and V lie at the same offsets); -1: no such key, filled with zeros
         int id[kTile / kCopy], pos0 = 0;
         const auto look_up = [&](int k0) {
             pos0 = k0 + tid;
@@ -593,7 +606,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                     for (int part = 0; part < (L::kSplit ? 2 : 1); ++part)
 #pragma unroll
                         for (int k = 0; k < SK / 16; ++k)
-                            mma_ts(o_col(t), p_col(t, part) + k * 8, desc_of(vt + k * 2048 / 16), id_pv, u > 0 || part + k > 0);
+                            mma_ts(o_col(t), p_col(t, part) + k * 8, desc_of(vt + k * 2048 / 16), id_pv, u > 0 ||
+                                part + k > 0);
                     tc::mma_commit(&bars[kPvDone + t]);
                     ++used[t];
                     if (t == int(two) && u % SUB == SUB - 1) tc::mma_commit(&bars[kFree + pos % NS]);
@@ -651,12 +665,14 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                     tc::tmem_ld_wait();
                     tc::tc_fence_before();
                     arrive_warp(&bars[kSFree + t]);       // the next scores may be written
-                    if (L::kSplit && g == g0 * SUB) sc *= __int_as_float((127 - row_exp[(piece & 1) * kRows + row]) << 23);
+                    if (L::kSplit && g == g0 * SUB) sc *= __int_as_float((127 - row_exp[(piece & 1) * kRows +
+                        row]) << 23);
                     if (edge) mask<SK>(x, first - k0, p - k0);
                     float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int i = 0; i < SK; i += 2)
-                        top4[i / 2 & 3] = fmaxf(fmaxf(top4[i / 2 & 3], __uint_as_float(x[i])), __uint_as_float(x[i + 1]));
+                        top4[i / 2 & 3] = fmaxf(fmaxf(top4[i / 2 & 3], __uint_as_float(x[i])), __uint_as_float(x[i +
+                            1]));
                     const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
                     const bool past = top > m + 8.f;
                     if (__any_sync(kFull, past)) {
@@ -715,12 +731,14 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 return z == 0.f ? 0.f : 1.f / z;
             };
             if (mine && good && flags[piece & 7] == piece + 1) {
-                // a value that some row must not see is NaN or infinite: the piece again, without products of masked values
+                // a value that some row must not see is NaN or infinite: the piece again, without products of masked
+                // values
                 const int klo = it.lo + g0 * kTile, khi = min(it.hi, it.lo + g1 * kTile);
                 for (int i = 0; i < 32; ++i) {
                     const int r = t * kHalf + (warp % 4) * 32 + i;
                     if (r >= it.rows) break;
-                    const int tk = int(group.div(r0 + r)), pp = it.s.len - it.s.n + tk, hd = it.h * G + (r0 + r - tk * G);
+                    const int tk = int(group.div(r0 + r)), pp = it.s.len - it.s.n + tk, hd = it.h * G + (r0 +
+                        r - tk * G);
                     float mm, ll, oo[D / 32];
                     careful_row<T, C, D>(c, b, a, it.b, it.h, (long long)(it.s.row0 + tk) * a.q_stride + hd * D,
                                          max(klo, a.window ? pp - a.window + 1 : 0), min(khi, pp + 1), &mm, &ll, oo);
@@ -729,7 +747,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                     const float inv = z == 0.f ? 0.f : 1.f / z;
                     for (int e = 0; e < D / 32; ++e) {
                         const int d = lane * (D / 32) + e;
-                        if (whole) store_as(a.out, (long long)(it.s.row0 + tk) * a.out_stride + hd * D + d, oo[e] * inv, a.type);
+                        if (whole) store_as(a.out, (long long)(it.s.row0 + tk) * a.out_stride + hd * D + d,
+                            oo[e] * inv, a.type);
                         else my[d * kRows + r] = oo[e];
                     }
                     if (!whole && lane == 0) {
@@ -779,7 +798,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 if (flags[8] && valid) {
                     float mm = -INFINITY, z = 0.f;
                     for (int i = c0; i <= c1; ++i)
-                        mm = fmaxf(mm, __ldcg(slots + (long long)(2 * i + (i == c0)) * slot_floats<D>() + kRows * D + row));
+                        mm = fmaxf(mm, __ldcg(slots + (long long)(2 * i + (i == c0)) * slot_floats<D>() + kRows * D +
+                            row));
                     const float base = mm == -INFINITY ? 0.f : mm;
                     for (int i = c0; i <= c1; ++i) {
                         const float* ps = slots + (long long)(2 * i + (i == c0)) * slot_floats<D>() + kRows * D;

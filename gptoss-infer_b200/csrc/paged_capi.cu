@@ -281,7 +281,8 @@ int gptoss_kv_fork(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tables
         require(seqs == 0 || children == 0 || (tables_out != tables && lens_out != lens),
                 "kv_fork: the children's tables and lengths need arrays of their own");
         check_device(p, "kv_fork");
-        gpt::ForkArgs a{refs, tables, lens, parents, extra, refs_out, tables_out, lens_out, seqs, children, table_stride};
+        gpt::ForkArgs a{refs, tables, lens, parents, extra, refs_out, tables_out, lens_out, seqs, children,
+            table_stride};
         gpt::launch_kv_fork(p->pages, a, page_ws(p, children, seqs), static_cast<cudaStream_t>(stream));
     });
 }

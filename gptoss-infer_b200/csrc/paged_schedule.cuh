@@ -57,8 +57,8 @@ struct Schedule {
         fill(it);
         return pad == 1 ? it.n : (it.n + pad - 1) / pad * pad;
     }
-    // Groups of one key/value head of each lane's sequence: a few tiles by the lane itself, more by the whole warp, a lane
-    // per tile (64 tiles by one lane took 4 us). All lanes call it.
+    // Groups of one key/value head of each lane's sequence: a few tiles by the lane itself, more by the whole warp, a
+    // lane per tile (64 tiles by one lane took 4 us). All lanes call it.
     __device__ __forceinline__ int head_groups(const Seq& s, int pad) const {
         const int lane = threadIdx.x % 32, nt = row_tiles(s.n);
         int sum = 0;
@@ -74,7 +74,8 @@ struct Schedule {
         }
         return sum;
     }
-    // The tile of the item's head that holds group `off` of it; off becomes the group within the tile. All lanes call it.
+    // The tile of the item's head that holds group `off` of it; off becomes the group within the tile. All lanes call
+    // it.
     __device__ __forceinline__ void find_tile(Item& it, int& off, int pad) const {
         const int lane = threadIdx.x % 32;
         for (int t0 = 0;; t0 += 32) {

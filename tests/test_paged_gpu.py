@@ -397,7 +397,8 @@ def rope_reference(x, cos, sin, rot, interleaved):
 
 @pytest.mark.parametrize("tin", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 @pytest.mark.parametrize("tq,tkv", PAIRS, ids=["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rot,interleaved", [(64, False), (64, True), (32, False), (16, True), (24, False), (2, True), (0, False)])
+@pytest.mark.parametrize("rot,interleaved", [(64, False), (64, True), (32, False), (16, True), (24, False), (2, True), (0, False),
+                                             (24, True), (8, False), (40, True), (20, False), (56, False)])
 def test_append(lib, tin, tq, tkv, rot, interleaved):
     run_append(lib, [1, 0, 9, 3], [70, 5, 9, 33], 16, 2, 64, 8, tin, tq, tkv, rot, interleaved)
 
