@@ -322,32 +322,45 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                 const auto q_off = [&](int r, int ch) { return (r / kHalf) * L::kTileBytes + image_off<D>(r % kHalf,
                     ch); };
                 if constexpr (L::kSplit) {
-#pragma unroll 4
-                    for (int r = warp - 8; r < kRows; r += kCopy / 32) {
-                        float x[D / 32], top = 0.f;
-                        const float* src = reinterpret_cast<const float*>(query(r < it.rows ? r : 0)) + lane * (D / 32);
+                    // eight lanes a row, 8 values of each 16-byte chunk to a lane
+                    constexpr int N = CH / 8;         // chunks of a lane
+#pragma unroll 2
+                    for (int r0w = (warp - 8) * 4; r0w < kRows; r0w += kCopy / 8) {
+                        const int r = r0w + lane / 8;
+                        const float4* src = reinterpret_cast<const float4*>(query(r < it.rows ? r : 0));
+                        float4 x[N][2];
+                        float top = 0.f;
 #pragma unroll
-                        for (int e = 0; e < D / 32; ++e) {
-                            x[e] = r < it.rows ? src[e] : 0.f;
-                            top = fmaxf(top, fabsf(x[e]));
+                        for (int n = 0; n < N; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                x[n][e] = __ldg(src + (n * 8 + lane % 8) * 2 + e);
+                                if (r >= it.rows) x[n][e] = make_float4(0, 0, 0, 0);
+                                top = fmaxf(top, fmaxf(fmaxf(fabsf(x[n][e].x), fabsf(x[n][e].y)),
+                                                       fmaxf(fabsf(x[n][e].z), fabsf(x[n][e].w))));
+                            }
+#pragma unroll
+                        for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                        // 2^ex brings the largest value into [2^10, 2^11)
+                        const int ex = min(max(11 + 126 - int(__float_as_uint(top) >> 23), -126), 126);
+                        const float by = __int_as_float((127 + ex) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+#pragma unroll
+                        for (int n = 0; n < N; ++n) {
+                            const float y[8] = {x[n][0].x * by, x[n][0].y * by, x[n][0].z * by, x[n][0].w * by,
+                                                x[n][1].x * by, x[n][1].y * by, x[n][1].z * by, x[n][1].w * by};
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                hi[e] = pack2(y[2 * e], y[2 * e + 1], true);
+                                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+                                lo[e] = pack2(y[2 * e] - h.x, y[2 * e + 1] - h.y, true);
+                            }
+                            char* to = q_tile + (r / kHalf) * 2 * L::kTileBytes +
+                                image_off<D>(r % kHalf, n * 8 + lane % 8);
+                            *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4*>(to + L::kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                         }
-#pragma unroll
-                        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-                        int ex = 0;
-                        if (top > 0.f && top < INFINITY) frexpf(top, &ex);
-                        ex = min(max(11 - ex, -126), 126);
-                        const float by = ldexpf(a.scale < 0.f ? -1.f : 1.f, ex);
-#pragma unroll
-                        for (int e = 0; e < D / 32; ++e) {
-                            const float y = x[e] * by;
-                            const __half hi = __float2half_rn(y);
-                            const int d = lane * (D / 32) + e;
-                            char* p = q_tile + (r / kHalf) * 2 * L::kTileBytes + image_off<D>(r % kHalf, d / 8) +
-                                d % 8 * 2;
-                            *reinterpret_cast<__half*>(p) = hi;
-                            *reinterpret_cast<__half*>(p + L::kTileBytes) = __float2half_rn(y - __half2float(hi));
-                        }
-                        if (lane == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
+                        if (lane % 8 == 0) row_exp[(piece & 1) * kRows + r] = int8_t(ex);
                     }
                 } else {
                     if (a.scale < 0.f) {
