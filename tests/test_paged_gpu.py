@@ -308,6 +308,21 @@ def test_attention_chunks_of_many_pieces(lib, dim, page, window):
     assert s.pool.status() == 0
 
 
+@pytest.mark.parametrize("pair", PAIRS[:2], ids=["f32", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 20])
+def test_attention_chunks_by_type_and_page(lib, pair, dim, page):
+    """Pages that are and are not multiples of 8 slots, queries of very different sizes from row to row."""
+    s = Setup(lib, [150, 1, 333], [900, 300, 333], page=page, kvh=2, dim=dim, dtype=pair[1], seed=17)
+    q = new_q(s.T, 6, dim, F32)
+    q = (q * torch.logspace(-6, 0, s.T, device="cuda")[:, None, None]).to(pair[0])
+    q[::7] = 0
+    sinks = torch.randn(6, device="cuda")
+    out = run_attention(lib, s, q, sinks)
+    check_attention(out, *reference_attention(s, q, sinks, dim ** -0.5, 0))
+    assert s.pool.status() == 0
+
+
 def test_attention_on_another_stream_and_in_a_graph(lib):
     s = Setup(lib, [1, 1], [800, 333], page=16, kvh=8, dim=64, dtype=F16, seed=12)
     q = new_q(s.T, 64, 64, F32)
