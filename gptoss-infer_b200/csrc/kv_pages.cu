@@ -1,10 +1,11 @@
 // Pages of the paged cache: fork (reorder, share, grow and free sequences with reference counts) and compaction.
 //
 // fork:    refs' = refs - (references from the given tables) + (references from the children's tables). A child shares
-//          its parent's full pages. A part-filled last page stays with the parent's first child if nobody else holds it
-//          (its count was 1), and is copied into a fresh page for every other child, in all layers. Fresh pages are the
-//          lowest free ones (count 0 after the given tables' references and the children's shared ones are counted), in
-//          the order of the children.
+//          its parent's full pages. A part-filled last page to which no reference would be left (the given tables'
+//          dropped, the children's full pages counted) stays with the first child of the sequences that hold it; every
+//          other child gets a copy in a fresh page, in all layers. Fresh pages are the lowest free ones (count 0 after
+//          that), in the order of the children. So a page that is copied from always keeps a reference and is never a
+//          fresh page of the same call: the copies may run in any order.
 // compact: live pages (count > 0) at or past the number of live pages move into the free pages below it, both in
 //          ascending order, so sources and destinations never overlap.
 //
@@ -129,7 +130,7 @@ __device__ __forceinline__ void copy_pages(const KvPages& p, int n, const int2* 
 __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArgs a, PageWs w) {
     __shared__ int sums[kThreads / 32];
     const long long step = (long long)gridDim.x * kThreads, t0 = (long long)blockIdx.x * kThreads + threadIdx.x;
-    // --- references dropped and added (full pages), each sequence's first child
+    // --- references dropped and added (full pages), the first child of each part-filled last page
     for (long long i = t0, n = (long long)a.seqs * a.stride; i < n; i += step) {
         const int s = int(i / a.stride), j = int(i - (long long)s * a.stride);
         if (j >= pages_of(table_len(a.lens, s, a.stride, p.page_size, p.err), p.page_size)) continue;
@@ -146,21 +147,28 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
         }
         a.tables_out[i] = id;
     }
-    for (long long m = t0; m < a.children; m += step) {
+    for (long long m = step - 1 - t0; m < a.children; m += step) {      // by the threads that have no table entries
         const int par = a.parents[m];
-        if (par >= 0 && par < a.seqs) atomicMin(&w.first[par], int(m));
-        else if (par != -1) report(p.err, kKvBadParent);
+        if (par >= 0 && par < a.seqs) {
+            const int len = table_len(a.lens, par, a.stride, p.page_size, p.err);
+            if (len % p.page_size == 0) continue;
+            const int id = a.tables[(long long)par * a.stride + len / p.page_size];
+            if (unsigned(id) < unsigned(p.num_pages)) atomicMin(&w.first[id], int(m));
+        } else if (par != -1) {
+            report(p.err, kKvBadParent);
+        }
     }
     grid_barrier(w.barrier, p.err);
     if (blockIdx.x == 0) {
-        // --- the last pages that stay
+        // --- the last pages that stay (only a page's first child looks at its count here, and adds to it)
         for (int m = threadIdx.x; m < a.children; m += kThreads) {
             const int par = a.parents[m];
-            if (par < 0 || par >= a.seqs || __ldcg(&w.first[par]) != m) continue;
+            if (par < 0 || par >= a.seqs) continue;
             const int len = table_len(a.lens, par, a.stride, p.page_size, p.err), full = len / p.page_size;
             if (len % p.page_size == 0) continue;
             const int id = a.tables[(long long)par * a.stride + full];
-            if (unsigned(id) < unsigned(p.num_pages) && a.refs[id] == 1) {
+            if (unsigned(id) < unsigned(p.num_pages) && __ldcg(&w.first[id]) == m &&
+                a.refs[id] + __ldcg(&w.delta[id]) == 0) {
                 atomicAdd(&w.delta[id], 1);
                 a.tables_out[(long long)m * a.stride + full] = id;
             }
@@ -202,9 +210,13 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
                     have = len / p.page_size;
                     if (len % p.page_size) {
                         const int id = a.tables[(long long)par * a.stride + have];
-                        if (unsigned(id) >= unsigned(p.num_pages)) report(p.err, kKvBadPage);
-                        else if (__ldcg(&a.tables_out[(long long)m * a.stride + have]) >= 0) ++have;
-                        else src = id;
+                        if (unsigned(id) < unsigned(p.num_pages)) {
+                            w.first[id] = kNoChild;
+                            if (__ldcg(&a.tables_out[(long long)m * a.stride + have]) >= 0) ++have;
+                            else src = id;
+                        } else {
+                            report(p.err, kKvBadPage);
+                        }
                     }
                     const long long want = (long long)len + (a.extra ? max(a.extra[m], 0) : 0);
                     const long long cap = (long long)a.stride * p.page_size;
@@ -233,7 +245,6 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
             copies += total_copies;
         }
         if (threadIdx.x == 0) *w.count = copies;
-        for (int i = threadIdx.x; i < a.seqs; i += kThreads) w.first[i] = kNoChild;
     }
     grid_barrier(w.barrier, p.err);
     copy_pages(p, __ldcg(w.count), w.moves);
@@ -313,20 +324,20 @@ long long page_bytes(const KvPages& p) { return 2ll * p.layers * p.page_size * p
 
 }  // namespace
 
-size_t kv_pages_ws_bytes(int num_pages, int children, int seqs) {
-    return 256 + 2 * up256(size_t(num_pages) * 4) + up256(size_t(std::max(num_pages, children)) * 8) + size_t(seqs) * 4;
+size_t kv_pages_ws_bytes(int num_pages) {
+    return 256 + 3 * up256(size_t(num_pages) * 4) + size_t(num_pages) * 8;
 }
 
-PageWs make_kv_pages_ws(void* ws, int num_pages, int children, int seqs) {
+PageWs make_kv_pages_ws(void* ws, int num_pages) {
     char* p = static_cast<char*>(ws);
     PageWs w;
     w.barrier = reinterpret_cast<int*>(p);
     w.count = reinterpret_cast<int*>(p + 128);
     w.delta = reinterpret_cast<int*>(p += 256);
     w.free_page = reinterpret_cast<int*>(p += up256(size_t(num_pages) * 4));
-    w.moves = reinterpret_cast<int2*>(p += up256(size_t(num_pages) * 4));
-    w.first = reinterpret_cast<int*>(p + up256(size_t(std::max(num_pages, children)) * 8));
-    if (seqs > 0) init_first_kernel<<<(seqs + 255) / 256, 256>>>(w.first, seqs);
+    w.first = reinterpret_cast<int*>(p += up256(size_t(num_pages) * 4));
+    w.moves = reinterpret_cast<int2*>(p + up256(size_t(num_pages) * 4));
+    init_first_kernel<<<std::min(1024, (num_pages + 255) / 256), 256>>>(w.first, num_pages);
     check_launch("kv_pages workspace");
     return w;
 }

@@ -120,18 +120,18 @@ struct KvPages {
     int layers, num_pages, page_size, kv_heads, row_bytes;
     int* err;
 };
-// Workspace of both, for up to so many children and sequences of a call: zeroed memory, laid out and prepared once by
-// make_kv_pages_ws (on the legacy default stream). The kernels leave it as they found it.
+// Workspace of both: zeroed memory, laid out and prepared once by make_kv_pages_ws (on the legacy default stream). The
+// kernels leave it as they found it. Every move has a destination page of its own, so the pages bound the moves.
 struct PageWs {
     int* barrier;                  // arrivals, left at 0, and the number of the last barrier passed
     int* count;                    // [0] moves
     int* delta;                    // [num_pages] change of the counts; left at 0
     int* free_page;                // [num_pages]
-    int2* moves;                   // (source, destination)
-    int* first;                    // [seqs] first child of each sequence; left at the largest int
+    int* first;                    // [num_pages] first child whose part-filled last page it is; left at the largest int
+    int2* moves;                   // [num_pages] (source, destination)
 };
-size_t kv_pages_ws_bytes(int num_pages, int children, int seqs);
-PageWs make_kv_pages_ws(void* ws, int num_pages, int children, int seqs);
+size_t kv_pages_ws_bytes(int num_pages);
+PageWs make_kv_pages_ws(void* ws, int num_pages);
 void launch_kv_fork(const KvPages& p, const ForkArgs& a, const PageWs& w, cudaStream_t s);
 void launch_kv_compact(const KvPages& p, const CompactArgs& a, const PageWs& w, cudaStream_t s);
 

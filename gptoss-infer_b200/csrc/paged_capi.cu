@@ -25,9 +25,8 @@ struct gptoss_kv_pool {
     int type = 0, dim = 0, device = 0;
     int* err = nullptr;
     void* attn_ws = nullptr;
-    void* page_mem = nullptr;                 // of page_ws, made for so many children and sequences
+    void* page_mem = nullptr;                 // of page_ws
     gpt::PageWs page_ws{};
-    int page_children = 0, page_seqs = 0;
 
     gpt::KvView view(int layer) const {
         gpt::KvView v{};
@@ -115,25 +114,6 @@ struct ThreadWs {
 };
 thread_local ThreadWs g_beam_ws;
 
-// The pool's page workspace, made anew when a call needs more than it was made for.
-const gpt::PageWs& page_ws(gptoss_kv_pool* p, int children, int seqs) {
-    if (!p->page_mem || p->page_children < children || p->page_seqs < seqs) {
-        children = std::max(children, p->page_children);
-        seqs = std::max(seqs, p->page_seqs);
-        if (p->page_mem) GPT_CHECK(cudaFree(p->page_mem));
-        p->page_mem = nullptr;
-        p->page_children = p->page_seqs = 0;
-        const size_t n = gpt::kv_pages_ws_bytes(p->pages.num_pages, children, seqs);
-        GPT_CHECK(cudaMalloc(&p->page_mem, n));
-        GPT_CHECK(cudaMemset(p->page_mem, 0, n));
-        p->page_ws = gpt::make_kv_pages_ws(p->page_mem, p->pages.num_pages, children, seqs);
-        GPT_CHECK(cudaDeviceSynchronize());
-        p->page_children = children;
-        p->page_seqs = seqs;
-    }
-    return p->page_ws;
-}
-
 }  // namespace
 
 extern "C" {
@@ -175,8 +155,11 @@ gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, in
         const size_t n = gpt::paged_attention_ws_bytes(head_dim);
         GPT_CHECK(cudaMalloc(&p->attn_ws, n));
         GPT_CHECK(cudaMemset(p->attn_ws, 0, n));
+        const size_t pages_n = gpt::kv_pages_ws_bytes(num_pages);
+        GPT_CHECK(cudaMalloc(&p->page_mem, pages_n));
+        GPT_CHECK(cudaMemset(p->page_mem, 0, pages_n));
+        p->page_ws = gpt::make_kv_pages_ws(p->page_mem, num_pages);
         GPT_CHECK(cudaDeviceSynchronize());
-        page_ws(p.get(), 256, 256);
         made = p.release();
     });
     return rc == 0 ? made : nullptr;
@@ -283,7 +266,7 @@ int gptoss_kv_fork(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tables
         check_device(p, "kv_fork");
         gpt::ForkArgs a{refs, tables, lens, parents, extra, refs_out, tables_out, lens_out, seqs, children,
             table_stride};
-        gpt::launch_kv_fork(p->pages, a, page_ws(p, children, seqs), static_cast<cudaStream_t>(stream));
+        gpt::launch_kv_fork(p->pages, a, p->page_ws, static_cast<cudaStream_t>(stream));
     });
 }
 
@@ -297,7 +280,7 @@ int gptoss_kv_compact(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tab
         require(seqs == 0 || table_stride == 0 || (tables && lens && tables_out), "kv_compact: null tables or lengths");
         check_device(p, "kv_compact");
         gpt::CompactArgs a{refs, tables, lens, refs_out, tables_out, remap, live, seqs, table_stride};
-        gpt::launch_kv_compact(p->pages, a, page_ws(p, 0, 0), static_cast<cudaStream_t>(stream));
+        gpt::launch_kv_compact(p->pages, a, p->page_ws, static_cast<cudaStream_t>(stream));
     });
 }
 

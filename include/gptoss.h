@@ -272,7 +272,7 @@ int gptoss_set_prefill_packing(int mode);
  * slot-major and head-major pages are described without a copy. type: 1 = fp16, 2 = bf16. head_dim 64 or 128; any
  * page_size >= 1. A sequence's table is an int32 row of page ids: position p lives in page table[p / page_size], slot
  * p % page_size; entries past its last position are never read. The handle owns its workspaces (about 22 MB, 43 MB for
- * head_dim 128, and 16 bytes per page) and an error word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
+ * head_dim 128, and 20 bytes per page) and an error word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
  * current at its creation. Returns NULL on failure (gptoss_last_error). Synchronizes. */
 typedef struct gptoss_kv_pool gptoss_kv_pool;
 gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, int num_pages, int page_size,
@@ -326,12 +326,12 @@ int gptoss_paged_attention(gptoss_kv_pool* pool, int layer, const gptoss_kv_batc
  * parents[m] (-1: an empty child) of the given `seqs` and gets room for extra[m] more positions (extra NULL: none):
  * tables_out [children][table_stride] (unused entries -1), lens_out[m] = lens[parent] + extra[m]. refs and refs_out
  * (int32 [num_pages], may alias) count each page's references: those of the given sequences are dropped (a sequence
- * without a child is thereby freed), the children's added. Full pages are shared. A part-filled last page stays with
- * the parent's first child if its count was 1, and is copied to a fresh page for every other child, in all layers of
- * the pool. Fresh pages are the lowest-numbered ones left with count 0, in the order of the children; if they run out,
- * the children concerned get the length that their pages hold and the pool's status is 304. The pool makes its
- * workspace anew when a call has more sequences or children than any before (256 at first): make such a call before a
- * stream capture. A cooperative launch. */
+ * without a child is thereby freed), the children's added. Full pages are shared. A part-filled last page that would be
+ * left without a reference (nobody but the given sequences holds it, and no child as a full page) stays with the first
+ * child of those sequences; for every other child it is copied to a fresh page, in all layers of the pool. Fresh pages
+ * are the lowest-numbered ones left with count 0, in the order of the children (never one that is copied from); if they
+ * run out, the children concerned get the length that their pages hold and the pool's status is 304. A cooperative
+ * launch. */
 int gptoss_kv_fork(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* tables, const int32_t* lens, int seqs,
                    const int32_t* parents, const int32_t* extra, int children, int table_stride, int32_t* refs_out,
                    int32_t* tables_out, int32_t* lens_out, void* stream);
