@@ -12,8 +12,7 @@
 // Products are transposed, so that keys (16 at a time) and not the few rows fill the m16n8k16 instructions' long side:
 // S^T [keys x rows] = K Q^T, O^T [dims x rows] += V^T P^T; P^T is S^T's own fragment with its 8 x 8 blocks turned by
 // movmatrix. The running maximum is a reference that all lanes share and that moves (with a rescaling of O) only when a
-// score passes it by 2^8: weights are at most 256, which both 16-bit types and the fp32 sums hold without loss, and
-// most groups need no exchange between lanes at all.
+// weight would pass what its type is used for (Weights in paged.cuh): most groups need no exchange between lanes at all.
 //
 // Measured: 64 sequences of 4K to 8K positions, one token each, 64 query heads over 8 of 64, bf16: 149 us, 5.5 TB/s
 // (0.84 of the measured copy) with slot-major pages, whose rows of one head are 1 KB apart, 135 us, 6.1 TB/s with
@@ -130,6 +129,7 @@ template <class T, class C, int D, int NT>
 __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kPerSm)
 paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* counters, float* slots) {
     using S = Shape<T, D, NT>;
+    using W = Weights<C>;
     constexpr int R = S::R, NS = S::kStages, CH = D / 8, kGroup = S::kKeys, KT = kGroup / 16, PITCH = S::kPitch;
     extern __shared__ __align__(128) char smem[];
     char* ring = smem;
@@ -353,14 +353,14 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
                     top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
                     for (int x = 1; x < KT; ++x) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[x][nt][e], s[x][nt][2 + e]));
-                    past |= top[nt][e] > m[nt][e] + 8.f;
+                    past |= top[nt][e] > m[nt][e] + (W::kLift + W::kSlack);
                 }
-            if (__any_sync(kFull, past)) {            // move the reference: the rows' true maxima so far
+            if (__any_sync(kFull, past)) {            // move the references: kLift below the rows' maxima so far
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mm = fmaxf(m[nt][e], top[nt][e]);
+                        float mm = fmaxf(m[nt][e], top[nt][e] - W::kLift);
 #pragma unroll
                         for (int z = 4; z < 32; z <<= 1) mm = fmaxf(mm, __shfl_xor_sync(kFull, mm, z));
                         const float f = ex2(m[nt][e] - (mm == -INFINITY ? 0.f : mm));

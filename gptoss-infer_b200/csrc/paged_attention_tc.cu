@@ -20,8 +20,8 @@
 //
 // Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output); the next two copy keys and values through
 // a ring of tiles with TMA (a box per run of slots in a page; page sizes that are multiples of 8), or the next four
-// with 16-byte asynchronous copies (any page size); one more issues the products. The running maximum moves only when
-// it grows by more than 2^8, so the accumulator in TMEM is rescaled rarely (weights stay at most 256).
+// with 16-byte asynchronous copies (any page size); one more issues the products. The weights' reference moves only
+// when the maximum has grown past kSlack (Weights in paged.cuh), so the accumulator in TMEM is rescaled rarely.
 //
 // fp32 queries: two fp16 parts of a row scaled by a power of two, and two of the weights, as in paged_attention.cu.
 // (2048 over 16384, heads of 64: 1.11 ms, 465 TFLOP/s of the sum's own operations, twice that in products.)
@@ -253,6 +253,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
     int* counters,
                    float* slots) {
     using L = Layout<T, D, TMA>;
+    using W = Weights<C>;
     constexpr int kThreads = block_threads(TMA), kCopy = copy_threads(TMA);
     constexpr int NS = L::kSlots, CH = D / 8, SK = L::kScores, SUB = kTile / SK;
     constexpr bool kBf16 = std::is_same<C, __nv_bfloat16>::value;
@@ -688,9 +689,9 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                         top4[i / 2 & 3] = fmaxf(fmaxf(top4[i / 2 & 3], __uint_as_float(x[i])), __uint_as_float(x[i +
                             1]));
                     const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
-                    const bool past = top > m + 8.f;
+                    const bool past = top > m + (W::kLift + W::kSlack);
                     if (__any_sync(kFull, past)) {
-                        const float mm = past ? top : m, f = past ? ex2(m - mm) : 1.f;
+                        const float mm = past ? top - W::kLift : m, f = past ? ex2(m - mm) : 1.f;
                         if (g > g0 * SUB) {
                             good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
                             if (!good) break;

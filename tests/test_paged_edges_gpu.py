@@ -4,9 +4,52 @@ import numpy as np
 import pytest
 import torch
 
-from test_paged_gpu import F16, Pool, lib, make_pages, run_fork  # noqa: F401
+from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, lib, make_pages, new_q, reference_attention,  # noqa: F401
+                            run_attention, run_fork)
 
 pytestmark = pytest.mark.gpu
+
+
+# --------------------------------------------------------------------------------------------------------- attention
+def set_kv(s, b, at, keys=None, values=None):
+    """Writes keys and values [n, heads, dim] of positions `at` of sequence b."""
+    at = torch.as_tensor(at)
+    where = torch.tensor(s.tables[b], dtype=torch.long)[at // s.page].cuda(), (at % s.page).cuda()
+    for x, store, mine in ((keys, s.pool.k, s.keys[b]), (values, s.pool.v, s.values[b])):
+        if x is not None:
+            mine[at.cuda()] = x.to(mine.dtype)
+            store[0][where] = x.to(mine.dtype)
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("new,length,dim,page", [(1, 16384, 64, 16), (1, 131072, 64, 16), (1, 9000, 128, 16),
+                                                 (150, 16384, 64, 16), (150, 9000, 128, 20), (40, 131072, 64, 64)])
+@pytest.mark.parametrize("rest,spread", [(0.065, 0.3), (1.1e-3, 0.3), (1.1e-3, 0.0)])
+def test_attention_beside_a_dominant_key(lib, new, length, dim, page, pair, rest, spread):
+    """The first key takes nearly all the weight and has no value (the sink of a long context): the others, `rest` of
+    the weight together, make the whole result.
+
+    Bound: as in test_paged_gpu.py (A = sum w |v| / sum w, here about `rest`), and for weights stored as fp16 2^-38 of
+    the row's largest weight for each key: fp16 ends at 2^-24, half of that is lost at most, and the largest weight is
+    stored as 2^13 or more."""
+    s = Setup(lib, [new], [length], page=page, kvh=1, dim=dim, dtype=pair[1], seed=30)
+    g = torch.Generator(device="cuda").manual_seed(31)
+    sign = torch.where(torch.rand(dim, device="cuda", generator=g) < 0.5, -1.0, 1.0)
+    keys = spread * torch.randn(length, 1, dim, device="cuda", generator=g)
+    values = torch.randn(length, 1, dim, device="cuda", generator=g) + 0.5
+    scale = dim ** -0.5
+    keys[0, 0] = sign * (np.log(length / rest) / (dim * scale))
+    values[0] = 0
+    set_kv(s, 0, np.arange(length), keys, values)
+    q = (sign + 0.05 * torch.randn(new, 8, dim, device="cuda", generator=g)).to(pair[0])
+    out = run_attention(lib, s, q)
+    want, mag = reference_attention(s, q, None, scale, 0)
+    u = U[pair[0]]
+    bound = u * want.abs() + (u + 1e-5) * mag + (2.0 ** -25 if pair[0] == F16 else 1e-30)
+    if pair[1] == F16:
+        bound = bound + 2.0 ** -38 * s.values[0].double().abs().sum(0)
+    worst = ((out.double() - want).abs() / bound).max().item()
+    assert worst <= 1.0, worst
 
 
 # --------------------------------------------------------------------------------------------------------- pages
