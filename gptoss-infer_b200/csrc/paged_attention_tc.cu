@@ -155,9 +155,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     return r;
 }
 
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max3_nan(float x, float y, float z) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+
 // 2^x of two values on the fp32 pipes: x = n + f with n = round(x), |f| <= 1/2 (the sum with 1.5 * 2^23 leaves n in the
 // low mantissa bits), 2^f by the polynomial of least largest relative error on [-1/2, 1/2] (weighted least squares
-// iterated to equal ripple; degree 3: 7.5e-5, degree 4: 2.6e-6), n added to its exponent. x below -126 counts as -126.
+// iterated to equal ripple; degree 3: 7.5e-5, degree 4: 2.6e-6), n added to its exponent. x below -126 counts as -126, and so does NaN: not for scores that are not finite.
 template <int DEGREE>
 __device__ __forceinline__ void exp2_pair(uint64_t x2, float& u, float& v) {
     const auto both = [](float c) { return pair(__float_as_uint(c), __float_as_uint(c)); };
@@ -686,9 +693,8 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                     float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int i = 0; i < SK; i += 2)
-                        top4[i / 2 & 3] = fmaxf(fmaxf(top4[i / 2 & 3], __uint_as_float(x[i])), __uint_as_float(x[i +
-                            1]));
-                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * sc;
+                        top4[i / 2 & 3] = max3_nan(top4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    const float top = max3_nan(top4[0], top4[1], max3_nan(top4[2], top4[3], top4[3])) * sc;
                     const bool past = top > m + (W::kLift + W::kSlack);
                     if (__any_sync(kFull, past)) {
                         const float mm = past ? top - W::kLift : m, f = past ? ex2(m - mm) : 1.f;
@@ -714,8 +720,9 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                     if (!good) break;
                     tc::tc_fence_after();             // the products have read the previous weights
                     const uint32_t p_at = p_col(t, 0) + lanes, p_low = p_col(t, 1) + lanes;
-                    // a row without a key so far needs exact zeros
-                    if (L::kSplit || edge || __any_sync(kFull, m == -INFINITY))
+                    // a row without a key so far needs exact zeros, and one with a score of NaN or +infinity (which make
+                    // it NaN) the exponential that keeps them
+                    if (L::kSplit || edge || __any_sync(kFull, m == -INFINITY || !(top < INFINITY)))
                         l += weights<C, L::kSplit, false, SK>(x, sc, -base, p_at, p_low);
                     else
                         l += weights<C, L::kSplit, true, SK>(x, sc, -base, p_at, p_low);

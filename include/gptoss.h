@@ -315,7 +315,8 @@ int gptoss_kv_append(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* bat
  * head_dim, q_stride and out_stride elements apart, 16-byte aligned, of the cache's type, or fp32 beside an fp16 cache
  * (queries and weights then in two fp16 parts, about 22 bits). The weights of the second product are rounded to the
  * cache's type; beside an fp16 cache to 2^-38 of the row's largest weight where that is more. scale: finite, not 0. Statistics and sums are fp32. A row that sees no key is 0,
- * and what a row may not see does not reach it, NaN and infinities included. Results do not depend on timing.
+ * and what a row may not see does not reach it, NaN and infinities included; a score of NaN or +infinity that it sees
+ * makes it NaN (with fp32 queries an infinite key does). Results do not depend on timing.
  * Sequences of up to 64 query rows (new tokens x q_heads / kv_heads; 16 for head_dim 128) run on one kernel, longer
  * chunks on another; a batch with both takes two launches. Page sizes that are multiples of 8 are the fast ones for
  * chunks. */

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, lib, make_pages, new_q, reference_attention,  # noqa: F401
-                            run_attention, run_fork)
+from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, check_attention, lib, make_pages, new_q,  # noqa: F401
+                            reference_attention, run_attention, run_fork)
 
 pytestmark = pytest.mark.gpu
 
@@ -50,6 +50,37 @@ def test_attention_beside_a_dominant_key(lib, new, length, dim, page, pair, rest
         bound = bound + 2.0 ** -38 * s.values[0].double().abs().sum(0)
     worst = ((out.double() - want).abs() / bound).max().item()
     assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (64, 20), (128, 16), (128, 20)])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("where", [0, 128])
+def test_attention_visible_scores_that_are_not_finite(lib, new, dim, page, pair, where):
+    """Sequence b holds a key of NaN, or one with an infinity, at position where + b, which all its rows see and whose
+    neighbours none of them masks: a score of NaN or +infinity makes the row NaN, one of -infinity has no weight."""
+    n, length = 32, 400
+    s = Setup(lib, [new] * n, [length] * n, page=page, kvh=1, dim=dim, dtype=pair[1], seed=40)
+    q = new_q(s.T, 8, dim, pair[0])
+    good = [k.clone() for k in s.keys]
+    for b in range(n):
+        set_kv(s, b, [where + b], keys=torch.full((1, 1, dim), float("nan"), device="cuda"))
+    assert torch.isnan(run_attention(lib, s, q)).all()
+    for b in range(n):
+        key = good[b][where + b].clone()
+        key[0, 5] = float("inf")
+        set_kv(s, b, [where + b], keys=key[None])
+    out = run_attention(lib, s, q)
+    up = q[:, :, 5] > 0
+    assert torch.isnan(out[up]).all()
+    if pair[0] == pair[1]:
+        for b in range(n):                            # a key far below the others in the place of -infinity
+            key = good[b][where + b].float()
+            key[0, 5] = 3e4
+            s.keys[b][where + b] = key.to(pair[1])
+        low = q[:, :, 5].float() < -0.1               # 3e4 * 0.1 / sqrt(dim) below the others: weight 0 in 64 bits too
+        want, mag = reference_attention(s, q, None, dim ** -0.5, 0)
+        check_attention(out[low], want[low], mag[low])
 
 
 # --------------------------------------------------------------------------------------------------------- pages
