@@ -83,6 +83,48 @@ def test_attention_visible_scores_that_are_not_finite(lib, new, dim, page, pair,
         check_attention(out[low], want[low], mag[low])
 
 
+@pytest.mark.parametrize("pair", PAIRS, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (64, 20), (128, 16), (128, 20)])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("new", [150, 400])
+def test_attention_chunks_beside_bad_positions_of_later_rows(lib, new, window, dim, page, pair):
+    """NaN and infinities in keys and values that only some rows of a chunk see, alone in a pool (items cut into pieces)
+    and with other sequences: the rows that do not see them are right, those that do are not finite."""
+    for shape in ([1500], [1500, 700, 1500]):
+        news = [new, 33, new][:len(shape)]
+        s = Setup(lib, news, shape, page=page, kvh=2, dim=dim, dtype=pair[1], seed=50)
+        q = new_q(s.T, 16, dim, pair[0])
+        want, mag = reference_attention(s, q, None, dim ** -0.5, window)
+        first = 1500 - new
+        # (position, its key or its value, what it holds)
+        bad = [(first + 20, "v", float("nan")), (first + 77, "k", float("nan")), (first + 103, "v", float("inf")),
+               (1499, "k", float("nan"))]
+        for pos, what, x in bad:
+            held = torch.full((1, 2, dim), x, device="cuda")
+            set_kv(s, 0, [pos], **({"keys": held} if what == "k" else {"values": held}))
+        out = run_attention(lib, s, q, None, window)
+        p = torch.arange(first, 1500, device="cuda")
+        sees = torch.zeros(s.T, dtype=torch.bool, device="cuda")
+        for pos, *_ in bad:
+            sees[:new] |= (p >= pos) & (p - pos < (window or 1 << 30))
+        assert 0 < sees.sum() < new
+        check_attention(out[~sees], want[~sees], mag[~sees])
+        assert not torch.isfinite(out[sees]).any()
+        assert s.pool.status() == 0
+
+
+@pytest.mark.parametrize("page", [16, 20])
+def test_attention_chunk_whose_window_begins_behind_bad_positions(lib, page):
+    """Positions before the first row's window share its tile (and its page) and hold NaN: no row sees them."""
+    s = Setup(lib, [300], [1000], page=page, kvh=1, dim=64, dtype=F16, seed=51)
+    q = new_q(300, 8, 64, F16)
+    want, mag = reference_attention(s, q, None, 0.125, 77)
+    gone = np.arange(701 - 77)                        # position 700's window begins at 624
+    nan = torch.full((len(gone), 1, 64), float("nan"), device="cuda")
+    set_kv(s, 0, gone, nan, nan)
+    check_attention(run_attention(lib, s, q, None, 77), want, mag)
+
+
 # --------------------------------------------------------------------------------------------------------- pages
 def fork_by_rule(refs, tables, lens, parents, extra, page):
     """The header's rule, by whole numbers: (counts, tables, lengths, [(source, destination)], ran short)."""
