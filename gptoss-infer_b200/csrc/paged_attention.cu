@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "paged_schedule.cuh"
+#include "device_once.h"
 #include "kernels.h"
 #include "tc.cuh"
 
@@ -566,9 +567,12 @@ constexpr int kSlotFloats = std::max(slot_floats<32, 64>(), slot_floats<16, 128>
 template <class T, class C, int D, int NT>
 void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
     using S = Shape<T, D, NT>;
-    static const cudaError_t attr = cudaFuncSetAttribute(paged_rows_kernel<T, C, D, NT>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    GPT_CHECK(attr);
+    static DeviceOnce once;
+    int dev = 0;
+    GPT_CHECK(cudaGetDevice(&dev));
+    once.run(dev, [] {
+        GPT_CHECK(cudaFuncSetAttribute(paged_rows_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    });
     const int grid = std::min(kMaxCtas, num_sms() * S::kPerSm);
     paged_rows_kernel<T, C, D, NT><<<grid, kThreads, S::kSmem, s>>>(
         c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),

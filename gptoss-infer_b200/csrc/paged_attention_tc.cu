@@ -29,6 +29,7 @@
 #include <type_traits>
 
 #include "paged_schedule.cuh"
+#include "device_once.h"
 #include "kernels.h"
 #include "tc.cuh"
 
@@ -857,9 +858,12 @@ constexpr int kMaxCtas = 160;
 template <class T, class C, int D, bool TMA>
 void launch(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws, cudaStream_t s) {
     using L = Layout<T, D, TMA>;
-    static const cudaError_t attr = cudaFuncSetAttribute(paged_tiles_kernel<T, C, D, TMA>,
-                                                         cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
-    GPT_CHECK(attr);
+    static DeviceOnce once;
+    int dev = 0;
+    GPT_CHECK(cudaGetDevice(&dev));
+    once.run(dev, [] {
+        GPT_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<T, C, D, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+    });
     paged_tiles_kernel<T, C, D, TMA><<<std::min(kMaxCtas, num_sms()), block_threads(TMA), L::kSmem, s>>>(
         maps, c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
         reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes));
