@@ -325,7 +325,8 @@ int gptoss_paged_attention(gptoss_kv_pool* pool, int layer, const gptoss_kv_batc
                            long long out_stride, void* stream);
 
 /* [extension] Forks, reorders, grows and frees sequences, asynchronous on `stream`. Child m continues sequence
- * parents[m] (-1: an empty child) of the given `seqs` and gets room for extra[m] more positions (extra NULL: none):
+ * parents[m] of the given `seqs` and gets room for extra[m] more positions (extra NULL, or negative: none). Parent -1
+ * makes an empty child of length 0 without pages, whose extra does not count: a later call gives it room.
  * tables_out [children][table_stride] (unused entries -1), lens_out[m] = lens[parent] + extra[m]. refs and refs_out
  * (int32 [num_pages], may alias) count each page's references: those of the given sequences are dropped (a sequence
  * without a child is thereby freed), the children's added. Full pages are shared. A part-filled last page that would be

@@ -226,3 +226,15 @@ def test_fork_shared_last_pages_at_random(lib, seed):
     children = int(r.randint(1, 3 * seqs))
     parents = [int(x) for x in r.randint(-1, seqs, children)]
     check_fork(lib, refs, tables, lens, parents, [int(x) for x in r.randint(0, 3, children)], page, 8)
+
+
+def test_fork_empty_children_get_no_pages(lib):
+    """Parent -1: length 0 and no pages whatever its extra says; the next call gives the room. Negative extras count as
+    none."""
+    check_fork(lib, [1, 1] + [0] * 6, [[0, 1]], [6], [-1, 0, -1], [5, 3, 9], 4, 4)
+    k, v = make_pages(1, 8, 4, 2, 64, F16, False, 3)
+    pool = Pool(lib, k, v)
+    got = run_fork(lib, pool, [0] * 8, [], [], [-1, -1], [5, 9], 4)
+    assert got == ([0] * 8, [[-1] * 4] * 2, [0, 0])
+    got = run_fork(lib, pool, got[0], [[], []], [0, 0], [0, 1], [5, -9], 4)
+    assert got[1:] == ([[0, 1, -1, -1], [-1] * 4], [5, 0]) and pool.status() == 0
