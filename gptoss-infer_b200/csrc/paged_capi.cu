@@ -7,6 +7,7 @@
 #include <memory>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 #include "capi_guard.h"
 #include "common.cuh"
@@ -88,28 +89,36 @@ gpt::KvBatch check_batch(const gptoss_kv_pool* p, int layer, const gptoss_kv_bat
     return r;
 }
 
-// Grow-only workspace owned by the calling thread, one per device, zeroed whenever it grows.
+// Grow-only workspace owned by the calling thread, one per device, zeroed when made. A stream capture keeps the address
+// that its call had, so what growth leaves behind stays until the thread ends (each is at least twice the one before it,
+// or 64 MB larger).
 struct ThreadWs {
-    void* p[64] = {};
-    size_t n[64] = {};
+    struct Held {
+        std::vector<void*> all;               // the last is the present one
+        size_t n = 0;
+    };
+    Held held[64];
     ~ThreadWs() {
-        for (int d = 0; d < 64; ++d)
-            if (p[d]) cudaFree(p[d]);
+        for (const Held& h : held)
+            for (void* p : h.all) cudaFree(p);
     }
     void* get(size_t bytes) {
         int dev = 0;
         GPT_CHECK(cudaGetDevice(&dev));
         if (dev < 0 || dev >= 64) throw std::runtime_error("device index out of range");
-        if (n[dev] < bytes) {
-            if (p[dev]) GPT_CHECK(cudaFree(p[dev]));
-            p[dev] = nullptr;
-            n[dev] = 0;
-            GPT_CHECK(cudaMalloc(&p[dev], bytes));
-            GPT_CHECK(cudaMemset(p[dev], 0, bytes));
+        Held& h = held[dev];
+        if (h.n < bytes) {
+            const size_t n = std::max(bytes, h.n + std::min(h.n, size_t(64) << 20));
+            h.all.reserve(h.all.size() + 1);
+            void* p = nullptr;
+            GPT_CHECK(cudaMalloc(&p, n));
+            h.all.push_back(p);
+            h.n = 0;                          // until it is zeroed
+            GPT_CHECK(cudaMemset(p, 0, n));
             GPT_CHECK(cudaDeviceSynchronize());   // the caller's stream may not be ordered with the memset's
-            n[dev] = bytes;
+            h.n = n;
         }
-        return p[dev];
+        return h.all.back();
     }
 };
 thread_local ThreadWs g_beam_ws;

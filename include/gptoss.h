@@ -273,7 +273,7 @@ int gptoss_set_prefill_packing(int mode);
  * page_size >= 1. A sequence's table is an int32 row of page ids: position p lives in page table[p / page_size], slot
  * p % page_size; entries past its last position are never read. The handle owns its workspaces (about 22 MB, 43 MB for
  * head_dim 128, and 20 bytes per page) and an error word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
- * current at its creation. Returns NULL on failure (gptoss_last_error). Synchronizes. */
+ * current at its creation. Calls allocate nothing; one captured in a graph needs the pool until its last replay. Returns NULL on failure (gptoss_last_error). Synchronizes. */
 typedef struct gptoss_kv_pool gptoss_kv_pool;
 gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, int num_pages, int page_size,
                                       int kv_heads, int head_dim, const long long* strides);
@@ -355,7 +355,8 @@ int gptoss_kv_compact(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* 
  * places without a candidate get score -inf, row -1, token -1. Outputs [batch][picks]: out_scores fp32, rows (of
  * logits, so they serve as gptoss_kv_fork's parents), tokens. Sums and ranking use fp32 statistics and fp64 scores.
  * Uses the calling thread's workspace: calls from one thread must not overlap on the GPU, and the first call at a
- * larger size allocates (make it before a stream capture). */
+ * larger size allocates (make it before a stream capture). A captured call goes on using the workspace of the thread
+ * that captured it, whatever larger calls follow: its replays count among that thread's calls and end before it does. */
 int gptoss_beam_select(const void* logits, int type, long long row_stride, const float* scores, const uint8_t* done,
                        int done_token, int batch, int beams, int vocab, int picks, float* out_scores, int32_t* rows,
                        int32_t* tokens, void* stream);

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, check_attention, lib, make_pages, new_q,  # noqa: F401
-                            reference_attention, run_attention, run_fork)
+                            reference_attention, run_attention, run_beams, run_fork)
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +238,28 @@ def test_fork_empty_children_get_no_pages(lib):
     assert got == ([0] * 8, [[-1] * 4] * 2, [0, 0])
     got = run_fork(lib, pool, got[0], [[], []], [0, 0], [0, 1], [5, -9], 4)
     assert got[1:] == ([[0, 1, -1, -1], [-1] * 4], [5, 0]) and pool.status() == 0
+
+
+# --------------------------------------------------------------------------------------------------------- beams
+def test_beams_captured_before_the_workspace_grows(lib):
+    """A graph of a small selection gives the same picks after larger calls of the same thread, in memory that other
+    tensors have been given meanwhile."""
+    g = torch.Generator(device="cuda").manual_seed(60)
+    x, scores = torch.randn(6, 40000, device="cuda", generator=g), -torch.rand(6, device="cuda", generator=g)
+    want = run_beams(lib, x, scores, None, 0, 3, 5)
+    out = [torch.zeros(10, dtype=t, device="cuda") for t in (torch.float32, torch.int32, torch.int32)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert lib.gptoss_beam_select(x.data_ptr(), 0, 40000, scores.data_ptr(), None, 0, 2, 3, 40000, 5,
+                                      *(t.data_ptr() for t in out), torch.cuda.current_stream().cuda_stream) == 0
+    for rows in (64, 256, 1024, 4096):
+        y = torch.randn(rows, 20000, device="cuda", generator=g)
+        z = torch.zeros(rows, device="cuda")
+        first = run_beams(lib, y, z, None, 0, 64, 64)
+        filler = [torch.full((1 << 18,), -1, device="cuda", dtype=torch.int32) for _ in range(64)]
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(np.array_equal(a.cpu().numpy(), b.reshape(-1)) for a, b in zip(out, want))
+        assert all((f == -1).all() for f in filler)
+        assert all(np.array_equal(a, b) for a, b in zip(first, run_beams(lib, y, z, None, 0, 64, 64)))
