@@ -27,9 +27,10 @@ using namespace paged;
 constexpr int kThreads = 512, kPer = 32, kPart = kThreads * kPer, kWarps = kThreads / 32, kMostPicks = 64;
 constexpr int kList = kMostPicks * kPer;
 
-// fp32 bits in an order that compares as unsigned: the larger float is the larger word; NaN is not passed in.
+// fp32 bits in an order that compares as unsigned: the larger float is the larger word, both zeros are the same one (the
+// sum makes -0 into +0); NaN is not passed in.
 __device__ __forceinline__ uint32_t ordered(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t o) {

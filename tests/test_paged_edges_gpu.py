@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, check_attention, lib, make_pages, new_q,  # noqa: F401
-                            reference_attention, run_attention, run_beams, run_fork)
+from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, check_attention, check_beams, lib, make_pages,  # noqa: F401
+                            new_q, reference_attention, run_attention, run_beams, run_fork)
 
 pytestmark = pytest.mark.gpu
 
@@ -263,3 +263,20 @@ def test_beams_captured_before_the_workspace_grows(lib):
             assert all(np.array_equal(a.cpu().numpy(), b.reshape(-1)) for a, b in zip(out, want))
         assert all((f == -1).all() for f in filler)
         assert all(np.array_equal(a, b) for a, b in zip(first, run_beams(lib, y, z, None, 0, 64, 64)))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, F16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [17, 9000, 50001])
+def test_beams_zeros_of_both_signs_are_equal(lib, dtype, vocab):
+    """-0.0 and +0.0 are equal scores: the lower token wins, within a part of a row, between parts and between rows."""
+    x = torch.zeros(4, vocab, device="cuda", dtype=dtype)
+    x[:, 0] = -0.0
+    check_beams(lib, x, torch.zeros(4, device="cuda"), None, 0, 1, 1)
+    x[:, ::2] = -0.0
+    check_beams(lib, x, torch.zeros(4, device="cuda"), None, 0, 2, 12)
+    x[:] = -0.0
+    x[:, vocab // 2:] = 0.0
+    check_beams(lib, x, torch.tensor([-0.0, 0.0, 0.0, -0.0], device="cuda"), None, 0, 4, 40)
+    x[:, 3:] = -1.0
+    x[2, 1] = 0.0
+    check_beams(lib, x, torch.zeros(4, device="cuda"), None, 0, 4, 9)
