@@ -268,9 +268,9 @@ int gptoss_kv_fork(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tables
         require(seqs >= 0 && children >= 0 && table_stride >= 0, "kv_fork: negative size");
         require(seqs <= (1 << 20) && children <= (1 << 20), "kv_fork: at most 2^20 sequences and children");
         require(refs && refs_out, "kv_fork: null reference counts");
-        require(seqs == 0 || table_stride == 0 || (tables && lens), "kv_fork: null tables or lengths");
+        require(seqs == 0 || (lens && (tables || table_stride == 0)), "kv_fork: null tables or lengths");
         require(children == 0 || (parents && lens_out && (tables_out || table_stride == 0)), "kv_fork: null children");
-        require(seqs == 0 || children == 0 || (tables_out != tables && lens_out != lens),
+        require(seqs == 0 || children == 0 || ((tables_out != tables || table_stride == 0) && lens_out != lens),
                 "kv_fork: the children's tables and lengths need arrays of their own");
         check_device(p, "kv_fork");
         gpt::ForkArgs a{refs, tables, lens, parents, extra, refs_out, tables_out, lens_out, seqs, children,

@@ -240,6 +240,18 @@ def test_fork_empty_children_get_no_pages(lib):
     assert got[1:] == ([[0, 1, -1, -1], [-1] * 4], [5, 0]) and pool.status() == 0
 
 
+def test_fork_refuses_null_lengths_and_tables(lib):
+    """Lengths are read for every parent, also where tables have no columns."""
+    k, v = make_pages(1, 4, 4, 1, 64, F16, False, 3)
+    pool, t = Pool(lib, k, v), torch.zeros(64, dtype=torch.int32, device="cuda")
+    p = t.data_ptr()
+    for tables, lens, stride in ((None, None, 0), (p, None, 0), (p, None, 1), (None, p, 1)):
+        rc = lib.gptoss_kv_fork(pool.h, p, tables, lens, 1, p, None, 1, stride, p + 64, p + 128, p + 192, None)
+        assert rc == -1 and b"null tables or lengths" in lib.gptoss_last_error()
+    assert lib.gptoss_kv_fork(pool.h, p, None, p, 1, p, None, 1, 0, p + 64, None, p + 192, None) == 0
+    assert pool.status() == 0 and (t == 0).all()
+
+
 # --------------------------------------------------------------------------------------------------------- beams
 def test_beams_captured_before_the_workspace_grows(lib):
     """A graph of a small selection gives the same picks after larger calls of the same thread, in memory that other
