@@ -78,16 +78,12 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
     return before + x - v;
 }
 
-__device__ __forceinline__ int pages_of(int len, int page) { return (len + page - 1) / page; }
+__device__ __forceinline__ int pages_of(int len, int page) {
+    return int((unsigned(len) + unsigned(page) - 1) / unsigned(page));        // (len may be close to 2^31)
+}
 
 __device__ __forceinline__ int table_len(const int* lens, int i, int stride, int page, int* err) {
-    const int len = lens[i];
-    const long long cap = (long long)stride * page;
-    if (len < 0 || len > cap) {
-        report(err, kKvBadLength);
-        return len < 0 ? 0 : int(cap);
-    }
-    return len;
+    return safe_len(lens[i], stride, page, err);
 }
 
 // Copies the pages of `moves` in all layers, K and V: pieces of 16 KB, one per CTA and step. Where a page is one run of
@@ -219,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
                         }
                     }
                     const long long want = (long long)len + (a.extra ? max(a.extra[m], 0) : 0);
-                    const long long cap = (long long)a.stride * p.page_size;
+                    const long long cap = min((long long)a.stride * p.page_size, (long long)kMostPositions);
                     if (want > cap) report(p.err, kKvBadLength);
                     want_len = int(min(want, cap));
                 }

@@ -15,7 +15,7 @@ enum KvType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
 // Codes of a pool's device-side error word (gptoss_kv_pool_status).
 enum KvError : int {
     kKvBadPage = 300,        // a table names a page outside the pool
-    kKvBadLength = 301,      // a cache length is negative or longer than its table
+    kKvBadLength = 301,      // a cache length is negative, longer than its table or near 2^31
     kKvBadBatch = 302,       // cu_tokens runs backwards or past the batch's tokens
     kKvBadPosition = 303,    // a new token's position is negative or past the cos/sin table
     kKvOutOfPages = 304,     // gptoss_kv_fork found fewer free pages than it needs

@@ -4,8 +4,10 @@ import numpy as np
 import pytest
 import torch
 
+from gptoss_b200 import capi
 from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, check_attention, check_beams, lib, make_pages,  # noqa: F401
-                            new_q, reference_attention, run_attention, run_beams, run_fork)
+                            ints, new_q, reference_attention, run_attention, run_beams, run_fork,
+                            stream)
 
 pytestmark = pytest.mark.gpu
 
@@ -123,6 +125,37 @@ def test_attention_chunk_whose_window_begins_behind_bad_positions(lib, page):
     nan = torch.full((len(gone), 1, 64), float("nan"), device="cuda")
     set_kv(s, 0, gone, nan, nan)
     check_attention(run_attention(lib, s, q, None, 77), want, mag)
+
+
+@pytest.mark.parametrize("new", [1, 80])
+def test_lengths_up_to_31_bits(lib, new):
+    """2048 pages of 2^20 slots that are all one page in memory: 2^31 - 4096 positions are right, more are flagged."""
+    page, most, W = 1 << 20, (1 << 31) - 4096, 100
+    g = torch.Generator(device="cuda").manual_seed(52)
+    k, v = (torch.randn(page, 1, 64, device="cuda", generator=g).half().as_strided((1, 2048, page, 1, 64), (0, 0, 64, 64, 1))
+            for _ in range(2))
+    s = Setup.__new__(Setup)
+    s.pool, s.T, s.kvh = Pool(lib, k, v), new, 1
+    s.cu, s.dlens, s.dtab = ints([0, new]), ints([most]), ints([list(range(2048))])
+    s.batch = capi.KvBatch(1, new, new, 2048, s.cu.data_ptr(), s.dlens.data_ptr(), s.dtab.data_ptr())
+    q = new_q(new, 8, 64, F16)
+    out = run_attention(lib, s, q, None, W)
+    assert s.pool.status() == 0
+    tail = torch.arange(most - 200, most, device="cuda") % page           # the same sum over the last 200 positions
+    s.new, s.lens, s.keys, s.values = [new], [200], [k[0, 0][tail]], [v[0, 0][tail]]
+    check_attention(out, *reference_attention(s, q, None, 0.125, W))
+    for length in (most + 1, (1 << 31) - 1):
+        s.dlens.fill_(length)
+        run_attention(lib, s, q, None, W)
+        assert s.pool.status() == 301
+    # room past 2^31 - 4096 is not given
+    refs, lens = ints([0] * 2048), ints([most - 5])
+    tables, lens_out, refs_out = torch.empty(1, 2048, dtype=torch.int32, device="cuda"), ints([7]), ints([0] * 2048)
+    for extra, want, code in ((5, most, 0), (6, most, 301), ((1 << 31) - 1, most, 301)):
+        assert lib.gptoss_kv_fork(s.pool.h, refs.fill_(1).data_ptr(), s.dtab.data_ptr(), lens.data_ptr(), 1, ints([0]).data_ptr(),
+                                  ints([extra]).data_ptr(), 1, 2048, refs_out.data_ptr(), tables.data_ptr(),
+                                  lens_out.data_ptr(), stream()) == 0
+        assert s.pool.status() == code and lens_out.item() == want
 
 
 # --------------------------------------------------------------------------------------------------------- pages
