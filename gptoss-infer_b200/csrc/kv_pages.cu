@@ -57,18 +57,19 @@ __device__ __forceinline__ void grid_barrier(int* barrier, int* err) {
 }
 
 // Exclusive prefix sum over the block; *total gets the sum. Three barriers.
-__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* total) {
+template <class V>
+__device__ __forceinline__ V block_scan(V v, V* warp_sums, V* total) {
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    int x = v;
+    V x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(kFull, x, o);
+        const V y = __shfl_up_sync(kFull, x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();
     if (lane == 31) warp_sums[warp] = x;
     __syncthreads();
-    int before = 0, all = 0;
+    V before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) before += warp_sums[w];
@@ -125,6 +126,7 @@ __device__ __forceinline__ void copy_pages(const KvPages& p, int n, const int2* 
 
 __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArgs a, PageWs w) {
     __shared__ int sums[kThreads / 32];
+    __shared__ long long wide_sums[kThreads / 32];
     const long long step = (long long)gridDim.x * kThreads, t0 = (long long)blockIdx.x * kThreads + threadIdx.x;
     // --- references dropped and added (full pages), the first child of each part-filled last page
     for (long long i = t0, n = (long long)a.seqs * a.stride; i < n; i += step) {
@@ -194,8 +196,9 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
             free_pages += total;
         }
         __syncthreads();
-        // --- fresh pages, in the order of the children
-        int used = 0, copies = 0;
+        // --- fresh pages, in the order of the children (what they ask for together may pass 2^31)
+        long long used = 0;
+        int copies = 0;
         for (int m0 = 0; m0 < a.children; m0 += kThreads) {
             const int m = m0 + threadIdx.x;
             int have = 0, want_len = 0, src = -1;
@@ -221,11 +224,12 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
                 }
             }
             const int n = max(0, pages_of(want_len, p.page_size) - have);
-            int total, total_copies;
-            const int at = used + block_scan(n, sums, &total);
-            const int got = max(0, min(n, free_pages - at));
+            long long total;
+            int total_copies;
+            const long long at = used + block_scan((long long)n, wide_sums, &total);
+            const int got = int(max(0ll, min((long long)n, free_pages - at)));
             const bool copy = src >= 0 && got > 0;
-            const int slot = copies + block_scan(copy, sums, &total_copies);
+            const int slot = copies + block_scan(int(copy), sums, &total_copies);
             if (m < a.children) {
                 if (got < n) report(p.err, kKvOutOfPages);
                 for (int i = 0; i < got; ++i) {

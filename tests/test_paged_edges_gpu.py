@@ -6,7 +6,7 @@ import torch
 
 from gptoss_b200 import capi
 from test_paged_gpu import (F16, PAIRS, Pool, Setup, U, check_attention, check_beams, lib, make_pages,  # noqa: F401
-                            ints, new_q, reference_attention, run_attention, run_beams, run_fork,
+                            ints, new_q, ok, reference_attention, run_attention, run_beams, run_fork,
                             stream)
 
 pytestmark = pytest.mark.gpu
@@ -259,6 +259,21 @@ def test_fork_shared_last_pages_at_random(lib, seed):
     children = int(r.randint(1, 3 * seqs))
     parents = [int(x) for x in r.randint(-1, seqs, children)]
     check_fork(lib, refs, tables, lens, parents, [int(x) for x in r.randint(0, 3, children)], page, 8)
+
+
+def test_fork_of_children_that_ask_for_more_than_31_bits_of_pages(lib):
+    """600 children of 2^22 pages each in a pool of five free ones: the first gets those, the others none."""
+    n, room = 600, 1 << 22
+    k, v = make_pages(1, 6, 1, 1, 64, F16, False, 3)
+    pool = Pool(lib, k, v)
+    refs, tables, lens = ints([0, 0, 1, 0, 0, 0]), torch.full((1, room), 2, dtype=torch.int32, device="cuda"), ints([1])
+    out, lens_out = torch.empty(n, room, dtype=torch.int32, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda")
+    parents, extra = ints([0] * n), ints([room - 1] * n)
+    ok(lib, lib.gptoss_kv_fork(pool.h, refs.data_ptr(), tables.data_ptr(), lens.data_ptr(), 1, parents.data_ptr(),
+                               extra.data_ptr(), n, room, refs.data_ptr(), out.data_ptr(), lens_out.data_ptr(), stream()))
+    assert pool.status() == 304
+    assert lens_out.tolist() == [6] + [1] * (n - 1) and refs.tolist() == [1, 1, n, 1, 1, 1]
+    assert out[0, :7].tolist() == [2, 0, 1, 3, 4, 5, -1] and (out[:, 0] == 2).all() and (out[1:, 1:] == -1).all()
 
 
 def test_fork_empty_children_get_no_pages(lib):
