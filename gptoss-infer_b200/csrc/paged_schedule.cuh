@@ -44,7 +44,7 @@ struct Schedule {
         it.rows = min(R, it.s.n * int(group.d) - r0);
         it.p0 = it.s.len - it.s.n + int(group.div(r0));
         it.p1 = it.s.len - it.s.n + int(group.div(r0 + it.rows - 1));
-        it.lo = window ? max(0, it.p0 - window + 1) & -align : 0;
+        it.lo = window ? max(0, max(it.p0, 0) - (window - 1)) & -align : 0;     // (p0 may be negative, the window 2^31 - 1)
         it.hi = max(it.lo, it.p1 + 1);
         it.n = max(1, (it.hi - it.lo + UNIT - 1) / UNIT);
     }

@@ -127,6 +127,18 @@ def test_attention_chunk_whose_window_begins_behind_bad_positions(lib, page):
     check_attention(run_attention(lib, s, q, None, 77), want, mag)
 
 
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("most", [1, 500])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 3, 1 << 30, 6])
+def test_attention_windows_of_any_size_beside_rows_before_position_0(lib, window, most, page):
+    """A window longer than every sequence hides nothing, also in tiles whose first rows stand before position 0."""
+    s = Setup(lib, [2, 12, 1, 130], [0, 5, 30, 9], page=page, kvh=1, dim=64, dtype=F16, seed=53)
+    q = new_q(s.T, 8, 64, F16)
+    out = run_attention(lib, s, q, None, window, max_new=most)
+    check_attention(out, *reference_attention(s, q, None, 0.125, window))
+    assert s.pool.status() == 0
+
+
 @pytest.mark.parametrize("new", [1, 80])
 def test_lengths_up_to_31_bits(lib, new):
     """2048 pages of 2^20 slots that are all one page in memory: 2^31 - 4096 positions are right, more are flagged."""
