@@ -20,6 +20,7 @@ enum KvError : int {
     kKvBadPosition = 303,    // a new token's position is negative or past the cos/sin table
     kKvOutOfPages = 304,     // gptoss_kv_fork found fewer free pages than it needs
     kKvBadParent = 305,      // a parent outside the given sequences
+    kKvTooMuch = 306,        // new tokens times cached positions past what one call of the attention counts
     kKvWait = 310            // a bounded wait inside a kernel gave up (310 .. 319)
 };
 
@@ -78,6 +79,7 @@ struct PagedAttnArgs {
     int type, kv_type, q_heads, window;
     float scale;
     int rows_from, rows_to;                  // sequences with so many query rows per key/value head; others are left out
+    bool check;                              // set by the launchers (many_groups in paged_schedule.cuh)
 };
 // Workspace of launch_paged_attention: counters and partial results; zeroed once, the kernels leave the counters at 0.
 // The two kernels share it (their counters are the same words).

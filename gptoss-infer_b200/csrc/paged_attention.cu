@@ -143,7 +143,7 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
     __shared__ long long scratch[kWarps + 2];
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Schedule<R, kGroup> sch{c, b, a.window, group, 1, a.rows_from, a.rows_to};
+    const Schedule<R, kGroup> sch{c, b, a.window, group, 1, a.rows_from, a.rows_to, a.check};
     const Span sp = find_span<kThreads>(sch, kWarps, scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
@@ -574,8 +574,10 @@ void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
         GPT_CHECK(cudaFuncSetAttribute(paged_rows_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     });
     const int grid = std::min(kMaxCtas, num_sms() * S::kPerSm);
+    PagedAttnArgs args = a;
+    args.check = many_groups(b, c, a, S::kKeys, S::R);
     paged_rows_kernel<T, C, D, NT><<<grid, kThreads, S::kSmem, s>>>(
-        c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
+        c, b, args, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
         reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes));
     check_launch("paged_attention");
 }

@@ -277,7 +277,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
 
     const int warp = int(threadIdx.x / 32), lane = threadIdx.x % 32;
     int* err = c.err;
-    const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1, a.rows_from, a.rows_to};
+    const Schedule<kRows, kTile> sch{c, b, a.window, group, TMA ? 1 << c.box_log : 1, a.rows_from, a.rows_to, a.check};
     const Span sp = find_span<kThreads>(sch, 4, scratch);
     if (sp.len == 0) return;
     const int G = int(group.d);
@@ -864,8 +864,10 @@ void launch(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAt
     once.run(dev, [] {
         GPT_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<T, C, D, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
     });
+    PagedAttnArgs args = a;
+    args.check = many_groups(b, c, a, kTile, kRows);
     paged_tiles_kernel<T, C, D, TMA><<<std::min(kMaxCtas, num_sms()), block_threads(TMA), L::kSmem, s>>>(
-        maps, c, b, a, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
+        maps, c, b, args, FastDiv::of(uint32_t(a.q_heads / c.kv_heads)), static_cast<int*>(ws),
         reinterpret_cast<float*>(static_cast<char*>(ws) + kCounterBytes));
     check_launch("paged_attention");
 }

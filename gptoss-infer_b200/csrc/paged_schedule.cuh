@@ -8,6 +8,8 @@
 // starts in and the item it ends in), which bounds the workspace by the grid alone. Every CTA finds its span itself
 // from the lengths in device memory: the host needs none of them.
 #pragma once
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace gpt {
@@ -22,6 +24,20 @@ struct Item {
     int n;                   // groups
 };
 
+// A head's groups are counted in 32 bits: n, a sequence's new tokens, or 0 (with an error word) where they would not fit.
+inline __device__ __noinline__ int countable(int n, int len, int tiles, int window, int unit, int tile_rows, int* err) {
+    const int keys = window ? min(len, min(window, 1 << 30) + tile_rows) : len;
+    if ((long long)tiles * (keys / unit + 3) < 1ll << 31) return n;
+    report(err, kKvTooMuch);
+    return 0;
+}
+// Whether tokens and tables allow a head of 2^31 groups, or so many groups for a CTA (then the kernel looks).
+inline bool many_groups(const KvBatch& b, const KvView& c, const PagedAttnArgs& a, int unit, int tile_rows) {
+    const double rows = std::min(double(b.tokens) * (a.q_heads / c.kv_heads), double(a.rows_to));
+    const double keys = std::min(double(b.table_stride) * c.page.d, a.window ? double(a.window) + tile_rows : 2147483648.0);
+    return (rows / tile_rows + b.seqs) * (keys / unit + 3) * c.kv_heads >= 2147483648.0;
+}
+
 template <int R, int UNIT>
 struct Schedule {
     const KvView& c;
@@ -30,11 +46,13 @@ struct Schedule {
     FastDiv group;
     int align;               // lo is a multiple of this (a power of two)
     int rows_from, rows_to;  // only sequences with so many rows (new tokens x group) have items
+    bool check;              // the host could not rule out a head of 2^31 groups (many_groups)
 
     __device__ __forceinline__ Seq seq(int i) const {
         Seq s = load_seq(b, c.page, i, c.err);
         const int rows = s.n * int(group.d);
         if (rows < rows_from || rows > rows_to) s.n = 0;
+        if (check) s.n = countable(s.n, s.len, row_tiles(s.n), window, UNIT, R, c.err);
         return s;
     }
     __device__ __forceinline__ int row_tiles(int n) const { return (n * int(group.d) + R - 1) / R; }
@@ -168,6 +186,13 @@ __device__ __forceinline__ long long block_prefix(long long v, long long* warp_s
     return before + x - v;
 }
 
+// Whether a CTA's share of all groups would not fit.
+inline __device__ __noinline__ bool too_much(long long total, int grid, int* err) {
+    if (total >> 30 < grid) return false;
+    report(err, kKvTooMuch);
+    return true;
+}
+
 // Finds this CTA's span; all NT threads call it. scratch: NT / 32 + 2 words of shared memory.
 //
 // With few items (an eighth of the grid at most) a span never crosses from one item into the next: items are laid out
@@ -192,6 +217,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
             items += __shfl_xor_sync(kFull, items, o);
         }
         const bool whole = items * 8 <= grid;
+        if (sch.check && too_much(total, grid, sch.c.err)) total = 0;
         sp.per = whole ? max(least, ceil_div(total, grid - items)) : ceil_div(total, grid);
         sp.start = (long long)blockIdx.x * sp.per;
         sp.len = 0;
@@ -230,6 +256,7 @@ __device__ __forceinline__ Span find_span(const Schedule<R, UNIT>& sch, int leas
         before = total + block_prefix<NT>(mine, scratch, &sum);
         total += sum;
     }
+    if (sch.check && too_much(total, grid, sch.c.err)) total = 0;
     sp.per = ceil_div(total, grid);
     sp.start = (long long)blockIdx.x * sp.per;
     sp.len = int(max(0ll, min((long long)sp.per, total - sp.start)));

@@ -280,8 +280,9 @@ gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, in
 void gptoss_kv_pool_destroy(gptoss_kv_pool* pool);
 /* [extension] Synchronizes, stores the pool's error word in *code and clears it. 0: every call since read valid tables
  * and lengths. Device-side data is checked on the device: 300 a page id outside the pool, 301 a length outside its
- * table or above 2^31 - 4096, 302 cu_tokens out of order, 303 a position outside the cos/sin table (or negative), 304 no free page left,
- * 305 a parent outside the sequences, 310 .. 319 a bounded wait gave up. What a flagged call wrote is not meaningful
+ * table or above 2^31 - 4096, 302 cu_tokens out of order, 303 a position outside the cos/sin table (or negative), 304 no
+ * free page left, 305 a parent outside the sequences, 306 more attention than one call counts (a sequence whose query
+ * rows times positions pass 2^38, or 2^46 where max_new was right), 310 .. 319 a bounded wait gave up. What a flagged call wrote is not meaningful
  * for the sequences concerned; nothing outside the given arrays is touched. */
 int gptoss_kv_pool_status(gptoss_kv_pool* pool, int* code);
 

@@ -127,6 +127,24 @@ def test_attention_chunk_whose_window_begins_behind_bad_positions(lib, page):
     check_attention(run_attention(lib, s, q, None, 77), want, mag)
 
 
+@pytest.mark.parametrize("others", [1, 40])
+def test_attention_of_more_than_one_call_counts_is_flagged(lib, others):
+    """2^17 new tokens of 8 heads over 2^20 positions, said to be one token: 2^33 groups of 16 keys. That sequence is left
+    out and flagged, the others are right."""
+    new, L, page = 1 << 17, 1 << 20, 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(54)
+    k, v = (torch.randn(1, 1, page, 1, 128, device="cuda", generator=g).half() for _ in range(2))
+    s = Setup.__new__(Setup)
+    s.pool, s.kvh, s.T, s.new, s.lens = Pool(lib, k, v), 1, new + 3 * others, [new] + [3] * others, [L] + [50] * others
+    s.cu, s.dlens, s.dtab = ints(np.cumsum([0] + s.new)), ints(s.lens), ints([[0]] * (1 + others))
+    s.batch = capi.KvBatch(1 + others, s.T, 1, 1, s.cu.data_ptr(), s.dlens.data_ptr(), s.dtab.data_ptr())
+    q = new_q(s.T, 8, 128, F16)
+    out = run_attention(lib, s, q)
+    assert s.pool.status() == 306
+    s.new, s.lens, s.keys, s.values = s.new[1:], s.lens[1:], [k[0, 0, :50]] * others, [v[0, 0, :50]] * others
+    check_attention(out[new:], *reference_attention(s, q[new:], None, 128 ** -0.5, 0))
+
+
 @pytest.mark.parametrize("page", [16, 20])
 @pytest.mark.parametrize("most", [1, 500])
 @pytest.mark.parametrize("window", [(1 << 31) - 1, (1 << 31) - 3, 1 << 30, 6])
