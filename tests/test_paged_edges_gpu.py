@@ -1,5 +1,7 @@
 """Paged key/value cache operators where they are easily wrong: shared last pages, rows that a few keys dominate, values
 that are not finite, zeros of both signs. Helpers and tolerances: test_paged_gpu.py."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -370,3 +372,24 @@ def test_beams_zeros_of_both_signs_are_equal(lib, dtype, vocab):
     x[:, 3:] = -1.0
     x[2, 1] = 0.0
     check_beams(lib, x, torch.zeros(4, device="cuda"), None, 0, 4, 9)
+
+
+def test_a_failed_allocation_does_not_fail_the_next_call(lib):
+    """A selection whose workspace (4 TB) cannot be had is refused; the next calls run."""
+    x, s, wide = torch.randn(2, 1000, device="cuda"), torch.zeros(2, device="cuda"), (1 << 25) - 1
+    k, v = make_pages(1, 4, 4, 1, 64, F16, False, 3)
+    pool, t = Pool(lib, k, v), torch.zeros(64, dtype=torch.int32, device="cuda")
+    p = t.data_ptr()
+    for _ in range(2):
+        assert lib.gptoss_beam_select(x.data_ptr(), 0, wide, s.data_ptr(), None, 0, 1 << 16, 64, wide, 64, p, p, p,
+                                      stream()) == -1
+        assert b"memory" in lib.gptoss_last_error()
+        check_beams(lib, x, s, None, 0, 2, 5)
+    cu, one, q, out = ints([0, 1]), ints([1]), new_q(1, 8, 64, F16), new_q(1, 8, 64, F16)
+    b = capi.KvBatch(1, 1, 1, 1, cu.data_ptr(), one.data_ptr(), p)
+    assert lib.gptoss_beam_select(x.data_ptr(), 0, wide, s.data_ptr(), None, 0, 1 << 16, 64, wide, 64, p, p, p,
+                                  stream()) == -1
+    t.zero_()
+    ok(lib, lib.gptoss_paged_attention(pool.h, 0, ctypes.byref(b), q.data_ptr(), 1, 512, 8, None, 0.125, 0, out.data_ptr(),
+                                       512, stream()))
+    assert pool.status() == 0 and torch.equal(out, v[0, 0, 0].expand(1, 8, 64))
