@@ -183,7 +183,10 @@ int gptoss_kv_pool_status(gptoss_kv_pool* p, int* code) {
         check_device(p, "kv_pool_status");
         GPT_CHECK(cudaDeviceSynchronize());
         GPT_CHECK(cudaMemcpy(code, p->err, sizeof(int), cudaMemcpyDeviceToHost));
-        if (*code) GPT_CHECK(cudaMemset(p->err, 0, sizeof(int)));
+        if (*code) {
+            GPT_CHECK(cudaMemset(p->err, 0, sizeof(int)));
+            GPT_CHECK(cudaDeviceSynchronize());   // or it could clear what a later call on another stream reports
+        }
     });
 }
 

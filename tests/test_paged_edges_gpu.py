@@ -190,6 +190,19 @@ def test_lengths_up_to_31_bits(lib, new):
         assert s.pool.status() == code and lens_out.item() == want
 
 
+def test_status_loses_no_report_of_the_next_call(lib):
+    """Reading the status clears it before it returns: what a call on another stream reports right after is kept."""
+    s = Setup(lib, [1], [20], page=16, kvh=1, dim=64, dtype=F16, seed=55)
+    q, side = new_q(1, 8, 64, F16), torch.cuda.Stream()
+    s.dtab.fill_(-1)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(300):
+            run_attention(lib, s, q)
+            assert s.pool.status() == 300
+    assert s.pool.status() == 0
+
+
 # --------------------------------------------------------------------------------------------------------- pages
 def fork_by_rule(refs, tables, lens, parents, extra, page):
     """The header's rule, by whole numbers: (counts, tables, lengths, [(source, destination)], ran short)."""
