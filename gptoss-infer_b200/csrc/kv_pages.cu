@@ -83,12 +83,9 @@ __device__ __forceinline__ int pages_of(int len, int page) {
     return int((unsigned(len) + unsigned(page) - 1) / unsigned(page));        // (len may be close to 2^31)
 }
 
-__device__ __forceinline__ int table_len(const int* lens, int i, int stride, int page, int* err) {
-    return safe_len(lens[i], stride, page, err);
-}
-
-// Copies the pages of `moves` in all layers, K and V: pieces of 16 KB, one per CTA and step. Where a page is one run of
-// memory (slot-major or head-major without gaps) a piece is eight 16-byte loads per thread in flight; otherwise rows.
+// Copies the pages of `moves` in all layers, K and V: pieces of 32 KB, one per CTA and step, four 16-byte loads of a
+// thread in flight. Where a page is one run of memory (slot-major or head-major without gaps) a piece is a part of the
+// run, otherwise rows.
 __device__ __forceinline__ void copy_pages(const KvPages& p, int n, const int2* moves) {
     const int rows = p.page_size * p.kv_heads, chunks = p.row_bytes / 16;
     const bool run = (p.head_stride == p.row_bytes && p.token_stride == (long long)p.row_bytes * p.kv_heads) ||
@@ -131,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
     // --- references dropped and added (full pages), the first child of each part-filled last page
     for (long long i = t0, n = (long long)a.seqs * a.stride; i < n; i += step) {
         const int s = int(i / a.stride), j = int(i - (long long)s * a.stride);
-        if (j >= pages_of(table_len(a.lens, s, a.stride, p.page_size, p.err), p.page_size)) continue;
+        if (j >= pages_of(safe_len(a.lens[s], a.most, p.err), p.page_size)) continue;
         const int id = a.tables[i];
         if (unsigned(id) < unsigned(p.num_pages)) atomicSub(&w.delta[id], 1);
         else report(p.err, kKvBadPage);
@@ -139,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
     for (long long i = t0, n = (long long)a.children * a.stride; i < n; i += step) {
         const int m = int(i / a.stride), j = int(i - (long long)m * a.stride), par = a.parents[m];
         int id = -1;
-        if (par >= 0 && par < a.seqs && j < table_len(a.lens, par, a.stride, p.page_size, p.err) / p.page_size) {
+        if (par >= 0 && par < a.seqs && j < safe_len(a.lens[par], a.most, p.err) / p.page_size) {
             id = a.tables[(long long)par * a.stride + j];
             if (unsigned(id) < unsigned(p.num_pages)) atomicAdd(&w.delta[id], 1);
         }
@@ -148,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
     for (long long m = step - 1 - t0; m < a.children; m += step) {      // by the threads that have no table entries
         const int par = a.parents[m];
         if (par >= 0 && par < a.seqs) {
-            const int len = table_len(a.lens, par, a.stride, p.page_size, p.err);
+            const int len = safe_len(a.lens[par], a.most, p.err);
             if (len % p.page_size == 0) continue;
             const int id = a.tables[(long long)par * a.stride + len / p.page_size];
             if (unsigned(id) < unsigned(p.num_pages)) atomicMin(&w.first[id], int(m));
@@ -162,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
         for (int m = threadIdx.x; m < a.children; m += kThreads) {
             const int par = a.parents[m];
             if (par < 0 || par >= a.seqs) continue;
-            const int len = table_len(a.lens, par, a.stride, p.page_size, p.err), full = len / p.page_size;
+            const int len = safe_len(a.lens[par], a.most, p.err), full = len / p.page_size;
             if (len % p.page_size == 0) continue;
             const int id = a.tables[(long long)par * a.stride + full];
             if (unsigned(id) < unsigned(p.num_pages) && __ldcg(&w.first[id]) == m &&
@@ -205,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
             if (m < a.children) {
                 const int par = a.parents[m];
                 if (par >= 0 && par < a.seqs) {
-                    const int len = table_len(a.lens, par, a.stride, p.page_size, p.err);
+                    const int len = safe_len(a.lens[par], a.most, p.err);
                     have = len / p.page_size;
                     if (len % p.page_size) {
                         const int id = a.tables[(long long)par * a.stride + have];
@@ -218,9 +215,8 @@ __global__ void __launch_bounds__(kThreads, 2) kv_fork_kernel(KvPages p, ForkArg
                         }
                     }
                     const long long want = (long long)len + (a.extra ? max(a.extra[m], 0) : 0);
-                    const long long cap = min((long long)a.stride * p.page_size, (long long)kMostPositions);
-                    if (want > cap) report(p.err, kKvBadLength);
-                    want_len = int(min(want, cap));
+                    if (want > a.most) report(p.err, kKvBadLength);
+                    want_len = int(min(want, (long long)a.most));
                 }
             }
             const int n = max(0, pages_of(want_len, p.page_size) - have);
@@ -301,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 2) kv_compact_kernel(KvPages p, Comp
     for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < n; i += (long long)gridDim.x * kThreads) {
         const int s = int(i / a.stride), j = int(i - (long long)s * a.stride);
         int id = -1;
-        if (j < pages_of(table_len(a.lens, s, a.stride, p.page_size, p.err), p.page_size)) {
+        if (j < pages_of(safe_len(a.lens[s], a.most, p.err), p.page_size)) {
             const int old = a.tables[i];
             if (unsigned(old) < unsigned(p.num_pages)) id = __ldcg(a.remap + old);
             else report(p.err, kKvBadPage);

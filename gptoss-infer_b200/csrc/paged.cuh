@@ -27,28 +27,25 @@ __device__ __forceinline__ int find_sequence(const int* __restrict__ cu, int seq
     return lo;
 }
 
-// The longest cache length: positions a few tiles past it are still 32-bit numbers.
-constexpr int kMostPositions = 0x7fffffff - 4095;
-// A length forced into its table's `entries` pages (with an error word).
-__device__ __forceinline__ int safe_len(int len, int entries, int page, int* err) {
-    const long long cap = min((long long)entries * page, (long long)kMostPositions);
-    if (len >= 0 && len <= cap) return len;
+// A length forced into 0 .. most (with an error word).
+__device__ __forceinline__ int safe_len(int len, int most, int* err) {
+    if (unsigned(len) <= unsigned(most)) return len;
     report(err, kKvBadLength);
-    return len < 0 ? 0 : int(cap);
+    return len < 0 ? 0 : most;
 }
 
 // Sequence b's rows and cache length, forced into range (with an error word) whatever the arrays hold.
 struct Seq {
     int row0, n, len;        // first row, new tokens, cache length with them
 };
-__device__ __forceinline__ Seq load_seq(const KvBatch& b, const FastDiv& page, int i, int* err) {
+__device__ __forceinline__ Seq load_seq(const KvBatch& b, int i, int* err) {
     int r0 = b.cu[i], r1 = b.cu[i + 1];
     if (r0 < 0 || r1 < r0 || r1 > b.tokens) {
         report(err, kKvBadBatch);
         r0 = min(max(r0, 0), b.tokens);
         r1 = min(max(r1, r0), b.tokens);
     }
-    return {r0, r1 - r0, safe_len(b.lens[i], b.table_stride, int(page.d), err)};
+    return {r0, r1 - r0, safe_len(b.lens[i], b.most, err)};
 }
 
 __device__ __forceinline__ int safe_page(int id, const KvView& c) {

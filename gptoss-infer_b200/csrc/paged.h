@@ -54,12 +54,20 @@ struct KvMaps {
     CUtensorMap k, v;
 };
 
+// The longest cache length of a table: its pages, and no more than positions a few tiles further on can be counted to in
+// 32 bits.
+inline int most_positions(int table_stride, int page_size) {
+    const long long n = static_cast<long long>(table_stride) * page_size;
+    return n < 0x7fffffff - 4095 ? static_cast<int>(n) : 0x7fffffff - 4095;
+}
+
 // Sequence b's new tokens are rows cu[b] .. cu[b + 1) of the batch; its cache holds lens[b] positions with them.
 struct KvBatch {
     const int* cu;
     const int* lens;
     const int* tables;
     int seqs, tokens, table_stride, max_new;
+    int most;                    // longest length of a table (most_positions)
 };
 
 struct AppendArgs {
@@ -109,11 +117,13 @@ struct ForkArgs {
     const int *refs, *tables, *lens, *parents, *extra;
     int *refs_out, *tables_out, *lens_out;
     int seqs, children, stride;
+    int most;                                // longest length of a table (most_positions)
 };
 struct CompactArgs {
     const int *refs, *tables, *lens;
     int *refs_out, *tables_out, *remap, *live;
     int seqs, stride;
+    int most;
 };
 // All layers of a pool, for copies of whole pages. Strides in bytes.
 struct KvPages {

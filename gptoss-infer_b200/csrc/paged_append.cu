@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(KvView c, KvBatch b
         const int t = t0 + warp, i = find_sequence(b.cu, b.seqs, t, lane);
         if (lane == 0) {
             Place w{nullptr, nullptr, -1};
-            const Seq q = load_seq(b, c.page, i, c.err);
+            const Seq q = load_seq(b, i, c.err);
             if (t >= q.row0 && t < q.row0 + q.n) {
                 const int pos = q.len - q.n + (t - q.row0);
                 if (pos < 0 || (a.rot > 0 && pos >= a.positions)) {

@@ -86,6 +86,7 @@ gpt::KvBatch check_batch(const gptoss_kv_pool* p, int layer, const gptoss_kv_bat
     r.tokens = b->tokens;
     r.table_stride = b->table_stride;
     r.max_new = b->max_new;
+    r.most = gpt::most_positions(b->table_stride, p->pages.page_size);
     return r;
 }
 
@@ -277,7 +278,7 @@ int gptoss_kv_fork(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tables
                 "kv_fork: the children's tables and lengths need arrays of their own");
         check_device(p, "kv_fork");
         gpt::ForkArgs a{refs, tables, lens, parents, extra, refs_out, tables_out, lens_out, seqs, children,
-            table_stride};
+            table_stride, gpt::most_positions(table_stride, p->pages.page_size)};
         gpt::launch_kv_fork(p->pages, a, p->page_ws, static_cast<cudaStream_t>(stream));
     });
 }
@@ -291,7 +292,8 @@ int gptoss_kv_compact(gptoss_kv_pool* p, const int32_t* refs, const int32_t* tab
         require(refs && refs_out && remap && live, "kv_compact: null pointer");
         require(seqs == 0 || table_stride == 0 || (tables && lens && tables_out), "kv_compact: null tables or lengths");
         check_device(p, "kv_compact");
-        gpt::CompactArgs a{refs, tables, lens, refs_out, tables_out, remap, live, seqs, table_stride};
+        gpt::CompactArgs a{refs, tables, lens, refs_out, tables_out, remap, live, seqs, table_stride,
+            gpt::most_positions(table_stride, p->pages.page_size)};
         gpt::launch_kv_compact(p->pages, a, p->page_ws, static_cast<cudaStream_t>(stream));
     });
 }

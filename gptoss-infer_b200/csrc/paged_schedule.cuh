@@ -49,7 +49,7 @@ struct Schedule {
     bool check;              // the host could not rule out a head of 2^31 groups (many_groups)
 
     __device__ __forceinline__ Seq seq(int i) const {
-        Seq s = load_seq(b, c.page, i, c.err);
+        Seq s = load_seq(b, i, c.err);
         const int rows = s.n * int(group.d);
         if (rows < rows_from || rows > rows_to) s.n = 0;
         if (check) s.n = countable(s.n, s.len, row_tiles(s.n), window, UNIT, R, c.err);
