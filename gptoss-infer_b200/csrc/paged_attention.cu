@@ -571,7 +571,8 @@ void launch(const KvView& c, const KvBatch& b, const PagedAttnArgs& a, void* ws,
     int dev = 0;
     GPT_CHECK(cudaGetDevice(&dev));
     once.run(dev, [] {
-        GPT_CHECK(cudaFuncSetAttribute(paged_rows_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        GPT_CHECK(cudaFuncSetAttribute(paged_rows_kernel<T, C, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       S::kSmem));
     });
     const int grid = std::min(kMaxCtas, num_sms() * S::kPerSm);
     PagedAttnArgs args = a;

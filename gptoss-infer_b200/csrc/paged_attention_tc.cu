@@ -9,14 +9,14 @@
 // released at once, so the next scores are made while this tile's exponentials run; the products are issued in the
 // order in which two halves half a step apart need them.
 //
-// Bound: the exponentials: 16 a clock and SM, 2048 cycles for 256 rows x 128 keys, against 1024 (heads of 64) and 2560
-// (heads of 128) of products. Measured, 2048 new tokens over 16384 positions, 64 query heads over 8, bf16: heads of 64
-// 668 us, 771 TFLOP/s, 46 % of the measured matrix rate: about 3100 cycles a step. Two warps of rows per scheduler do
-// not keep the special-function unit busy alone (a warp's 128 exponentials take about 1800 cycles by themselves), and
-// waits for products (about 600 cycles from weights written to their product seen) fall between. 32 heads of 128 over
-// 4: 500 us, 1031 TFLOP/s. Tried: reading the scores twice instead of holding them (1110 us), halves taking strict
-// turns at the exponentials (974 us), polling for whatever product is ready (735 us), 3 and 4 of 8 exponentials on the
-// fp32 pipes.
+// Bound: the exponentials: 16 a clock and SM, 2048 cycles for 256 rows x 128 keys, against 1024 (heads of 64) and
+// 2560 (heads of 128) of products. Measured, 2048 new tokens over 16384 positions, 64 query heads over 8, bf16:
+// heads of 64 691 us in a graph of 20 calls, 745 TFLOP/s, 45 % of the measured matrix rate (677 us at its best):
+// about 3100 cycles a step. Two warps of rows per scheduler do not keep the special-function unit busy alone (a
+// warp's 128 exponentials take about 1800 cycles by themselves), and waits for products (about 600 cycles from
+// weights written to their product seen) fall between. 32 heads of 128 over 4: 538 us, 958 TFLOP/s (510 us alone).
+// Tried: reading the scores twice instead of holding them (1110 us), halves taking strict turns at the exponentials
+// (974 us), polling for whatever product is ready (735 us), 3 and 4 of 8 exponentials on the fp32 pipes.
 //
 // Warps: 0-3 and 4-7 the rows of the two halves (softmax, rescaling, output); the next two copy keys and values through
 // a ring of tiles with TMA (a box per run of slots in a page; page sizes that are multiples of 8), or the next four
@@ -24,7 +24,7 @@
 // when the maximum has grown past kSlack (Weights in paged.cuh), so the accumulator in TMEM is rescaled rarely.
 //
 // fp32 queries: two fp16 parts of a row scaled by a power of two, and two of the weights, as in paged_attention.cu.
-// (2048 over 16384, heads of 64: 1.11 ms, 465 TFLOP/s of the sum's own operations, twice that in products.)
+// (2048 over 16384, heads of 64: 1.13 ms, 456 TFLOP/s of the sum's own operations, twice that in products.)
 #include <algorithm>
 #include <type_traits>
 
@@ -165,7 +165,8 @@ __device__ __forceinline__ float max3_nan(float x, float y, float z) {
 
 // 2^x of two values on the fp32 pipes: x = n + f with n = round(x), |f| <= 1/2 (the sum with 1.5 * 2^23 leaves n in the
 // low mantissa bits), 2^f by the polynomial of least largest relative error on [-1/2, 1/2] (weighted least squares
-// iterated to equal ripple; degree 3: 7.5e-5, degree 4: 2.6e-6), n added to its exponent. x below -126 counts as -126, and so does NaN: not for scores that are not finite.
+// iterated to equal ripple; degree 3: 7.5e-5, degree 4: 2.6e-6), n added to its exponent. x below -126 counts as
+// -126, and so does NaN: not for scores that are not finite.
 template <int DEGREE>
 __device__ __forceinline__ void exp2_pair(uint64_t x2, float& u, float& v) {
     const auto both = [](float c) { return pair(__float_as_uint(c), __float_as_uint(c)); };
@@ -862,7 +863,8 @@ void launch(const KvMaps& maps, const KvView& c, const KvBatch& b, const PagedAt
     int dev = 0;
     GPT_CHECK(cudaGetDevice(&dev));
     once.run(dev, [] {
-        GPT_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<T, C, D, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+        GPT_CHECK(cudaFuncSetAttribute(paged_tiles_kernel<T, C, D, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       L::kSmem));
     });
     PagedAttnArgs args = a;
     args.check = many_groups(b, c, a, kTile, kRows);

@@ -34,7 +34,7 @@ inline __device__ __noinline__ int countable(int n, int len, int tiles, int wind
 // Whether tokens and tables allow a head of 2^31 groups, or so many groups for a CTA (then the kernel looks).
 inline bool many_groups(const KvBatch& b, const KvView& c, const PagedAttnArgs& a, int unit, int tile_rows) {
     const double rows = std::min(double(b.tokens) * (a.q_heads / c.kv_heads), double(a.rows_to));
-    const double keys = std::min(double(b.table_stride) * c.page.d, a.window ? double(a.window) + tile_rows : 2147483648.0);
+    const double keys = std::min(double(b.most), a.window ? double(a.window) + tile_rows : 2147483648.0);
     return (rows / tile_rows + b.seqs) * (keys / unit + 3) * c.kv_heads >= 2147483648.0;
 }
 
@@ -62,7 +62,7 @@ struct Schedule {
         it.rows = min(R, it.s.n * int(group.d) - r0);
         it.p0 = it.s.len - it.s.n + int(group.div(r0));
         it.p1 = it.s.len - it.s.n + int(group.div(r0 + it.rows - 1));
-        it.lo = window ? max(0, max(it.p0, 0) - (window - 1)) & -align : 0;     // (p0 may be negative, the window 2^31 - 1)
+        it.lo = window ? max(0, max(it.p0, 0) - (window - 1)) & -align : 0;   // (p0 may be negative, window 2^31 - 1)
         it.hi = max(it.lo, it.p1 + 1);
         it.n = max(1, (it.hi - it.lo + UNIT - 1) / UNIT);
     }

@@ -267,22 +267,25 @@ int gptoss_set_prefill_packing(int mode);
 /* ---- [extension] Paged key/value cache: many sequences, prompt chunks and beams ---------------------------- */
 
 /* [extension] A pool of cache pages of `layers` layers in the caller's device memory (it must stay valid for the
- * handle's lifetime): element (layer l, page p, slot s, head h, dim d) of k and of v sits at l * strides[0] +
- * p * strides[1] + s * strides[2] + h * strides[3] + d (strides in elements, host array of 4, multiples of 8), so both
+ * handle's lifetime): element (layer l, page p, slot s, head h, dim d) of k and of v sits at l * strides[0] + p *
+ * strides[1] + s * strides[2] + h * strides[3] + d (strides in elements, host array of 4, multiples of 8), so both
  * slot-major and head-major pages are described without a copy. type: 1 = fp16, 2 = bf16. head_dim 64 or 128; any
  * page_size >= 1. A sequence's table is an int32 row of page ids: position p lives in page table[p / page_size], slot
- * p % page_size; entries past its last position are never read. The handle owns its workspaces (about 22 MB, 43 MB for
- * head_dim 128, and 20 bytes per page) and an error word: calls that use one pool must not overlap on the GPU (order its streams), and belong to the device that was
- * current at its creation. Calls allocate nothing; one captured in a graph needs the pool until its last replay. Returns NULL on failure (gptoss_last_error). Synchronizes. */
+ * p % page_size; entries past its last position are never read. The handle owns its workspaces (about 22 MB, 43 MB
+ * for head_dim 128, and 20 bytes per page) and an error word: calls that use one pool must not overlap on the GPU
+ * (order its streams), and belong to the device that was current at its creation. Calls allocate nothing; one
+ * captured in a graph needs the pool until its last replay. Returns NULL on failure (gptoss_last_error).
+ * Synchronizes. */
 typedef struct gptoss_kv_pool gptoss_kv_pool;
 gptoss_kv_pool* gptoss_kv_pool_create(void* k, void* v, int type, int layers, int num_pages, int page_size,
                                       int kv_heads, int head_dim, const long long* strides);
 void gptoss_kv_pool_destroy(gptoss_kv_pool* pool);
-/* [extension] Synchronizes, stores the pool's error word in *code and clears it. 0: every call since read valid tables
- * and lengths. Device-side data is checked on the device: 300 a page id outside the pool, 301 a length outside its
- * table or above 2^31 - 4096, 302 cu_tokens out of order, 303 a position outside the cos/sin table (or negative), 304 no
- * free page left, 305 a parent outside the sequences, 306 more attention than one call counts (a sequence whose query
- * rows times positions pass 2^38, or 2^46 where max_new was right), 310 .. 319 a bounded wait gave up. What a flagged call wrote is not meaningful
+/* [extension] Synchronizes, stores the pool's error word in *code and clears it. 0: every call since read valid
+ * tables and lengths. Device-side data is checked on the device: 300 a page id outside the pool, 301 a length outside
+ * its table or above 2^31 - 4096, 302 cu_tokens out of order, 303 a position outside the cos/sin table (or negative),
+ * 304 no free page left, 305 a parent outside the sequences, 306 more attention than one call counts (a sequence
+ * whose query rows times positions pass 2^38, or 2^46 where max_new was right), 310 .. 319 a bounded wait gave up
+ * (destroy the pool: its workspaces are not as the kernels leave them). What a flagged call wrote is not meaningful
  * for the sequences concerned; nothing outside the given arrays is touched. */
 int gptoss_kv_pool_status(gptoss_kv_pool* pool, int* code);
 
@@ -311,16 +314,16 @@ int gptoss_kv_append(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* bat
 
 /* [extension] Causal attention of a batch's new tokens over the cache (their own keys and values appended before),
  * asynchronous on `stream`: out[t][h] = sum_j w_j v_j / (sum_j w_j + exp(sinks[h])), w_j = exp(scale q.k_j), over the
- * positions j <= p of the token at p, and j > p - window with window > 0. Query head h reads key/value head
- * h / (q_heads / kv_heads). sinks: fp32 [q_heads] or NULL (no sink term). q and out: [tokens] rows of q_heads *
- * head_dim, q_stride and out_stride elements apart, 16-byte aligned, of the cache's type, or fp32 beside an fp16 cache
- * (queries and weights then in two fp16 parts, about 22 bits). The weights of the second product are rounded to the
- * cache's type; beside an fp16 cache to 2^-38 of the row's largest weight where that is more. scale: finite, not 0. Statistics and sums are fp32. A row that sees no key is 0,
- * and what a row may not see does not reach it, NaN and infinities included; a score of NaN or +infinity that it sees
- * makes it NaN (with fp32 queries an infinite key does). Results do not depend on timing.
- * Sequences of up to 64 query rows (new tokens x q_heads / kv_heads; 16 for head_dim 128) run on one kernel, longer
- * chunks on another; a batch with both takes two launches. Page sizes that are multiples of 8 are the fast ones for
- * chunks. */
+ * positions j <= p of the token at p, and j > p - window with window > 0. Query head h reads key/value head h /
+ * (q_heads / kv_heads). sinks: fp32 [q_heads] or NULL (no sink term). q and out: [tokens] rows of q_heads * head_dim,
+ * q_stride and out_stride elements apart, 16-byte aligned, of the cache's type, or fp32 beside an fp16 cache (queries
+ * and weights then in two fp16 parts, about 22 bits). The weights of the second product are rounded to the cache's
+ * type; beside an fp16 cache to 2^-38 of the row's largest weight where that is more. scale: finite, not 0.
+ * Statistics and sums are fp32. A row that sees no key is 0, and what a row may not see does not reach it, NaN and
+ * infinities included; a score of NaN or +infinity that it sees makes it NaN (with fp32 queries an infinite key
+ * does). Results do not depend on timing. out must not overlap q. Sequences of up to 64 query rows (new tokens x
+ * q_heads / kv_heads; 16 for head_dim 128) run on one kernel, longer chunks on another; a batch with chunks takes two
+ * launches unless all its sequences have max_new. Page sizes that are multiples of 8 are the fast ones for chunks. */
 int gptoss_paged_attention(gptoss_kv_pool* pool, int layer, const gptoss_kv_batch* batch, const void* q, int type,
                            long long q_stride, int q_heads, const float* sinks, float scale, int window, void* out,
                            long long out_stride, void* stream);
@@ -348,16 +351,17 @@ int gptoss_kv_compact(gptoss_kv_pool* pool, const int32_t* refs, const int32_t* 
                       int table_stride, int32_t* refs_out, int32_t* tables_out, int32_t* remap, int32_t* live,
                       void* stream);
 
-/* [extension] Beam selection, asynchronous on `stream`: for each of `batch` requests the best `picks` (1 .. 64) of its
- * beams (1 .. 64) x vocab candidates, score = scores[row] + log softmax(logits[row])[token], best first, equal scores
- * to the lower row, then the lower token. logits: [batch * beams] rows of vocab, row_stride elements apart, type 0 =
- * fp32, 1 = fp16, 2 = bf16; scores fp32 [batch * beams]. done (NULL, or uint8 [batch * beams]): a finished row's only
- * candidate is done_token, at scores[row]. A NaN logit counts as -inf; candidates of score -inf are not picked, and
- * places without a candidate get score -inf, row -1, token -1. Outputs [batch][picks]: out_scores fp32, rows (of
- * logits, so they serve as gptoss_kv_fork's parents), tokens. Sums and ranking use fp32 statistics and fp64 scores.
- * Uses the calling thread's workspace: calls from one thread must not overlap on the GPU, and the first call at a
- * larger size allocates (make it before a stream capture). A captured call goes on using the workspace of the thread
- * that captured it, whatever larger calls follow: its replays count among that thread's calls and end before it does. */
+/* [extension] Beam selection, asynchronous on `stream`: for each of `batch` requests the best `picks` (1 .. 64) of
+ * its beams (1 .. 64) x vocab candidates, score = scores[row] + log softmax(logits[row])[token], best first, equal
+ * scores to the lower row, then the lower token. logits: [batch * beams] rows of vocab, row_stride elements apart,
+ * type 0 = fp32, 1 = fp16, 2 = bf16; scores fp32 [batch * beams]. done (NULL, or uint8 [batch * beams]): a finished
+ * row's only candidate is done_token, at scores[row]. A NaN logit counts as -inf; candidates of score -inf are not
+ * picked, and places without a candidate get score -inf, row -1, token -1. Outputs [batch][picks]: out_scores fp32,
+ * rows (of logits, so they serve as gptoss_kv_fork's parents), tokens. Sums and ranking use fp32 statistics and fp64
+ * scores. Uses the calling thread's workspace: calls from one thread must not overlap on the GPU, and the first call
+ * at a larger size allocates (make it before a stream capture). A captured call goes on using the workspace of the
+ * thread that captured it, whatever larger calls follow: its replays count among that thread's calls and end before
+ * it does. */
 int gptoss_beam_select(const void* logits, int type, long long row_stride, const float* scores, const uint8_t* done,
                        int done_token, int batch, int beams, int vocab, int picks, float* out_scores, int32_t* rows,
                        int32_t* tokens, void* stream);

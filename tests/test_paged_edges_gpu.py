@@ -164,8 +164,8 @@ def test_lengths_up_to_31_bits(lib, new):
     """2048 pages of 2^20 slots that are all one page in memory: 2^31 - 4096 positions are right, more are flagged."""
     page, most, W = 1 << 20, (1 << 31) - 4096, 100
     g = torch.Generator(device="cuda").manual_seed(52)
-    k, v = (torch.randn(page, 1, 64, device="cuda", generator=g).half().as_strided((1, 2048, page, 1, 64), (0, 0, 64, 64, 1))
-            for _ in range(2))
+    k, v = (torch.randn(page, 1, 64, device="cuda", generator=g).half() for _ in range(2))
+    k, v = (x.as_strided((1, 2048, page, 1, 64), (0, 0, 64, 64, 1)) for x in (k, v))
     s = Setup.__new__(Setup)
     s.pool, s.T, s.kvh = Pool(lib, k, v), new, 1
     s.cu, s.dlens, s.dtab = ints([0, new]), ints([most]), ints([list(range(2048))])
@@ -183,10 +183,13 @@ def test_lengths_up_to_31_bits(lib, new):
     # room past 2^31 - 4096 is not given
     refs, lens = ints([0] * 2048), ints([most - 5])
     tables, lens_out, refs_out = torch.empty(1, 2048, dtype=torch.int32, device="cuda"), ints([7]), ints([0] * 2048)
+    parent, room = ints([0]), ints([0])
     for extra, want, code in ((5, most, 0), (6, most, 301), ((1 << 31) - 1, most, 301)):
-        assert lib.gptoss_kv_fork(s.pool.h, refs.fill_(1).data_ptr(), s.dtab.data_ptr(), lens.data_ptr(), 1, ints([0]).data_ptr(),
-                                  ints([extra]).data_ptr(), 1, 2048, refs_out.data_ptr(), tables.data_ptr(),
-                                  lens_out.data_ptr(), stream()) == 0
+        refs.fill_(1)
+        room.fill_(extra)
+        ok(lib, lib.gptoss_kv_fork(s.pool.h, refs.data_ptr(), s.dtab.data_ptr(), lens.data_ptr(), 1, parent.data_ptr(),
+                                   room.data_ptr(), 1, 2048, refs_out.data_ptr(), tables.data_ptr(), lens_out.data_ptr(),
+                                   stream()))
         assert s.pool.status() == code and lens_out.item() == want
 
 
@@ -312,7 +315,7 @@ def test_fork_of_children_that_ask_for_more_than_31_bits_of_pages(lib):
     k, v = make_pages(1, 6, 1, 1, 64, F16, False, 3)
     pool = Pool(lib, k, v)
     refs, tables, lens = ints([0, 0, 1, 0, 0, 0]), torch.full((1, room), 2, dtype=torch.int32, device="cuda"), ints([1])
-    out, lens_out = torch.empty(n, room, dtype=torch.int32, device="cuda"), torch.empty(n, dtype=torch.int32, device="cuda")
+    out, lens_out = (torch.empty(shape, dtype=torch.int32, device="cuda") for shape in ((n, room), (n,)))
     parents, extra = ints([0] * n), ints([room - 1] * n)
     ok(lib, lib.gptoss_kv_fork(pool.h, refs.data_ptr(), tables.data_ptr(), lens.data_ptr(), 1, parents.data_ptr(),
                                extra.data_ptr(), n, room, refs.data_ptr(), out.data_ptr(), lens_out.data_ptr(), stream()))
@@ -403,6 +406,6 @@ def test_a_failed_allocation_does_not_fail_the_next_call(lib):
     assert lib.gptoss_beam_select(x.data_ptr(), 0, wide, s.data_ptr(), None, 0, 1 << 16, 64, wide, 64, p, p, p,
                                   stream()) == -1
     t.zero_()
-    ok(lib, lib.gptoss_paged_attention(pool.h, 0, ctypes.byref(b), q.data_ptr(), 1, 512, 8, None, 0.125, 0, out.data_ptr(),
-                                       512, stream()))
+    ok(lib, lib.gptoss_paged_attention(pool.h, 0, ctypes.byref(b), q.data_ptr(), 1, 512, 8, None, 0.125, 0,
+                                       out.data_ptr(), 512, stream()))
     assert pool.status() == 0 and torch.equal(out, v[0, 0, 0].expand(1, 8, 64))
