@@ -354,14 +354,15 @@ paged_rows_kernel(KvView c, KvBatch b, PagedAttnArgs a, FastDiv group, int* coun
                     top[nt][e] = fmaxf(s[0][nt][e], s[0][nt][2 + e]);
 #pragma unroll
                     for (int x = 1; x < KT; ++x) top[nt][e] = fmaxf(top[nt][e], fmaxf(s[x][nt][e], s[x][nt][2 + e]));
-                    past |= top[nt][e] > m[nt][e] + (W::kLift + W::kSlack);
+                    past |= top[nt][e] - m[nt][e] > W::kLift + W::kSlack;
                 }
+            // (as the weights' exponents are computed, and the reference rounded up: no weight is larger than meant)
             if (__any_sync(kFull, past)) {            // move the references: kLift below the rows' maxima so far
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mm = fmaxf(m[nt][e], top[nt][e] - W::kLift);
+                        float mm = fmaxf(m[nt][e], __fsub_ru(top[nt][e], W::kLift));
 #pragma unroll
                         for (int z = 4; z < 32; z <<= 1) mm = fmaxf(mm, __shfl_xor_sync(kFull, mm, z));
                         const float f = ex2(m[nt][e] - (mm == -INFINITY ? 0.f : mm));

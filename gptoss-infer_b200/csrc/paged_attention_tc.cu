@@ -696,10 +696,12 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
 #pragma unroll
                     for (int i = 0; i < SK; i += 2)
                         top4[i / 2 & 3] = max3_nan(top4[i / 2 & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                    const float top = max3_nan(top4[0], top4[1], max3_nan(top4[2], top4[3], top4[3])) * sc;
-                    const bool past = top > m + (W::kLift + W::kSlack);
+                    const float top = max3_nan(top4[0], top4[1], max3_nan(top4[2], top4[3], top4[3]));
+                    // as the weights' own exponents are computed, and the reference rounded up: no weight is larger
+                    // than meant, however large the scores
+                    const bool past = fmaf(top, sc, -m) > W::kLift + W::kSlack;
                     if (__any_sync(kFull, past)) {
-                        const float mm = past ? top - W::kLift : m, f = past ? ex2(m - mm) : 1.f;
+                        const float mm = past ? __fmaf_ru(top, sc, -W::kLift) : m, f = past ? ex2(m - mm) : 1.f;
                         if (g > g0 * SUB) {
                             good = all_ok(tc::mbar_wait(&bars[kPvDone + t], (step - 1) & 1, err, kKvWait + 1));
                             if (!good) break;
@@ -724,7 +726,7 @@ paged_tiles_kernel(const __grid_constant__ KvMaps maps, KvView c, KvBatch b, Pag
                     const uint32_t p_at = p_col(t, 0) + lanes, p_low = p_col(t, 1) + lanes;
                     // a row without a key so far needs exact zeros, and one with a score of NaN or +infinity (which make
                     // it NaN) the exponential that keeps them
-                    if (L::kSplit || edge || __any_sync(kFull, m == -INFINITY || !(top < INFINITY)))
+                    if (L::kSplit || edge || __any_sync(kFull, m == -INFINITY || !(top * sc < INFINITY)))
                         l += weights<C, L::kSplit, false, SK>(x, sc, -base, p_at, p_low);
                     else
                         l += weights<C, L::kSplit, true, SK>(x, sc, -base, p_at, p_low);

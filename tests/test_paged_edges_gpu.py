@@ -57,6 +57,35 @@ def test_attention_beside_a_dominant_key(lib, new, length, dim, page, pair, rest
 
 
 @pytest.mark.parametrize("pair", PAIRS, ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 20)])
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("power", range(17, 25))
+def test_attention_scores_in_the_millions(lib, power, new, dim, page, pair):
+    """Scores near 2^power, where fp32 steps by up to 2: a second large key, some tiles on, lies 1 to 4 above the first,
+    about the distance at which weights are rescaled. Nothing overflows.
+
+    Bound: a score's rounding (three of them: product, scale, difference) is 3 steps of 2^(power - 22) at most, and the
+    first key's share 1 / (1 + exp(difference)) has a slope of 1/4 at most; 0.01 for weights and outputs of 8 bits."""
+    n, length = 64, 400
+    s = Setup(lib, [new] * n, [length] * n, page=page, kvh=1, dim=dim, dtype=pair[1], seed=41)
+    for b in range(n):
+        keys, values = torch.zeros(length, 1, dim, device="cuda"), torch.zeros(length, 1, dim, device="cuda")
+        keys[[3, 200 + b], 0, 0] = 2048.0
+        keys[200 + b, 0, 1] = 1 + b * 3 / 64
+        values[3, 0, 0], values[200 + b, 0, 1] = 1.0, 1.0
+        set_kv(s, b, np.arange(length), keys, values)
+    q = torch.zeros(s.T, 8, dim, device="cuda", dtype=pair[0])
+    q[:, :, 0], q[:, :, 1] = 2.0 ** (power - 11), 1.0
+    out = run_attention(lib, s, q, scale=1.0)
+    assert torch.isfinite(out).all()
+    first, later = out[:, :, 0].float(), out[:, :, 1].float()
+    assert ((first + later - 1).abs() <= 0.01).all() and (first >= 0).all() and (later >= 0).all()
+    above = torch.stack([k[200 + b, 0, 1].double() for b, k in enumerate(s.keys)]).repeat_interleave(new)
+    share = (1 / (1 + above.exp())).float()[:, None]
+    assert ((first - share).abs() <= 0.01 + 0.75 * 2.0 ** (power - 22)).all()
+
+
+@pytest.mark.parametrize("pair", PAIRS, ids=["f32", "f16", "bf16"])
 @pytest.mark.parametrize("dim,page", [(64, 16), (64, 20), (128, 16), (128, 20)])
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("where", [0, 128])
