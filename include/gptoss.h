@@ -292,7 +292,8 @@ int gptoss_kv_pool_status(gptoss_kv_pool* pool, int* code);
 /* [extension] A batch of sequences with their new tokens. Sequence b owns rows cu_tokens[b] .. cu_tokens[b + 1) of
  * the batch (none, one or many); kv_lens[b] counts its cached positions with these new ones, so its row i stands at
  * position kv_lens[b] - new + i. tables: int32 [seqs][table_stride]. Device pointers. max_new: an upper bound on the
- * new tokens of one sequence, as the host knows it: it only steers the choice of kernel. */
+ * new tokens of one sequence, as the host knows it: it only steers the choice of kernel. Rows of no sequence are left
+ * as they are. */
 typedef struct {
     int32_t seqs, tokens, max_new, table_stride;
     const int32_t* cu_tokens;                /* [seqs + 1], cu_tokens[0] = 0, cu_tokens[seqs] = tokens */

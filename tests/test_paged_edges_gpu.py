@@ -1,5 +1,6 @@
-"""Paged key/value cache operators where they are easily wrong: shared last pages, rows that a few keys dominate, values
-that are not finite, zeros of both signs. Helpers and tolerances: test_paged_gpu.py."""
+"""Paged key/value cache operators where they are easily wrong: shared last pages, rows that a few keys dominate, scores
+and values that are not finite or very large, lengths and sums near 2^31, zeros of both signs, failed calls and captured
+ones. Helpers and tolerances: test_paged_gpu.py."""
 import ctypes
 
 import numpy as np
@@ -220,6 +221,26 @@ def test_lengths_up_to_31_bits(lib, new):
                                    room.data_ptr(), 1, 2048, refs_out.data_ptr(), tables.data_ptr(), lens_out.data_ptr(),
                                    stream()))
         assert s.pool.status() == code and lens_out.item() == want
+
+
+@pytest.mark.parametrize("most", [1, 200])
+def test_rows_of_no_sequence_are_left_as_they_are(lib, most):
+    """A batch padded to more tokens than its sequences have, before the first and behind the last."""
+    s = Setup(lib, [1, 100], [30, 120], page=16, kvh=1, dim=64, dtype=F16, seed=56)
+    cu = ints([3, 4, 104])
+    q, out = new_q(110, 8, 64, F16), torch.full((110, 8, 64), 7.0, device="cuda", dtype=F16)
+    s.batch.cu_tokens, s.batch.tokens = cu.data_ptr(), 110
+    run_attention(lib, s, q, max_new=most, out=out)
+    want, mag = reference_attention(s, q[3:104], None, 0.125, 0)
+    check_attention(out[3:104], want, mag)
+    assert (out[:3] == 7).all() and (out[104:] == 7).all()
+    x, q_out = torch.ones(110, 10 * 64, device="cuda"), torch.full((110, 8, 64), 7.0, device="cuda")
+    cos = torch.ones(120, 32, device="cuda")
+    p = x.data_ptr()
+    ok(lib, lib.gptoss_kv_append(s.pool.h, 0, ctypes.byref(s.batch), p, p + 8 * 256, p + 9 * 256, 0, 640, 640, 8,
+                                 cos.data_ptr(), cos.data_ptr(), 120, 64, 0, q_out.data_ptr(), 0, stream()))
+    assert (q_out[:3] == 7).all() and (q_out[104:] == 7).all() and (q_out[3:104] != 7).all()
+    assert s.pool.status() == 0
 
 
 def test_status_loses_no_report_of_the_next_call(lib):
